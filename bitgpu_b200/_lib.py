@@ -22,7 +22,8 @@ EXPORTS = [
     "bg_deltanet_chunked", "bg_qk_norm_rope", "bg_conv1d_causal", "bg_slice_cols",
     "bg_kv_snapshot_bytes", "bg_kv_snapshot_save", "bg_kv_snapshot_restore", "bg_attention_noalloc_limit",
     "bg_selftest_wait_expiry", "bg_kv_append_kv_pair", "bg_peer_exchange_bytes", "bg_peer_exchange_flags_offset",
-    "bg_attention_peer_workspace_size", "bg_attention_peer",
+    "bg_attention_peer_workspace_size", "bg_attention_peer", "bg_paged_append", "bg_paged_attention_workspace_size",
+    "bg_paged_attention",
 ]
 
 
@@ -44,6 +45,21 @@ class PeerExchange(C.Structure):
     _fields_ = [("nranks", C.c_uint32), ("rank", C.c_uint32), ("gather", C.c_void_p * MAX_PEERS),
                 ("flags", C.c_void_p * MAX_PEERS), ("step", C.c_void_p), ("done", C.c_void_p),
                 ("tickets", C.c_void_p), ("spin_limit", C.c_uint32)]
+
+
+class PagedCacheDesc(C.Structure):
+    _fields_ = [("K", C.c_void_p), ("V", C.c_void_p), ("Ks", C.c_void_p), ("Vs", C.c_void_p),
+                ("num_pages", C.c_uint64), ("page_size", C.c_uint32), ("mode", C.c_uint32)]
+
+
+class PagedBatchDesc(C.Structure):
+    _fields_ = [("cu_q", C.c_void_p), ("kv_len", C.c_void_p), ("page_table", C.c_void_p), ("prefix_pages", C.c_void_p),
+                ("batch", C.c_uint32), ("tokens", C.c_uint32), ("max_q", C.c_uint32), ("table_stride", C.c_uint32),
+                ("prefix_len", C.c_uint32)]
+
+
+class Rows(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("token_stride", C.c_uint64), ("head_stride", C.c_uint64)]
 
 
 class BgError(RuntimeError):
@@ -94,6 +110,11 @@ _SIGS = {
     "bg_attention_peer": (C.c_int, [C.POINTER(AttnParams), U32, P, U32, C.POINTER(KVCacheDesc), F, U32, U32,
                                     C.POINTER(PeerExchange), P, P, U32, P, SZ, P]),
     "bg_selftest_wait_expiry": (C.c_int, [U32, P]),
+    "bg_paged_append": (C.c_int, [C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), U32, U32, U32, C.POINTER(Rows),
+                                  C.POINTER(Rows), C.POINTER(Rows), U32, P, P, F, P, P, U32, U32, P, U32, P]),
+    "bg_paged_attention_workspace_size": (SZ, [C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), U32, U32, U32]),
+    "bg_paged_attention": (C.c_int, [C.POINTER(PagedCacheDesc), C.POINTER(PagedBatchDesc), U32, U32, U32, P, U32, F, P,
+                                     P, U32, P, SZ, P]),
     "bg_attention_noalloc": (C.c_int, [C.POINTER(AttnParams), U32, P, U32, C.POINTER(KVCacheDesc), P, P, F, P, P,
                                        U32, P]),
 }

@@ -5,6 +5,7 @@
 
 #include "attn.h"
 #include "kv.h"
+#include "paged.h"
 #include "prefill.h"
 
 using namespace bg;
@@ -283,6 +284,7 @@ int bg_device_status(bg_stream_t stream) {
   if (!e) e = poll_device_error_deltanet();
   if (!e) e = poll_device_error_dnchunk();
   if (!e) e = poll_device_error_peer();
+  if (!e) e = poll_device_error_paged();
   return e ? (e < 0 ? e : BG_ELAUNCH) : BG_OK;
 }
 

@@ -1,0 +1,139 @@
+// extern "C" entry points of the paged-cache operators: argument checks and the choice of kernels.
+#include <math.h>
+
+#include "paged.h"
+
+using namespace bg;
+
+namespace {
+
+bool d_ok(uint32_t D) { return D == 64 || D == 128 || D == 256; }
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+int check_paged(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t KV, uint32_t D) {
+  if (!kv || !b || KV == 0) return BG_EINVAL;
+  if (!d_ok(D)) return BG_EUNSUPPORTED;
+  if (kv->mode == BG_KV_Q8R) return BG_EUNSUPPORTED;
+  if (kv->mode > BG_KV_Q8R) return BG_EINVAL;
+  if (!kv->K || !kv->V || !aligned16(kv->K) || !aligned16(kv->V)) return BG_EINVAL;
+  if (kv->mode == BG_KV_Q8 && (!kv->Ks || !kv->Vs || !aligned16(kv->Ks) || !aligned16(kv->Vs))) return BG_EINVAL;
+  if (kv->num_pages == 0 || kv->num_pages > 0x7fffffffull || kv->page_size == 0) return BG_EINVAL;
+  if (b->batch == 0 || b->tokens == 0) return BG_OK;
+  if (!b->kv_len || !b->page_table || b->table_stride == 0 || b->max_q == 0) return BG_EINVAL;
+  if (!b->cu_q && b->tokens != b->batch) return BG_EINVAL;
+  if (b->batch > 0x7ffffffeu || b->tokens > 0x7fffffffu) return BG_EINVAL;
+  if (b->prefix_len && !b->prefix_pages) return BG_EINVAL;
+  if ((uint64_t)b->table_stride * kv->page_size + b->prefix_len > 0x7fffffffull) return BG_EINVAL;
+  return BG_OK;
+}
+
+PagedView view(const bg_paged_cache *kv, uint32_t KV) {
+  return PagedView{kv->K, kv->V, kv->Ks, kv->Vs, (uint32_t)kv->num_pages, kv->page_size, KV};
+}
+
+BatchView view(const bg_paged_batch *b) {
+  return BatchView{b->cu_q, b->kv_len, b->page_table, b->prefix_pages, b->batch, b->tokens, b->table_stride,
+                   b->prefix_len};
+}
+
+// How a call's partial rows are laid out: o [rows][D] f32, then ml [rows] float2.
+struct Plan {
+  uint32_t nsplit;     // CUDA-core kernel: splits of every row
+  uint64_t part_rows;  // partial rows
+};
+
+Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, uint32_t KV, uint32_t D) {
+  Plan p;
+  p.nsplit = paged_generic_splits(b->tokens, H, KV, (uint64_t)b->table_stride * kv->page_size + b->prefix_len);
+  p.part_rows = p.nsplit > 1 ? (uint64_t)p.nsplit * b->tokens * H : 0;
+  return p;
+}
+
+}  // namespace
+
+namespace bg {
+int poll_device_error_paged() {
+  int e = poll_device_error_paged_append();
+  if (!e) e = poll_device_error_paged_generic();
+  return e;
+}
+}  // namespace bg
+
+extern "C" {
+
+int bg_paged_append(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV, uint32_t D,
+                    const bg_rows *q, const bg_rows *k, const bg_rows *v, uint32_t src_dtype, const float *q_gamma,
+                    const float *k_gamma, float eps, const float *cosT, const float *sinT, uint32_t rot,
+                    uint32_t table_rows, void *q_out, uint32_t q_out_dtype, bg_stream_t stream) {
+  if (int rc = check_paged(kv, batch, KV, D)) return rc;
+  if (!k || !v || !k->x || !v->x || src_dtype > BG_DT_F16 || q_out_dtype > BG_DT_F16) return BG_EINVAL;
+  if (q && (!q->x || !q_out || H == 0 || !aligned16(q_out))) return BG_EINVAL;
+  if ((cosT == nullptr) != (sinT == nullptr)) return BG_EINVAL;
+  if (cosT && (rot == 0 || rot % 2 || rot > D || !aligned16(cosT) || !aligned16(sinT))) return BG_EINVAL;
+  if (batch->batch == 0 || batch->tokens == 0) return BG_OK;
+  PagedAppendArgs a;
+  a.kv = view(kv, KV);
+  a.bv = view(batch);
+  a.mode = (int)kv->mode;
+  a.src_f16 = src_dtype == BG_DT_F16;
+  a.out_f16 = q_out_dtype == BG_DT_F16;
+  a.H = q ? H : 0;
+  a.D = D;
+  a.rot = cosT ? rot : 0;
+  a.table_rows = table_rows;
+  a.q = q ? q->x : nullptr;
+  a.q_ts = q ? q->token_stride : 0;
+  a.q_hs = q ? q->head_stride : 0;
+  a.k = k->x;
+  a.k_ts = k->token_stride;
+  a.k_hs = k->head_stride;
+  a.v = v->x;
+  a.v_ts = v->token_stride;
+  a.v_hs = v->head_stride;
+  a.q_gamma = q_gamma;
+  a.k_gamma = k_gamma;
+  a.cosT = cosT;
+  a.sinT = sinT;
+  a.eps = eps;
+  a.q_out = q_out;
+  return launch_paged_append(a, (cudaStream_t)stream);
+}
+
+size_t bg_paged_attention_workspace_size(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV,
+                                         uint32_t D) {
+  if (check_paged(kv, batch, KV, D) || H == 0 || H % KV || batch->batch == 0 || batch->tokens == 0) return 0;
+  return (size_t)make_plan(kv, batch, H, KV, D).part_rows * (D + 2) * sizeof(float);
+}
+
+int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV, uint32_t D,
+                       const void *q, uint32_t q_dtype, float scale, const float *gate, void *out, uint32_t out_dtype,
+                       void *workspace, size_t workspace_bytes, bg_stream_t stream) {
+  if (int rc = check_paged(kv, batch, KV, D)) return rc;
+  if (H == 0 || H % KV || q_dtype > BG_DT_F16 || out_dtype > BG_DT_F16) return BG_EINVAL;
+  if (batch->batch == 0 || batch->tokens == 0) return BG_OK;
+  if (!q || !out || !aligned16(q) || !aligned16(out) || !aligned16(gate) || !aligned16(workspace)) return BG_EINVAL;
+  const Plan plan = make_plan(kv, batch, H, KV, D);
+  const size_t need = (size_t)plan.part_rows * (D + 2) * sizeof(float);
+  if (need && (!workspace || workspace_bytes < need)) return BG_ENOMEM;
+  PagedAttnArgs a;
+  a.kv = view(kv, KV);
+  a.bv = view(batch);
+  a.mode = (int)kv->mode;
+  a.q_f16 = q_dtype == BG_DT_F16;
+  a.out_f16 = out_dtype == BG_DT_F16;
+  a.H = H;
+  a.G = H / KV;
+  a.D = D;
+  a.max_q = batch->max_q;
+  a.sl2 = (scale > 0.f ? scale : 1.0f / sqrtf((float)D)) * kLog2e;
+  a.q = q;
+  a.gate = gate;
+  a.out = out;
+  a.part_o = static_cast<float *>(workspace);
+  a.part_ml = reinterpret_cast<float2 *>(a.part_o + plan.part_rows * D);
+  a.part_rows = plan.part_rows;
+  return launch_paged_generic(a, plan.nsplit, (cudaStream_t)stream);
+}
+
+}  // extern "C"

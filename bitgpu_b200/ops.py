@@ -4,7 +4,8 @@ Each function launches the sm_100a kernels of ``libbgattn.so`` through its C ABI
 torch CUDA stream.  Names follow the reference engine (``src/engine.ts``): ``KVCache.append``
 is ``appendKV`` (engine.ts:1385-1393), ``KVCache.evict`` is ``evict`` (:1188-1212),
 ``attention`` is the ATT dispatch (:1543 / :1580 / :1487-1491), ``deltanet_*`` are the
-hybrid-layer dispatches (:1438-1462).  Errors surface as ``BgError`` (the engine throws);
+hybrid-layer dispatches (:1438-1462).  ``PagedKVCache``, ``PagedBatch``, ``paged_append`` and
+``paged_attention`` serve ragged batches from one page pool (no reference counterpart).  Errors surface as ``BgError`` (the engine throws);
 nothing here falls back to a CPU or torch implementation.
 """
 import ctypes as C
@@ -12,7 +13,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import AttnParams, KVCacheDesc, check, lib
+from ._lib import AttnParams, KVCacheDesc, PagedBatchDesc, PagedCacheDesc, Rows, check, lib
 
 MODES = {"f32": _lib.KV_F32, "f16": _lib.KV_F16, "q8": _lib.KV_Q8, "q8r": _lib.KV_Q8R}
 _DT = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16}
@@ -321,6 +322,224 @@ def gate_sigmoid(x, gate):
     y = torch.empty_like(x)
     check("bg_gate_sigmoid", lib().bg_gate_sigmoid(_p(x), _p(gate), x.numel(), _p(y), _stream()))
     return y
+
+
+class PagedKVCache:
+    """One layer's K/V pool for many sequences: ``num_pages`` pages of ``page_size`` positions, each
+    ``[kv_head][head_dim]`` in the codec of ``mode`` ('f32' | 'f16' | 'q8').  Which pages belong to
+    which sequence is a ``PagedBatch``'s page table.  ``from_tensors`` wraps a pool that the caller
+    allocated."""
+
+    def __init__(self, num_pages, page_size, kv_heads, head_dim, mode="f16", device="cuda"):
+        if mode not in MODES or mode == "q8r":
+            raise ValueError(f"paged caches are 'f32', 'f16' or 'q8', got {mode!r}")
+        if num_pages < 1 or page_size < 1 or kv_heads < 1:
+            raise ValueError("num_pages, page_size and kv_heads must be positive")
+        shape = (num_pages, page_size, kv_heads, head_dim)
+        dt = {"f32": torch.float32, "f16": torch.float16, "q8": torch.int8}[mode]
+        ks = vs = None
+        if mode == "q8":
+            if head_dim % 32:
+                raise ValueError("q8 KV needs head_dim % 32 == 0")
+            ks, vs = (torch.zeros(shape[:3] + (head_dim // 32,), dtype=torch.float32, device=device) for _ in "kv")
+        self._set(torch.zeros(shape, dtype=dt, device=device), torch.zeros(shape, dtype=dt, device=device), ks, vs)
+
+    @classmethod
+    def from_tensors(cls, K, V, Ks=None, Vs=None):
+        """Wrap ``K, V [num_pages, page_size, kv_heads, head_dim]`` (f32, f16, or int8 codes with
+        their block scales ``Ks, Vs [num_pages, page_size, kv_heads, head_dim / 32]``)."""
+        self = cls.__new__(cls)
+        self._set(K, V, Ks, Vs)
+        return self
+
+    def _set(self, K, V, Ks, Vs):
+        modes = {torch.float32: "f32", torch.float16: "f16", torch.int8: "q8"}
+        if K.dtype not in modes:
+            raise ValueError(f"K must be float32, float16 or int8, got {K.dtype}")
+        if K.dim() != 4 or 0 in K.shape:
+            raise ValueError("K must be [num_pages, page_size, kv_heads, head_dim]")
+        self.mode = modes[K.dtype]
+        _need(K, name="K")
+        _need(V, K.dtype, "V")
+        if V.shape != K.shape or V.device != K.device:
+            raise ValueError("K and V must have one shape and device")
+        if (self.mode == "q8") != (Ks is not None) or (Ks is None) != (Vs is None):
+            raise ValueError("q8 pools, and only they, have block scales Ks and Vs")
+        if Ks is not None:
+            for t, name in ((Ks, "Ks"), (Vs, "Vs")):
+                _need(t, torch.float32, name)
+                if t.shape != K.shape[:3] + (K.shape[3] // 32,) or K.shape[3] % 32 or t.device != K.device:
+                    raise ValueError(f"{name} must be [num_pages, page_size, kv_heads, head_dim / 32] beside K")
+        self.K, self.V, self.Ks, self.Vs = K, V, Ks, Vs
+        self.num_pages, self.page_size, self.KV, self.D = K.shape
+        self.device = K.device
+        self._desc = PagedCacheDesc(K.data_ptr(), V.data_ptr(), Ks.data_ptr() if Ks is not None else None,
+                                    Vs.data_ptr() if Vs is not None else None, self.num_pages, self.page_size,
+                                    MODES[self.mode])
+
+    def desc(self):
+        return self._desc
+
+
+class PagedBatch:
+    """Which token rows belong to which sequence, and where each sequence's positions live.
+
+    ``page_table[batch, width]`` (int32) lists every sequence's pages, ``kv_len[batch]`` (int32) its
+    own positions with the new tokens among them, ``cu_q[batch + 1]`` (int32) the first token row of
+    each sequence (None: one token each).  ``tokens``: rows of q / k / v, the padding behind
+    ``cu_q[-1]`` included; ``max_q``: the largest number of tokens of a sequence (selects kernels).
+    A prefix that all sequences share lives in ``prefix_pages`` (int32) and has ``prefix_len``
+    positions, in front of the own ones.
+
+    The tensors are read on the device at every call: a decode loop updates them in place, and a
+    captured graph follows them."""
+
+    def __init__(self, page_table, kv_len, cu_q=None, tokens=None, max_q=1, prefix_pages=None, prefix_len=0):
+        given = (("page_table", page_table, 2), ("kv_len", kv_len, 1), ("cu_q", cu_q, 1), ("prefix_pages", prefix_pages, 1))
+        for name, t, dim in given:
+            if t is None:
+                continue
+            _need(t, torch.int32, name)
+            if t.dim() != dim:
+                raise ValueError(f"{name} must have {dim} dimension(s)")
+            if t.device != page_table.device:
+                raise ValueError("the batch's tensors must be on one device")
+        B, width = page_table.shape
+        if kv_len.numel() != B or (cu_q is not None and cu_q.numel() != B + 1):
+            raise ValueError("kv_len has one entry per row of page_table, cu_q one more")
+        if cu_q is None:
+            if tokens not in (None, B) or max_q != 1:
+                raise ValueError("without cu_q every sequence has one token")
+            tokens = B
+        elif tokens is None:
+            raise ValueError("tokens is needed beside cu_q")
+        if tokens < 0 or max_q < 1 or prefix_len < 0:
+            raise ValueError("tokens and prefix_len must not be negative, max_q must be positive")
+        if prefix_len and prefix_pages is None:
+            raise ValueError("prefix_len needs prefix_pages")
+        self.page_table, self.kv_len, self.cu_q, self.prefix_pages = page_table, kv_len, cu_q, prefix_pages
+        self.batch, self.tokens, self.max_q, self.prefix_len = B, tokens, max_q, prefix_len
+        self.device = page_table.device
+        self._desc = PagedBatchDesc(_ptr(cu_q), kv_len.data_ptr(), page_table.data_ptr(), _ptr(prefix_pages), B, tokens,
+                                    max_q, width, prefix_len)
+        self._ws = {}
+
+    def desc(self):
+        return self._desc
+
+    def _fits(self, cache):
+        if cache.device != self.device:
+            raise ValueError("the cache and the batch must be on one device")
+        if self.prefix_len and self.prefix_pages.numel() * cache.page_size < self.prefix_len:
+            raise ValueError("prefix_pages holds fewer than prefix_len positions")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream_of(device):
+    """The current stream of the tensors' device (which need not be the current device)."""
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _rows(t, name, T, heads, D, dtype, device):
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {dtype} on {device}")
+    if t.dim() != 3 or t.shape[0] != T or t.shape[2] != D or (heads and t.shape[1] != heads):
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] = [{T}, {heads or 'H'}, {D}]")
+    st, sh, sd = t.stride()
+    if sd != 1 or st < 0 or sh < 0:
+        raise ValueError(f"the values of a {name} row must be contiguous")
+    return Rows(t.data_ptr(), st, sh)
+
+
+def paged_append(cache, batch, k, v, cos=None, sin=None, k_gamma=None, eps=1e-6, q=None, q_gamma=None,
+                 q_dtype=torch.float32, q_out=None):
+    """Append the batch's new tokens to a paged cache, with the q/k prologue on the way (one launch).
+
+    ``k, v [tokens, kv_heads, head_dim]`` and ``q [tokens, heads, head_dim]`` (f32 or f16, all one
+    type; views of a fused projection are taken as they are, any token and head stride).  k and q are
+    RMS-normed (``k_gamma`` / ``q_gamma [head_dim]``; None: not) and rotated in their first
+    ``cos.shape[1]`` dims by ``cos, sin [positions, rot]`` at row ``prefix_len + own position``
+    (None: not); k and v go through the cache's codec into their pages.  Returns the rotated q
+    ``[tokens, heads, head_dim]`` (``q_out``, or new in ``q_dtype``; padding rows are not written),
+    or None without q."""
+    T, KV, D, dev = batch.tokens, cache.KV, cache.D, cache.device
+    batch._fits(cache)
+    if k.dtype not in _DT:
+        raise ValueError(f"k must be float32 or float16, got {k.dtype}")
+    kr, vr = _rows(k, "k", T, KV, D, k.dtype, dev), _rows(v, "v", T, KV, D, k.dtype, dev)
+    rot = positions = 0
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    if cos is not None:
+        _need(cos, torch.float32, "cos")
+        _need(sin, torch.float32, "sin")
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.device != dev or sin.device != dev:
+            raise ValueError("cos and sin must be [positions, rot] on the cache's device")
+        positions, rot = cos.shape
+    for g, name in ((k_gamma, "k_gamma"), (q_gamma, "q_gamma")):
+        if g is not None:
+            _need(g, torch.float32, name)
+            if g.numel() != D or g.device != dev:
+                raise ValueError(f"{name} must be [head_dim] on the cache's device")
+    qr, H = None, 0
+    if q is not None:
+        qr, H = _rows(q, "q", T, 0, D, k.dtype, dev), q.shape[1]
+        if q_out is None:
+            q_out = torch.empty((T, H, D), dtype=q_dtype, device=dev)
+        else:
+            _need(q_out, name="q_out")
+            if q_out.shape != (T, H, D) or q_out.device != dev:
+                raise ValueError("q_out must be [tokens, heads, head_dim] on the cache's device")
+        if q_out.dtype not in _DT:
+            raise ValueError(f"q_out must be float32 or float16, got {q_out.dtype}")
+    with torch.cuda.device(dev):
+        check("bg_paged_append", lib().bg_paged_append(
+            C.byref(cache._desc), C.byref(batch._desc), H, KV, D, C.byref(qr) if qr is not None else None, C.byref(kr),
+            C.byref(vr), _DT[k.dtype], _ptr(q_gamma), _ptr(k_gamma), eps, _ptr(cos), _ptr(sin), rot, positions,
+            _ptr(q_out) if qr is not None else None, _DT[q_out.dtype] if qr is not None else 0, _stream_of(dev)))
+    return q_out if qr is not None else None
+
+
+def paged_attention(q, cache, batch, scale=0.0, gate=None, out_dtype=torch.float32, out=None):
+    """Causal GQA attention of ``q[tokens, H, D]`` (f32 or f16) over a paged cache: the token at own
+    position ``o`` of its sequence attends the batch's shared prefix and own positions ``0 .. o``.
+    ``scale`` 0 means ``1/sqrt(D)``; ``gate[tokens, H, D]`` (f32) applies the sigmoid output gate.
+    Returns ``out[tokens, H, D]``; rows behind the last sequence are not written."""
+    _need(q, name="q")
+    if q.dtype not in _DT:
+        raise ValueError(f"q must be float32 or float16, got {q.dtype}")
+    dev = cache.device
+    if q.dim() != 3 or q.shape[0] != batch.tokens or q.shape[2] != cache.D or q.device != dev:
+        raise ValueError("q must be [tokens, heads, head_dim] on the cache's device")
+    batch._fits(cache)
+    H = q.shape[1]
+    if out is None:
+        out = torch.empty(q.shape, dtype=out_dtype, device=dev)
+    else:
+        _need(out, name="out")
+        if out.shape != q.shape or out.device != dev:
+            raise ValueError("out must have the shape and device of q")
+    if out.dtype not in _DT:
+        raise ValueError(f"out must be float32 or float16, got {out.dtype}")
+    if gate is not None:
+        _need(gate, torch.float32, "gate")
+        if gate.shape != q.shape or gate.device != dev:
+            raise ValueError("gate must have the shape and device of q")
+    cd, bd, L = C.byref(cache._desc), C.byref(batch._desc), lib()
+    key = (H, cache.KV, cache.D, cache.mode, cache.page_size, cache.num_pages)
+    nbytes = batch._ws.get(key)
+    if nbytes is None:
+        nbytes = batch._ws[key] = L.bg_paged_attention_workspace_size(cd, bd, H, cache.KV, cache.D)
+    # scratch of this call alone: calls on other streams and captured graphs each have their own
+    with torch.cuda.device(dev):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        check("bg_paged_attention", L.bg_paged_attention(
+            cd, bd, H, cache.KV, cache.D, q.data_ptr(), _DT[q.dtype], float(scale), _ptr(gate), out.data_ptr(),
+            _DT[out.dtype], _ptr(ws), nbytes, _stream_of(dev)))
+    return out
 
 
 class Graphed:

@@ -201,6 +201,74 @@ int bg_qk_norm_rope(const float *x, uint32_t batch, uint32_t S, uint32_t heads, 
                     const float *sinT, uint32_t rot, uint32_t pos0, float eps, float *y,
                     const bg_kv_cache *kv, bg_stream_t stream);
 
+/* ---- paged cache: append, ragged attention, shared prefix (no reference counterpart: the engine
+ * serves one stream from one slab; a server of many streams of different lengths keeps their positions in
+ * pages of one pool) -------------------------------------------------------------------------------
+ * Pool: K, V [num_pages][page_size][KV][D] in the codec of `mode` (BG_KV_F32, BG_KV_F16 or BG_KV_Q8; q8
+ * scales Ks, Vs [num_pages][page_size][KV][D/32]).  All pointers are 16-byte aligned.
+ * Batch: token rows [cu_q[b], cu_q[b+1]) belong to sequence b and are its newest tokens; cu_q NULL means
+ * one token per sequence (tokens == batch).  kv_len[b] counts the sequence's own positions, the new
+ * tokens among them, so token i of n has own position o = kv_len[b] - n + i, held in slot o % page_size
+ * of page page_table[b*table_stride + o / page_size].  With prefix_len > 0 every sequence also has
+ * positions 0 .. prefix_len-1 in front of its own, held in prefix_pages[j / page_size].
+ * cu_q (not decreasing), kv_len, page_table and prefix_pages are read on the device, so a captured
+ * graph follows them; batch, tokens, max_q (the largest number of tokens of a sequence: it selects
+ * kernels, results do not depend on it), the table's width and prefix_len are fixed by the call.
+ *   - Token rows at or behind cu_q[batch] are padding: their outputs are left as they were.
+ *   - A token whose o is negative has no position: the append skips it, attention gives it the prefix
+ *     alone (zeros without one).
+ *   - Pool slots at or behind kv_len[b] and pages outside the lists may hold anything, NaN included.
+ *     Values below kv_len[b] are the caller's: a NaN or infinity there may also reach rows of the same
+ *     sequence whose own position lies in front of it.
+ *   - A page id outside the pool is never followed: attention reads zeros for it and the append drops
+ *     the row, as it does where the page table is too narrow; bg_device_status then reports BG_EINVAL.
+ * prefix_len + table_stride*page_size has to fit 31 bits. */
+typedef struct {
+  void *K, *V;
+  float *Ks, *Vs;
+  uint64_t num_pages;
+  uint32_t page_size, mode;
+} bg_paged_cache;
+
+typedef struct {
+  const int32_t *cu_q;         /* [batch+1] or NULL */
+  const int32_t *kv_len;       /* [batch] */
+  const int32_t *page_table;   /* [batch][table_stride] */
+  const int32_t *prefix_pages; /* [ceil(prefix_len/page_size)] or NULL */
+  uint32_t batch, tokens, max_q, table_stride, prefix_len;
+} bg_paged_batch;
+
+/* Rows of a projection: row (t, head) starts at x + t*token_stride + head*head_stride (elements), its D
+ * values are contiguous. */
+typedef struct {
+  const void *x;
+  uint64_t token_stride, head_stride;
+} bg_rows;
+
+/* bg_paged_append: for every token, k: [RMSNorm with gamma] -> rotation -> codec -> page, v: codec ->
+ * page, and (q != NULL) q: [RMSNorm] -> rotation -> q_out [tokens][H][D], in one launch.
+ *   norm      y = x / sqrt(mean(x^2) + eps) * gamma[d]              (gamma NULL: y = x)
+ *   rotation  y[d]*cos[p][d] + h[d]*sin[p][d] for d < rot, h = (-y[d+rot/2] | y[d-rot/2]), p = prefix_len
+ *             + o, tables [table_rows][rot] (cosT = sinT = NULL: none).  A token with p >= table_rows is
+ *             skipped and bg_device_status reports BG_EINVAL.
+ * Sources share src_dtype; rot is even and at most D.  Two tokens of one call must not share a slot. */
+int bg_paged_append(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV, uint32_t D,
+                    const bg_rows *q, const bg_rows *k, const bg_rows *v, uint32_t src_dtype, const float *q_gamma,
+                    const float *k_gamma, float eps, const float *cosT, const float *sinT, uint32_t rot,
+                    uint32_t table_rows, void *q_out, uint32_t q_out_dtype, bg_stream_t stream);
+
+/* bg_paged_attention: causal GQA attention of q [tokens][H][D] over the paged cache; the token at own
+ * position o attends the whole prefix and own positions 0 .. o.  scale == 0 selects 1/sqrt(D); gate
+ * [tokens][H][D] f32 or NULL as in bg_attention; out [tokens][H][D].  The shared prefix is read once
+ * for all rows of the batch and joined with each sequence's own part by their log-sum-exp.
+ * workspace: bg_paged_attention_workspace_size bytes, 16-byte aligned, of any content; calls that may
+ * overlap on the GPU need one each. */
+size_t bg_paged_attention_workspace_size(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV,
+                                         uint32_t D);
+int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV, uint32_t D,
+                       const void *q, uint32_t q_dtype, float scale, const float *gate, void *out, uint32_t out_dtype,
+                       void *workspace, size_t workspace_bytes, bg_stream_t stream);
+
 /* ---- KV snapshot wire format ---------------------------------------------------------------
  * saveCache / restoreCache of engine.ts:2719-2872 (KvSnapshot, src/types.ts:364-390): one
  * layer's share of `data` is, for cache positions [base, base+count) in LOGICAL order, the K rows,
