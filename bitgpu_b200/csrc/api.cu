@@ -224,6 +224,8 @@ int snapshot_copy(const bg_kv_cache *kv, uint32_t seq, uint32_t KV, uint32_t D, 
 }  // namespace
 
 namespace bg {
+bool generic_forced() { return g_force_generic != 0; }
+
 size_t attention_split_workspace_bytes(const bg_attn_params *p, uint32_t batch) {
   if (!p || !p->KV || !p->H) return 0;
   const uint32_t L = p->Ltot ? p->Ltot : 1;

@@ -66,6 +66,220 @@ __device__ __forceinline__ int64_t paged_row(const PagedView &kv, const int32_t 
   return pg < kv.num_pages ? (int64_t)pg * kv.page_size + j % kv.page_size : -1;
 }
 
+// ---- the work of a ragged batch as one line of K/V tiles --------------------------------------------
+// A unit is up to RU rows R of one kv head against the positions they attend: of the shared prefix (rows
+// of the whole batch) or of one sequence's own positions.  Units lie one behind the other, each as many
+// tiles of KT positions as its last token attends (at least one, so that rows that attend nothing are
+// written too), and block c of the grid takes tiles [c*per, (c+1)*per).  So every block has the same
+// work whatever the lengths, decided on the device from the lengths of this very call.  A unit that a
+// border cuts leaves partial rows: the piece that starts in block c in slot 2c+1, the piece that block
+// c goes on with in slot 2c.  Only a block's first and last piece can be cut, so two slots suffice.
+struct UnitShape {
+  uint32_t G, KV, RU, KT;
+  uint32_t rows_lo, rows_hi;  // own sequences of rows_lo < n*G <= rows_hi rows (others are another kernel's)
+  int prefix;                 // whether the prefix's units are this kernel's
+};
+
+struct TileSpan {
+  uint64_t total, per, t0, t1;  // all tiles, tiles of a block, this block's [t0, t1)
+  uint64_t pre;                 // tiles of the prefix's units, which come first
+  uint32_t b0;                  // sequence that tile max(t0, pre) belongs to
+  uint64_t off0;                // its index among that sequence's tiles
+};
+
+// Positions that the last row of chunk ch attends (own part of a sequence), and the chunk's tiles.
+__device__ __forceinline__ uint32_t chunk_tiles(const SeqRange &s, const UnitShape &u, uint32_t ch) {
+  const uint32_t rows = s.n * u.G, last = (min((ch + 1) * u.RU, rows) - 1) / u.G;
+  const int32_t m = min(s.len, max(0, s.len - (int32_t)s.n + (int32_t)last + 1));
+  return max(1u, ((uint32_t)m + u.KT - 1) / u.KT);
+}
+
+// Tiles of one kv head of a sequence's own units (0: none of this kernel's).
+__device__ __forceinline__ uint32_t seq_tiles(const SeqRange &s, const UnitShape &u) {
+  const uint32_t rows = s.n * u.G;
+  if (rows <= u.rows_lo || rows > u.rows_hi) return 0;
+  uint32_t n = 0;
+  for (uint32_t ch = 0; ch * u.RU < rows; ++ch) n += chunk_tiles(s, u, ch);
+  return n;
+}
+
+// Rows R that the prefix's units cover: every row of a token of some sequence.
+__device__ __forceinline__ uint32_t batch_rows(const BatchView &bv, uint32_t G) {
+  const int32_t t = bv.cu_q ? __ldg(bv.cu_q + bv.B) : (int32_t)bv.B;
+  return (uint32_t)min(max(t, 0), (int32_t)bv.T) * G;
+}
+
+// All NTHR threads of the block: the block's span.  `sh`: 2 * (NTHR / 32) + 8 words of shared memory.
+template <int NTHR>
+__device__ __forceinline__ TileSpan block_span(const BatchView &bv, const UnitShape &u, uint32_t page_size,
+                                               uint32_t min_tiles, uint64_t *sh) {
+  constexpr int NW = NTHR / 32;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t per_thread = (bv.B + NTHR - 1) / NTHR;
+  const uint32_t lo = min(bv.B, tid * per_thread), hi = min(bv.B, lo + per_thread);
+  uint64_t mine = 0;
+  uint32_t first = 0;
+  for (uint32_t b = lo; b < hi; ++b) {
+    const uint32_t n = u.KV * seq_tiles(seq_range(bv, b, page_size), u);
+    if (b == lo) first = n;
+    mine += n;
+  }
+  uint64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sh[warp] = incl;
+  if (tid == 0) sh[NW] = 0;
+  __syncthreads();
+  uint64_t before = incl - mine, own = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < (int)warp) before += sh[w];
+    own += sh[w];
+  }
+  TileSpan s;
+  s.pre = 0;
+  if (u.prefix && bv.prefix_len) {
+    const uint32_t nch = (batch_rows(bv, u.G) + u.RU - 1) / u.RU;
+    s.pre = (uint64_t)u.KV * nch * ((bv.prefix_len + u.KT - 1) / u.KT);
+  }
+  s.total = s.pre + own;
+  const uint64_t even = (s.total + gridDim.x - 1) / gridDim.x;
+  s.per = even > min_tiles ? even : min_tiles;
+  s.t0 = min(s.total, s.per * blockIdx.x);
+  s.t1 = min(s.total, s.t0 + s.per);
+  const uint64_t want = s.t0 > s.pre ? s.t0 - s.pre : 0;  // among the own tiles
+  if (mine && want >= before && want < before + mine) {
+    uint64_t x = want - before;
+    uint32_t b = lo, n = first;
+    while (x >= n) {
+      x -= n;
+      ++b;
+      n = u.KV * seq_tiles(seq_range(bv, b, page_size), u);
+    }
+    sh[NW] = b;
+    sh[NW + 1] = x;
+  }
+  __syncthreads();
+  s.b0 = (uint32_t)sh[NW];
+  s.off0 = sh[NW + 1];
+  return s;
+}
+
+// One block's pieces of units, in order (uniform over the calling threads).
+struct Piece {
+  uint32_t R0, rows, kvh;   // rows [R0, R0 + rows) of kv head kvh
+  uint32_t tile0, ntiles;   // tiles of the unit
+  uint32_t len;             // positions of the list (the prefix's or the sequence's)
+  int32_t lim_base;         // token t attends positions <= lim_base + t
+  const int32_t *pages;
+  uint32_t c0, npieces;     // block of the unit's first piece, number of pieces
+  bool own, starts;         // own part (or prefix); whether the unit starts in this block
+};
+
+struct PieceWalk {
+  uint64_t cur, t1, per, pre, base;  // next tile; base: tile where sequence b begins
+  uint32_t b, kvh, ch, in;           // own part: sequence, kv head, chunk, tiles before `cur` in the unit
+  SeqRange sr;
+
+  __device__ __forceinline__ void seek(const BatchView &bv, const UnitShape &u, uint32_t page_size, uint64_t off) {
+    // position inside sequence b: (kvh, chunk, tile)
+    sr = seq_range(bv, b, page_size);
+    const uint32_t s = seq_tiles(sr, u);
+    kvh = (uint32_t)(off / s);
+    uint32_t x = (uint32_t)(off % s);
+    ch = 0;
+    for (;;) {
+      const uint32_t n = chunk_tiles(sr, u, ch);
+      if (x < n) break;
+      x -= n;
+      ++ch;
+    }
+    in = x;
+  }
+
+  __device__ __forceinline__ void init(const TileSpan &s, const BatchView &bv, const UnitShape &u, uint32_t page_size) {
+    cur = s.t0;
+    t1 = s.t1;
+    per = s.per;
+    pre = s.pre;
+    b = s.b0;
+    kvh = ch = in = 0;
+    sr = SeqRange{0, 0, 0};
+    if (cur < t1 && t1 > pre) seek(bv, u, page_size, s.off0);
+  }
+
+  __device__ __forceinline__ bool next(Piece &p, const BatchView &bv, const UnitShape &u, uint32_t page_size) {
+    if (cur >= t1) return false;
+    uint64_t a;
+    uint32_t n;
+    if (cur < pre) {
+      const uint32_t rows = batch_rows(bv, u.G), nch = (rows + u.RU - 1) / u.RU;
+      n = (bv.prefix_len + u.KT - 1) / u.KT;
+      const uint64_t unit = cur / n;
+      a = unit * n;
+      p.kvh = (uint32_t)(unit / nch);
+      p.R0 = (uint32_t)(unit % nch) * u.RU;
+      p.rows = min(u.RU, rows - p.R0);
+      p.tile0 = (uint32_t)(cur - a);
+      p.len = bv.prefix_len;
+      p.lim_base = 0x40000000;
+      p.pages = bv.prefix_pages;
+      p.own = false;
+      p.ntiles = (uint32_t)min((uint64_t)(n - p.tile0), t1 - cur);
+    } else {
+      const uint32_t rows = sr.n * u.G;
+      n = chunk_tiles(sr, u, ch);
+      a = cur - in;
+      p.kvh = kvh;
+      p.R0 = sr.begin * u.G + ch * u.RU;
+      p.rows = min(u.RU, rows - ch * u.RU);
+      p.tile0 = in;
+      p.len = (uint32_t)sr.len;
+      p.lim_base = sr.len - (int32_t)sr.n - (int32_t)sr.begin;
+      p.pages = bv.table + (uint64_t)b * bv.table_stride;
+      p.own = true;
+      p.ntiles = (uint32_t)min((uint64_t)(n - in), t1 - cur);
+      in += p.ntiles;
+      if (in == n) {  // on to the next unit: chunk, kv head, sequence
+        in = 0;
+        if (++ch * u.RU >= rows) {
+          ch = 0;
+          if (++kvh == u.KV) {
+            kvh = 0;
+            if (cur + p.ntiles < t1) {
+              do {
+                ++b;
+                sr = seq_range(bv, b, page_size);
+              } while (seq_tiles(sr, u) == 0);
+            }
+          }
+        }
+      }
+    }
+    p.c0 = (uint32_t)(a / per);
+    p.npieces = (uint32_t)((a + n - 1) / per) - p.c0 + 1;
+    p.starts = p.tile0 == 0;
+    cur += p.ntiles;
+    return true;
+  }
+};
+
+// Where a unit's rows wait to be joined.  Without a prefix only cut units leave any: one CutUnit per
+// block (npieces 0: none).  With a prefix every row joins two lists of pieces: one RowPieces per (kv
+// head, R) and part; piece 0 is partial row idx0, piece k row idx0 + (2k - 1) * step.
+struct CutUnit {
+  uint32_t R0, rows, kvh, npieces;
+};
+struct RowPieces {
+  uint32_t idx0, npieces, step, pad;
+};
+__host__ __device__ __forceinline__ uint32_t piece_index(uint32_t idx0, uint32_t step, uint32_t k) {
+  return k ? idx0 + (2 * k - 1) * step : idx0;
+}
+
 struct PagedAppendArgs {
   PagedView kv;
   BatchView bv;
@@ -91,6 +305,11 @@ struct PagedAttnArgs {
   float *part_o;
   float2 *part_ml;
   uint64_t part_rows;
+  // pieces to join: of the own parts (RowPieces or, without a prefix, CutUnit) and of the prefix
+  CutUnit *cuts;
+  RowPieces *own_pieces, *pre_pieces;
+  uint32_t slot0, own_row0, pre_row0;  // first partial row of this kernel's slots, of whole own / prefix units
+  uint32_t min_tiles;
 };
 
 int launch_paged_append(const PagedAppendArgs &a, cudaStream_t st);
@@ -99,7 +318,18 @@ int launch_paged_append(const PagedAppendArgs &a, cudaStream_t st);
 uint32_t paged_generic_splits(uint32_t T, uint32_t H, uint32_t KV, uint64_t max_positions);
 int launch_paged_generic(const PagedAttnArgs &a, uint32_t nsplit, cudaStream_t st);
 
+// Tensor-core decode kernel (mma.sync): few rows a sequence, f16 and q8 pools.
+bool paged_decode_supported(int mode, uint32_t D, uint32_t page_size);
+
+uint32_t paged_decode_blocks(int mode, uint32_t D, uint32_t ru);  // blocks that fill the GPU
+int launch_paged_decode(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_hi, bool prefix, cudaStream_t st);
+// Join the cut units of `blocks` blocks of ru rows (no prefix), or every row's pieces (prefix).
+int launch_paged_join_cuts(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, cudaStream_t st);
+int launch_paged_join_rows(const PagedAttnArgs &a, cudaStream_t st);
+
+int poll_device_error_paged_decode();
 int poll_device_error_paged();  // of all paged operators
+bool generic_forced();  // bg_force_generic
 int poll_device_error_paged_append();
 int poll_device_error_paged_generic();
 

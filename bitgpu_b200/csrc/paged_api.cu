@@ -37,16 +37,38 @@ BatchView view(const bg_paged_batch *b) {
                    b->prefix_len};
 }
 
-// How a call's partial rows are laid out: o [rows][D] f32, then ml [rows] float2.
+// The kernels of one call and the layout of its workspace: partial rows o [part_rows][D] f32, then ml
+// [part_rows] float2, then the descriptions of what is to be joined.
 struct Plan {
+  bool fast;           // tensor-core kernels (else the CUDA-core one)
+  bool join;           // a shared prefix: every row joins its parts
   uint32_t nsplit;     // CUDA-core kernel: splits of every row
-  uint64_t part_rows;  // partial rows
+  uint32_t ru, blocks; // decode kernel: rows of a unit, blocks
+  uint64_t rows;       // tokens * H
+  uint64_t part_rows;
+  size_t desc, bytes;  // offset of the descriptions, size of all
 };
 
-Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, uint32_t KV, uint32_t D) {
-  Plan p;
-  p.nsplit = paged_generic_splits(b->tokens, H, KV, (uint64_t)b->table_stride * kv->page_size + b->prefix_len);
-  p.part_rows = p.nsplit > 1 ? (uint64_t)p.nsplit * b->tokens * H : 0;
+Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, uint32_t KV, uint32_t D, bool fast) {
+  Plan p = {};
+  const uint32_t G = H / KV;
+  const uint64_t cap = (uint64_t)b->table_stride * kv->page_size;
+  p.rows = (uint64_t)b->tokens * H;
+  p.join = b->prefix_len > 0;
+  p.fast = fast && paged_decode_supported((int)kv->mode, D, kv->page_size) && p.rows < 0x3fffffffull;
+  if (!p.fast) {
+    p.nsplit = paged_generic_splits(b->tokens, H, KV, cap + b->prefix_len);
+    p.part_rows = p.nsplit > 1 ? (uint64_t)p.nsplit * p.rows : 0;
+    p.bytes = (size_t)p.part_rows * (D * 4 + 8);
+    return p;
+  }
+  // rows of a unit: 8 where a sequence's rows (or, behind a prefix, all rows) fill no more
+  const uint64_t group = (uint64_t)b->max_q * G, all = (uint64_t)b->tokens * G;
+  p.ru = group <= 8 && !(p.join && all > 8) ? 8 : 16;
+  p.blocks = paged_decode_blocks((int)kv->mode, D, p.ru);
+  p.part_rows = 2ull * p.blocks * p.ru + (p.join ? 2 * p.rows : 0);
+  p.desc = (size_t)p.part_rows * (D * 4 + 8);
+  p.bytes = p.desc + (p.join ? 2 * p.rows * sizeof(RowPieces) : p.blocks * sizeof(CutUnit));
   return p;
 }
 
@@ -56,6 +78,7 @@ namespace bg {
 int poll_device_error_paged() {
   int e = poll_device_error_paged_append();
   if (!e) e = poll_device_error_paged_generic();
+  if (!e) e = poll_device_error_paged_decode();
   return e;
 }
 }  // namespace bg
@@ -103,7 +126,9 @@ int bg_paged_append(const bg_paged_cache *kv, const bg_paged_batch *batch, uint3
 size_t bg_paged_attention_workspace_size(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV,
                                          uint32_t D) {
   if (check_paged(kv, batch, KV, D) || H == 0 || H % KV || batch->batch == 0 || batch->tokens == 0) return 0;
-  return (size_t)make_plan(kv, batch, H, KV, D).part_rows * (D + 2) * sizeof(float);
+  // enough for either kind of kernel, so that bg_force_generic does not change what a caller needs
+  const size_t a = make_plan(kv, batch, H, KV, D, true).bytes, b = make_plan(kv, batch, H, KV, D, false).bytes;
+  return a > b ? a : b;
 }
 
 int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV, uint32_t D,
@@ -113,10 +138,10 @@ int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, ui
   if (H == 0 || H % KV || q_dtype > BG_DT_F16 || out_dtype > BG_DT_F16) return BG_EINVAL;
   if (batch->batch == 0 || batch->tokens == 0) return BG_OK;
   if (!q || !out || !aligned16(q) || !aligned16(out) || !aligned16(gate) || !aligned16(workspace)) return BG_EINVAL;
-  const Plan plan = make_plan(kv, batch, H, KV, D);
-  const size_t need = (size_t)plan.part_rows * (D + 2) * sizeof(float);
-  if (need && (!workspace || workspace_bytes < need)) return BG_ENOMEM;
-  PagedAttnArgs a;
+  const Plan plan = make_plan(kv, batch, H, KV, D, !generic_forced());
+  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes)) return BG_ENOMEM;
+  cudaStream_t st = (cudaStream_t)stream;
+  PagedAttnArgs a = {};
   a.kv = view(kv, KV);
   a.bv = view(batch);
   a.mode = (int)kv->mode;
@@ -133,7 +158,20 @@ int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, ui
   a.part_o = static_cast<float *>(workspace);
   a.part_ml = reinterpret_cast<float2 *>(a.part_o + plan.part_rows * D);
   a.part_rows = plan.part_rows;
-  return launch_paged_generic(a, plan.nsplit, (cudaStream_t)stream);
+  a.min_tiles = 1;
+  if (!plan.fast) return launch_paged_generic(a, plan.nsplit, st);
+  unsigned char *desc = static_cast<unsigned char *>(workspace) + plan.desc;
+  a.slot0 = 0;
+  if (plan.join) {
+    a.own_pieces = reinterpret_cast<RowPieces *>(desc);
+    a.pre_pieces = a.own_pieces + plan.rows;
+    a.own_row0 = 2 * plan.blocks * plan.ru;
+    a.pre_row0 = a.own_row0 + (uint32_t)plan.rows;
+  } else {
+    a.cuts = reinterpret_cast<CutUnit *>(desc);
+  }
+  if (int rc = launch_paged_decode(a, plan.blocks, plan.ru, 0xffffffffu, plan.join, st)) return rc;
+  return plan.join ? launch_paged_join_rows(a, st) : launch_paged_join_cuts(a, plan.blocks, plan.ru, st);
 }
 
 }  // extern "C"
