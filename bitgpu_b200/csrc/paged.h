@@ -280,6 +280,18 @@ __host__ __device__ __forceinline__ uint32_t piece_index(uint32_t idx0, uint32_t
   return k ? idx0 + (2 * k - 1) * step : idx0;
 }
 
+// Raise a kernel's dynamic shared memory limit once per device (`done`: one bit per device).
+template <typename K>
+inline bool allow_smem(K kern, int bytes, unsigned long long &done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (__atomic_load_n(&done, __ATOMIC_ACQUIRE) & bit)) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  if (bit) __atomic_fetch_or(&done, bit, __ATOMIC_RELEASE);
+  return true;
+}
+
 struct PagedAppendArgs {
   PagedView kv;
   BatchView bv;

@@ -404,8 +404,11 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           moved |= corr != 1.0f;
         }
       }
-      // rescale the output only when a running max of this warp moved
-      if (__any_sync(0xffffffffu, moved)) {
+      // f16 rows: rescale the output only when a running max of this warp moved.  f32 rows: every tile's
+      // products start from zero and are added to the rescaled output by one fused multiply-add per
+      // value -- the MMA truncates what it accumulates, and over the ~100 tiles of a long split that bias
+      // alone (3e-6 at 131072 positions) is more than all other errors together.
+      if (!LO && __any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -450,8 +453,15 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma16816(oacc[nt][mt], f, pb0[nt], pb1[nt]);
-            if constexpr (LO) mma16816(oacc[nt][mt], f, pl0[nt], pl1[nt]);
+            if constexpr (LO) {
+              float acc[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816(acc, f, pl0[nt], pl1[nt]);
+              mma16816(acc, f, pb0[nt], pb1[nt]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) oacc[nt][mt][i] = fmaf(oacc[nt][mt][i], cr[nt][i & 1], acc[i]);
+            } else {
+              mma16816(oacc[nt][mt], f, pb0[nt], pb1[nt]);
+            }
           }
         }
       } else {
@@ -480,11 +490,20 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           const uint32_t a1[4] = {code(r[2], kSelEven), code(r[2], kSelOdd), code(r[3], kSelEven), code(r[3], kSelOdd)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma16816(oacc[nt][2 * bk], a0, pb0[nt], pb1[nt]);
-            mma16816(oacc[nt][2 * bk + 1], a1, pb0[nt], pb1[nt]);
             if constexpr (LO) {
-              mma16816(oacc[nt][2 * bk], a0, pl0[nt], pl1[nt]);
-              mma16816(oacc[nt][2 * bk + 1], a1, pl0[nt], pl1[nt]);
+              float x0[4] = {0.f, 0.f, 0.f, 0.f}, x1[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816(x0, a0, pl0[nt], pl1[nt]);
+              mma16816(x1, a1, pl0[nt], pl1[nt]);
+              mma16816(x0, a0, pb0[nt], pb1[nt]);
+              mma16816(x1, a1, pb0[nt], pb1[nt]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                oacc[nt][2 * bk][i] = fmaf(oacc[nt][2 * bk][i], cr[nt][i & 1], x0[i]);
+                oacc[nt][2 * bk + 1][i] = fmaf(oacc[nt][2 * bk + 1][i], cr[nt][i & 1], x1[i]);
+              }
+            } else {
+              mma16816(oacc[nt][2 * bk], a0, pb0[nt], pb1[nt]);
+              mma16816(oacc[nt][2 * bk + 1], a1, pb0[nt], pb1[nt]);
             }
           }
         }
@@ -590,7 +609,8 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_hi, bool p
   if (make_tmap_4d(&tk, dt, a.kv.K, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return BG_EUNSUPPORTED;
   if (make_tmap_4d(&tv, dt, a.kv.V, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return BG_EUNSUPPORTED;
   auto kern = paged_decode_kernel<MODE, D, NT, LO>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return BG_ELAUNCH;
+  static unsigned long long allowed = 0;
+  if (!allow_smem(kern, C::SMEM, allowed)) return BG_ELAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(kThreads);

@@ -376,6 +376,7 @@ class PagedKVCache:
         self._desc = PagedCacheDesc(K.data_ptr(), V.data_ptr(), Ks.data_ptr() if Ks is not None else None,
                                     Vs.data_ptr() if Vs is not None else None, self.num_pages, self.page_size,
                                     MODES[self.mode])
+        self._ref = C.byref(self._desc)
 
     def desc(self):
         return self._desc
@@ -422,6 +423,7 @@ class PagedBatch:
         self.device = page_table.device
         self._desc = PagedBatchDesc(_ptr(cu_q), kv_len.data_ptr(), page_table.data_ptr(), _ptr(prefix_pages), B, tokens,
                                     max_q, width, prefix_len)
+        self._ref = C.byref(self._desc)
         self._ws = {}
 
     def desc(self):
@@ -438,9 +440,19 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream_of(device):
-    """The current stream of the tensors' device (which need not be the current device)."""
-    return torch.cuda.current_stream(device).cuda_stream
+# the handle of a device's current stream, without building a Stream object around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _on(device, fn, *args):
+    """Call ``fn(*args, stream)`` on the tensors' device (which need not be the current device) and
+    its current stream."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(*args, _raw_stream(index))
 
 
 def _rows(t, name, T, heads, D, dtype, device):
@@ -451,7 +463,7 @@ def _rows(t, name, T, heads, D, dtype, device):
     st, sh, sd = t.stride()
     if sd != 1 or st < 0 or sh < 0:
         raise ValueError(f"the values of a {name} row must be contiguous")
-    return Rows(t.data_ptr(), st, sh)
+    return C.byref(Rows(t.data_ptr(), st, sh))
 
 
 def paged_append(cache, batch, k, v, cos=None, sin=None, k_gamma=None, eps=1e-6, q=None, q_gamma=None,
@@ -495,12 +507,14 @@ def paged_append(cache, batch, k, v, cos=None, sin=None, k_gamma=None, eps=1e-6,
                 raise ValueError("q_out must be [tokens, heads, head_dim] on the cache's device")
         if q_out.dtype not in _DT:
             raise ValueError(f"q_out must be float32 or float16, got {q_out.dtype}")
-    with torch.cuda.device(dev):
-        check("bg_paged_append", lib().bg_paged_append(
-            C.byref(cache._desc), C.byref(batch._desc), H, KV, D, C.byref(qr) if qr is not None else None, C.byref(kr),
-            C.byref(vr), _DT[k.dtype], _ptr(q_gamma), _ptr(k_gamma), eps, _ptr(cos), _ptr(sin), rot, positions,
-            _ptr(q_out) if qr is not None else None, _DT[q_out.dtype] if qr is not None else 0, _stream_of(dev)))
-    return q_out if qr is not None else None
+    else:
+        q_out = None
+    rc = _on(dev, lib().bg_paged_append, cache._ref, batch._ref, H, KV, D, qr, kr, vr, _DT[k.dtype], _ptr(q_gamma),
+             _ptr(k_gamma), eps, _ptr(cos), _ptr(sin), rot, positions, _ptr(q_out),
+             _DT[q_out.dtype] if q is not None else 0)
+    if rc:
+        check("bg_paged_append", rc)
+    return q_out
 
 
 def paged_attention(q, cache, batch, scale=0.0, gate=None, out_dtype=torch.float32, out=None):
@@ -517,7 +531,7 @@ def paged_attention(q, cache, batch, scale=0.0, gate=None, out_dtype=torch.float
     batch._fits(cache)
     H = q.shape[1]
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype, device=dev)
+        out = torch.empty_like(q, dtype=out_dtype)
     else:
         _need(out, name="out")
         if out.shape != q.shape or out.device != dev:
@@ -528,17 +542,17 @@ def paged_attention(q, cache, batch, scale=0.0, gate=None, out_dtype=torch.float
         _need(gate, torch.float32, "gate")
         if gate.shape != q.shape or gate.device != dev:
             raise ValueError("gate must have the shape and device of q")
-    cd, bd, L = C.byref(cache._desc), C.byref(batch._desc), lib()
-    key = (H, cache.KV, cache.D, cache.mode, cache.page_size, cache.num_pages)
+    key = (H, cache.KV, cache.D, cache.mode, cache.page_size)
     nbytes = batch._ws.get(key)
     if nbytes is None:
-        nbytes = batch._ws[key] = L.bg_paged_attention_workspace_size(cd, bd, H, cache.KV, cache.D)
-    # scratch of this call alone: calls on other streams and captured graphs each have their own
-    with torch.cuda.device(dev):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        check("bg_paged_attention", L.bg_paged_attention(
-            cd, bd, H, cache.KV, cache.D, q.data_ptr(), _DT[q.dtype], float(scale), _ptr(gate), out.data_ptr(),
-            _DT[out.dtype], _ptr(ws), nbytes, _stream_of(dev)))
+        nbytes = batch._ws[key] = lib().bg_paged_attention_workspace_size(cache._ref, batch._ref, H, cache.KV, cache.D)
+    # scratch of this call alone, from the stream's own allocator: calls on other streams and captured
+    # graphs each have theirs
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    rc = _on(dev, lib().bg_paged_attention, cache._ref, batch._ref, H, cache.KV, cache.D, q.data_ptr(), _DT[q.dtype],
+             float(scale), _ptr(gate), out.data_ptr(), _DT[out.dtype], _ptr(ws), nbytes)
+    if rc:
+        check("bg_paged_attention", rc)
     return out
 
 
