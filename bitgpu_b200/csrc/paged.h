@@ -81,11 +81,17 @@ struct UnitShape {
 };
 
 struct TileSpan {
-  uint64_t total, per, t0, t1;  // all tiles, tiles of a block, this block's [t0, t1)
-  uint64_t pre;                 // tiles of the prefix's units, which come first
+  uint32_t total, per, t0, t1;  // all tiles, tiles of a block, this block's [t0, t1)
+  uint32_t pre;                 // tiles of the prefix's units, which come first
   uint32_t b0;                  // sequence that tile max(t0, pre) belongs to
-  uint64_t off0;                // its index among that sequence's tiles
+  uint32_t off0;                // its index among that sequence's tiles
 };
+
+// An upper bound of all tiles of a call, from what the host knows.
+inline uint64_t most_tiles(const UnitShape &u, uint64_t tokens, uint64_t batch, uint64_t capacity, uint64_t prefix) {
+  const uint64_t units = tokens * u.G / u.RU + batch + 1;
+  return u.KV * units * ((capacity + u.KT - 1) / u.KT + 1 + (prefix + u.KT - 1) / u.KT);
+}
 
 // Positions that the last row of chunk ch attends (own part of a sequence), and the chunk's tiles.
 __device__ __forceinline__ uint32_t chunk_tiles(const SeqRange &s, const UnitShape &u, uint32_t ch) {
@@ -109,31 +115,32 @@ __device__ __forceinline__ uint32_t batch_rows(const BatchView &bv, uint32_t G) 
   return (uint32_t)min(max(t, 0), (int32_t)bv.T) * G;
 }
 
-// All NTHR threads of the block: the block's span.  `sh`: 2 * (NTHR / 32) + 8 words of shared memory.
+// All NTHR threads of the block: the block's span.  `sh`: NTHR / 32 + 2 words of shared memory.  Tile
+// numbers have 32 bits: most_tiles() of the call's bounds says whether that is enough.
 template <int NTHR>
 __device__ __forceinline__ TileSpan block_span(const BatchView &bv, const UnitShape &u, uint32_t page_size,
-                                               uint32_t min_tiles, uint64_t *sh) {
+                                               uint32_t min_tiles, uint32_t *sh) {
   constexpr int NW = NTHR / 32;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t per_thread = (bv.B + NTHR - 1) / NTHR;
   const uint32_t lo = min(bv.B, tid * per_thread), hi = min(bv.B, lo + per_thread);
-  uint64_t mine = 0;
+  uint32_t mine = 0;
   uint32_t first = 0;
   for (uint32_t b = lo; b < hi; ++b) {
     const uint32_t n = u.KV * seq_tiles(seq_range(bv, b, page_size), u);
     if (b == lo) first = n;
     mine += n;
   }
-  uint64_t incl = mine;
+  uint32_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += v;
   }
   if (lane == 31) sh[warp] = incl;
   if (tid == 0) sh[NW] = 0;
   __syncthreads();
-  uint64_t before = incl - mine, own = 0;
+  uint32_t before = incl - mine, own = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     if (w < (int)warp) before += sh[w];
@@ -143,16 +150,16 @@ __device__ __forceinline__ TileSpan block_span(const BatchView &bv, const UnitSh
   s.pre = 0;
   if (u.prefix && bv.prefix_len) {
     const uint32_t nch = (batch_rows(bv, u.G) + u.RU - 1) / u.RU;
-    s.pre = (uint64_t)u.KV * nch * ((bv.prefix_len + u.KT - 1) / u.KT);
+    s.pre = u.KV * nch * ((bv.prefix_len + u.KT - 1) / u.KT);
   }
   s.total = s.pre + own;
-  const uint64_t even = (s.total + gridDim.x - 1) / gridDim.x;
+  const uint32_t even = s.total / gridDim.x + (s.total % gridDim.x != 0);
   s.per = even > min_tiles ? even : min_tiles;
-  s.t0 = min(s.total, s.per * blockIdx.x);
-  s.t1 = min(s.total, s.t0 + s.per);
-  const uint64_t want = s.t0 > s.pre ? s.t0 - s.pre : 0;  // among the own tiles
+  s.t0 = (uint32_t)min((uint64_t)s.total, (uint64_t)s.per * blockIdx.x);
+  s.t1 = s.t0 + min(s.per, s.total - s.t0);
+  const uint32_t want = s.t0 > s.pre ? s.t0 - s.pre : 0;  // among the own tiles
   if (mine && want >= before && want < before + mine) {
-    uint64_t x = want - before;
+    uint32_t x = want - before;
     uint32_t b = lo, n = first;
     while (x >= n) {
       x -= n;
@@ -163,7 +170,7 @@ __device__ __forceinline__ TileSpan block_span(const BatchView &bv, const UnitSh
     sh[NW + 1] = x;
   }
   __syncthreads();
-  s.b0 = (uint32_t)sh[NW];
+  s.b0 = sh[NW];
   s.off0 = sh[NW + 1];
   return s;
 }
@@ -175,21 +182,21 @@ struct Piece {
   uint32_t len;             // positions of the list (the prefix's or the sequence's)
   int32_t lim_base;         // token t attends positions <= lim_base + t
   const int32_t *pages;
-  uint32_t c0, npieces;     // block of the unit's first piece, number of pieces
+  uint32_t npieces;         // pieces of the unit
   bool own, starts;         // own part (or prefix); whether the unit starts in this block
 };
 
 struct PieceWalk {
-  uint64_t cur, t1, per, pre, base;  // next tile; base: tile where sequence b begins
+  uint32_t cur, t1, per, pre;  // next tile, end of the span
   uint32_t b, kvh, ch, in;           // own part: sequence, kv head, chunk, tiles before `cur` in the unit
   SeqRange sr;
 
-  __device__ __forceinline__ void seek(const BatchView &bv, const UnitShape &u, uint32_t page_size, uint64_t off) {
+  __device__ __forceinline__ void seek(const BatchView &bv, const UnitShape &u, uint32_t page_size, uint32_t off) {
     // position inside sequence b: (kvh, chunk, tile)
     sr = seq_range(bv, b, page_size);
     const uint32_t s = seq_tiles(sr, u);
-    kvh = (uint32_t)(off / s);
-    uint32_t x = (uint32_t)(off % s);
+    kvh = off / s;
+    uint32_t x = off % s;
     ch = 0;
     for (;;) {
       const uint32_t n = chunk_tiles(sr, u, ch);
@@ -213,22 +220,21 @@ struct PieceWalk {
 
   __device__ __forceinline__ bool next(Piece &p, const BatchView &bv, const UnitShape &u, uint32_t page_size) {
     if (cur >= t1) return false;
-    uint64_t a;
-    uint32_t n;
+    uint32_t a, n;
     if (cur < pre) {
       const uint32_t rows = batch_rows(bv, u.G), nch = (rows + u.RU - 1) / u.RU;
       n = (bv.prefix_len + u.KT - 1) / u.KT;
-      const uint64_t unit = cur / n;
+      const uint32_t unit = cur / n;
       a = unit * n;
-      p.kvh = (uint32_t)(unit / nch);
-      p.R0 = (uint32_t)(unit % nch) * u.RU;
+      p.kvh = unit / nch;
+      p.R0 = unit % nch * u.RU;
       p.rows = min(u.RU, rows - p.R0);
-      p.tile0 = (uint32_t)(cur - a);
+      p.tile0 = cur - a;
       p.len = bv.prefix_len;
       p.lim_base = 0x40000000;
       p.pages = bv.prefix_pages;
       p.own = false;
-      p.ntiles = (uint32_t)min((uint64_t)(n - p.tile0), t1 - cur);
+      p.ntiles = min(n - p.tile0, t1 - cur);
     } else {
       const uint32_t rows = sr.n * u.G;
       n = chunk_tiles(sr, u, ch);
@@ -241,7 +247,7 @@ struct PieceWalk {
       p.lim_base = sr.len - (int32_t)sr.n - (int32_t)sr.begin;
       p.pages = bv.table + (uint64_t)b * bv.table_stride;
       p.own = true;
-      p.ntiles = (uint32_t)min((uint64_t)(n - in), t1 - cur);
+      p.ntiles = min(n - in, t1 - cur);
       in += p.ntiles;
       if (in == n) {  // on to the next unit: chunk, kv head, sequence
         in = 0;
@@ -259,8 +265,7 @@ struct PieceWalk {
         }
       }
     }
-    p.c0 = (uint32_t)(a / per);
-    p.npieces = (uint32_t)((a + n - 1) / per) - p.c0 + 1;
+    p.npieces = (a + n - 1) / per - a / per + 1;
     p.starts = p.tile0 == 0;
     cur += p.ntiles;
     return true;
@@ -278,6 +283,18 @@ struct RowPieces {
 };
 __host__ __device__ __forceinline__ uint32_t piece_index(uint32_t idx0, uint32_t step, uint32_t k) {
   return k ? idx0 + (2 * k - 1) * step : idx0;
+}
+
+// Positions of a page box: the largest number that divides pages and tiles alike, so that a box that
+// starts on a multiple of it never leaves its page.
+inline uint32_t page_box(uint32_t page_size, uint32_t tile) {
+  uint32_t x = page_size, y = tile;
+  while (y) {
+    const uint32_t z = x % y;
+    x = y;
+    y = z;
+  }
+  return x;
 }
 
 // Raise a kernel's dynamic shared memory limit once per device (`done`: one bit per device).
@@ -335,11 +352,16 @@ bool paged_decode_supported(int mode, uint32_t D, uint32_t page_size);
 
 uint32_t paged_decode_blocks(int mode, uint32_t D, uint32_t ru);  // blocks that fill the GPU
 int launch_paged_decode(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_hi, bool prefix, cudaStream_t st);
+// tcgen05 kernel: many rows a sequence (own part), or the rows of the batch against the shared prefix.
+bool paged_tc_supported(int mode, uint32_t D, uint32_t page_size);
+uint32_t paged_tc_rows(bool lo, uint64_t rows);
+int launch_paged_tc(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_lo, bool prefix, cudaStream_t st);
 // Join the cut units of `blocks` blocks of ru rows (no prefix), or every row's pieces (prefix).
 int launch_paged_join_cuts(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, cudaStream_t st);
 int launch_paged_join_rows(const PagedAttnArgs &a, cudaStream_t st);
 
 int poll_device_error_paged_decode();
+int poll_device_error_paged_tc();
 int poll_device_error_paged();  // of all paged operators
 bool generic_forced();  // bg_force_generic
 int poll_device_error_paged_append();

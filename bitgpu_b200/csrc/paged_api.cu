@@ -37,38 +37,63 @@ BatchView view(const bg_paged_batch *b) {
                    b->prefix_len};
 }
 
+constexpr uint32_t kSMs = 148;
+
 // The kernels of one call and the layout of its workspace: partial rows o [part_rows][D] f32, then ml
 // [part_rows] float2, then the descriptions of what is to be joined.
+//   join        a shared prefix: every row joins its parts
+//   tc_pre      the prefix's units run on tcgen05: from 33 rows on.  (Fewer fit two or three units of the
+//               decode kernel, which then reads the prefix that often, from L2 after the first time.)
+//   tc_own      sequences of more than 16 rows run on tcgen05
+//   decode      the decode kernel has the rest: sequences of at most 16 rows beside tc_own -- not launched
+//               where tokens == batch * max_q says that there are none; were it wrong, tc_own has them
 struct Plan {
-  bool fast;           // tensor-core kernels (else the CUDA-core one)
-  bool join;           // a shared prefix: every row joins its parts
-  uint32_t nsplit;     // CUDA-core kernel: splits of every row
-  uint32_t ru, blocks; // decode kernel: rows of a unit, blocks
-  uint64_t rows;       // tokens * H
-  uint64_t part_rows;
-  size_t desc, bytes;  // offset of the descriptions, size of all
+  bool fast, join, tc_pre, tc_own, decode;
+  uint32_t nsplit;                  // CUDA-core kernel: splits of every row
+  uint32_t ru, blocks;              // decode kernel: rows of a unit, blocks
+  uint32_t ru_own, ru_pre;          // tcgen05 kernels: rows of a unit
+  uint32_t slot_own, slot_pre;      // first partial row of each kernel's slots (the decode kernel's: 0)
+  uint32_t row_own, row_pre;        // ... of the whole units behind a prefix
+  uint64_t rows, part_rows;         // tokens * H; all partial rows
+  size_t desc, bytes;               // offset of the descriptions, size of all
 };
 
-Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, uint32_t KV, uint32_t D, bool fast) {
+Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, uint32_t KV, uint32_t D, bool fast, bool lo) {
   Plan p = {};
   const uint32_t G = H / KV;
   const uint64_t cap = (uint64_t)b->table_stride * kv->page_size;
   p.rows = (uint64_t)b->tokens * H;
   p.join = b->prefix_len > 0;
-  p.fast = fast && paged_decode_supported((int)kv->mode, D, kv->page_size) && p.rows < 0x3fffffffull;
+  const UnitShape small{G, KV, 8, 64, 0, 0, 0};  // the most units and tiles that any kernel may count
+  p.fast = fast && paged_decode_supported((int)kv->mode, D, kv->page_size) && p.rows < 0x10000000ull &&
+           most_tiles(small, b->tokens, b->batch, cap, b->prefix_len) < 0xffffffffull;
   if (!p.fast) {
     p.nsplit = paged_generic_splits(b->tokens, H, KV, cap + b->prefix_len);
     p.part_rows = p.nsplit > 1 ? (uint64_t)p.nsplit * p.rows : 0;
     p.bytes = (size_t)p.part_rows * (D * 4 + 8);
     return p;
   }
-  // rows of a unit: 8 where a sequence's rows (or, behind a prefix, all rows) fill no more
   const uint64_t group = (uint64_t)b->max_q * G, all = (uint64_t)b->tokens * G;
-  p.ru = group <= 8 && !(p.join && all > 8) ? 8 : 16;
+  const bool tc = paged_tc_supported((int)kv->mode, D, kv->page_size);
+  p.tc_own = tc && group > 16;
+  p.tc_pre = tc && p.join && all > 32;
+  p.decode = !p.tc_own || (p.join && !p.tc_pre) || b->tokens < (uint64_t)b->batch * b->max_q;
+  // rows of a unit: 8 where a sequence's rows (or, behind a prefix, all rows) fill no more
+  p.ru = !p.tc_own && group <= 8 && !(p.join && !p.tc_pre && all > 8) ? 8 : 16;
   p.blocks = paged_decode_blocks((int)kv->mode, D, p.ru);
-  p.part_rows = 2ull * p.blocks * p.ru + (p.join ? 2 * p.rows : 0);
+  p.ru_own = paged_tc_rows(lo, group);
+  p.ru_pre = paged_tc_rows(lo, all);
+  uint64_t at = p.decode ? 2ull * p.blocks * p.ru : 0;
+  p.slot_own = (uint32_t)at;
+  if (p.tc_own) at += 2ull * kSMs * p.ru_own;
+  p.slot_pre = (uint32_t)at;
+  if (p.tc_pre) at += 2ull * kSMs * p.ru_pre;
+  p.row_own = (uint32_t)at;
+  p.row_pre = (uint32_t)(at + p.rows);
+  if (p.join) at += 2 * p.rows;
+  p.part_rows = at;
   p.desc = (size_t)p.part_rows * (D * 4 + 8);
-  p.bytes = p.desc + (p.join ? 2 * p.rows * sizeof(RowPieces) : p.blocks * sizeof(CutUnit));
+  p.bytes = p.desc + (p.join ? 2 * p.rows * sizeof(RowPieces) : (p.blocks + kSMs) * sizeof(CutUnit));
   return p;
 }
 
@@ -79,6 +104,7 @@ int poll_device_error_paged() {
   int e = poll_device_error_paged_append();
   if (!e) e = poll_device_error_paged_generic();
   if (!e) e = poll_device_error_paged_decode();
+  if (!e) e = poll_device_error_paged_tc();
   return e;
 }
 }  // namespace bg
@@ -127,8 +153,13 @@ size_t bg_paged_attention_workspace_size(const bg_paged_cache *kv, const bg_page
                                          uint32_t D) {
   if (check_paged(kv, batch, KV, D) || H == 0 || H % KV || batch->batch == 0 || batch->tokens == 0) return 0;
   // enough for either kind of kernel, so that bg_force_generic does not change what a caller needs
-  const size_t a = make_plan(kv, batch, H, KV, D, true).bytes, b = make_plan(kv, batch, H, KV, D, false).bytes;
-  return a > b ? a : b;
+  // (and for either type of rows)
+  size_t n = 0;
+  for (int i = 0; i < 3; ++i) {
+    const size_t m = make_plan(kv, batch, H, KV, D, i < 2, i == 1).bytes;
+    n = m > n ? m : n;
+  }
+  return n;
 }
 
 int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV, uint32_t D,
@@ -138,7 +169,7 @@ int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, ui
   if (H == 0 || H % KV || q_dtype > BG_DT_F16 || out_dtype > BG_DT_F16) return BG_EINVAL;
   if (batch->batch == 0 || batch->tokens == 0) return BG_OK;
   if (!q || !out || !aligned16(q) || !aligned16(out) || !aligned16(gate) || !aligned16(workspace)) return BG_EINVAL;
-  const Plan plan = make_plan(kv, batch, H, KV, D, !generic_forced());
+  const Plan plan = make_plan(kv, batch, H, KV, D, !generic_forced(), !(q_dtype == BG_DT_F16 && out_dtype == BG_DT_F16));
   if (plan.bytes && (!workspace || workspace_bytes < plan.bytes)) return BG_ENOMEM;
   cudaStream_t st = (cudaStream_t)stream;
   PagedAttnArgs a = {};
@@ -161,17 +192,33 @@ int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, ui
   a.min_tiles = 1;
   if (!plan.fast) return launch_paged_generic(a, plan.nsplit, st);
   unsigned char *desc = static_cast<unsigned char *>(workspace) + plan.desc;
-  a.slot0 = 0;
+  CutUnit *cuts = reinterpret_cast<CutUnit *>(desc);
   if (plan.join) {
     a.own_pieces = reinterpret_cast<RowPieces *>(desc);
     a.pre_pieces = a.own_pieces + plan.rows;
-    a.own_row0 = 2 * plan.blocks * plan.ru;
-    a.pre_row0 = a.own_row0 + (uint32_t)plan.rows;
-  } else {
-    a.cuts = reinterpret_cast<CutUnit *>(desc);
+    a.own_row0 = plan.row_own;
+    a.pre_row0 = plan.row_pre;
   }
-  if (int rc = launch_paged_decode(a, plan.blocks, plan.ru, 0xffffffffu, plan.join, st)) return rc;
-  return plan.join ? launch_paged_join_rows(a, st) : launch_paged_join_cuts(a, plan.blocks, plan.ru, st);
+  auto with = [&](uint32_t slot0, CutUnit *c) {
+    PagedAttnArgs x = a;
+    x.slot0 = slot0;
+    x.cuts = plan.join ? nullptr : c;
+    return x;
+  };
+  const PagedAttnArgs dec = with(0, cuts), own = with(plan.slot_own, cuts + plan.blocks), pre = with(plan.slot_pre, nullptr);
+  if (plan.tc_pre)
+    if (int rc = launch_paged_tc(pre, kSMs, plan.ru_pre, 0, true, st)) return rc;
+  if (plan.tc_own)
+    if (int rc = launch_paged_tc(own, kSMs, plan.ru_own, plan.decode ? 16 : 0, false, st)) return rc;
+  if (plan.decode)
+    if (int rc = launch_paged_decode(dec, plan.blocks, plan.ru, plan.tc_own ? 16 : 0xffffffffu, plan.join && !plan.tc_pre, st))
+      return rc;
+  if (plan.join) return launch_paged_join_rows(a, st);
+  if (plan.tc_own)
+    if (int rc = launch_paged_join_cuts(own, kSMs, plan.ru_own, st)) return rc;
+  if (plan.decode)
+    if (int rc = launch_paged_join_cuts(dec, plan.blocks, plan.ru, st)) return rc;
+  return BG_OK;
 }
 
 }  // extern "C"

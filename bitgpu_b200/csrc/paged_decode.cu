@@ -40,7 +40,7 @@ constexpr int kUnits = 2;    // staged units
 struct DecodeParams {
   PagedAttnArgs a;
   UnitShape u;
-  uint32_t ppt;         // page boxes per tile (page_size < 64), else 1
+  uint32_t ppt;         // page boxes per tile
   uint32_t box;         // positions per box
   uint32_t join_rows;   // 1: every unit leaves partial rows (a shared prefix exists)
 };
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::oB);
   uint64_t *empty = full + NST, *ufull = empty + NST, *uempty = ufull + kUnits;
   uint64_t *meet = uempty + kUnits;  // the consumer warps' barrier
-  uint64_t *scan = meet + 1;
+  uint32_t *scan = reinterpret_cast<uint32_t *>(meet + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const PagedAttnArgs &a = p.a;
   if (smem_u32(smem) & 1023) {  // the swizzled tiles need it; dynamic shared memory starts on such a border
@@ -597,7 +597,7 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_hi, bool p
   DecodeParams p;
   p.a = a;
   p.u = UnitShape{a.G, a.kv.KV, 8 * NT, kTile, 0, rows_hi, prefix};
-  p.box = ps < kTile ? ps : kTile;
+  p.box = page_box(ps, kTile);
   p.ppt = kTile / p.box;
   p.join_rows = a.own_pieces != nullptr;
   CUtensorMap tk, tv;
@@ -636,10 +636,9 @@ int launch_md(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t row
 
 }  // namespace
 
-// 64-position tiles are made of whole page boxes: pages of 16 or 32 positions, or multiples of 64.
+// Page boxes of at least 8 positions keep the 128-byte swizzle's pattern.
 bool paged_decode_supported(int mode, uint32_t D, uint32_t page_size) {
-  return (mode == BG_KV_F16 || mode == BG_KV_Q8) && (D == 128 || D == 256) &&
-         (page_size == 16 || page_size == 32 || page_size % kTile == 0);
+  return (mode == BG_KV_F16 || mode == BG_KV_Q8) && (D == 128 || D == 256) && page_size % 8 == 0;
 }
 
 uint32_t paged_decode_blocks(int mode, uint32_t D, uint32_t ru) {

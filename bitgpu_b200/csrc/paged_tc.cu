@@ -1,0 +1,738 @@
+// Attention of many rows over a paged cache on the 5th-generation tensor cores (tcgen05 + TMEM): chunked
+// prefill of a ragged batch, and the rows of a whole batch against its shared prefix.
+//
+// A unit (paged.h) is 128 or 256 rows R = token*G + g of one kv head -- queries of several tokens and all
+// heads of the group, so K and V are shared by all of them -- against a page list; blocks take even shares
+// of the units' K/V tiles and leave partial rows where a border cuts a unit.
+//
+// Two streams keep the tensor pipe and the softmax warps busy at once.  Each has its own score tile S_t,
+// output tile O_t (TMEM, f32) and softmax warpgroup:
+//   NQT = 2 (256 rows): stream t is rows [128 t, 128 t + 128) and both use every K/V tile;
+//   NQT = 1 (128 rows): the streams take even and odd K/V tiles of the same rows, and their outputs are
+//           joined at the end (stream 0 reads both from TMEM).
+// The MMA thread issues PV_t(i) and right behind it the next S_t, which overwrites the columns that P_t was
+// read from: MMAs of one thread execute in order, and the commit behind S_t covers PV_t too.
+//
+// Precision, by the types of the call:
+//   f16 rows, f16 pool: operands are exact, P is rounded once to f16 (kept 2^6 up, away from subnormals);
+//   f32 rows (LO): q and p are split into two f16 halves (22 bits) -- two products for S, two for O;
+//   q8 pool: code * scale has more than 11 bits, so K and V are split too when they are dequantised into
+//           the operand tiles: one more product each.  (A single f16 rounding of K and V would double the
+//           error of f16 rows; the extra products cost less than that here, because the softmax warps
+//           and not the tensor pipe set the pace of the single-product form.)
+//
+// Warp roles: warp 0 TMA producer of K and V (f16 pool; page boxes, 128-byte swizzle), warp 1 MMA issuer,
+// warps 2-3 load the next unit's query rows as soon as the last S of the current one is done, warps 4-11
+// softmax (one row per thread), warps 12-15 (q8 pool) dequantise, one tile ahead in registers.
+// All waits are bounded; on expiry the block records BG_ETIMEOUT, stops issuing, waits for what it issued,
+// frees its TMEM and exits.
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include "paged.h"
+#include "paged_merge.cuh"
+#include "umma.cuh"
+
+namespace bg {
+namespace {
+
+constexpr int kM = 128;             // rows of a UMMA tile
+constexpr float kRescale = 8.0f;    // lazy rescale threshold, log2 units
+constexpr float kUp = 6.0f;         // p carries 2^6: at most 2^14 with the lazy rescale
+
+template <int D, bool Q8, bool LO, int NQT>
+struct TcCfg {
+  static constexpr int NQ = LO ? 2 : 1, NK = Q8 ? 2 : 1;     // operand halves
+  static constexpr int QT = kM * D * 2;                      // bytes of one f16 query tile
+  static constexpr int KT = D == 128 ? (Q8 ? 64 : 128) : (Q8 || LO ? 32 : 64);
+  static constexpr int KVT = KT * D * 2;                     // bytes of one f16 K (or V) tile
+  static constexpr int oQ = 0, oK = NQT * NQ * QT, oV = oK + 2 * NK * KVT, oB = oV + 2 * NK * KVT;
+  static constexpr int oInfo = oB + 256, oML = oInfo + 64, oScan = oML + kM * 8;
+  static constexpr int SMEM = oScan + 20 * 8;
+  static constexpr int THREADS = Q8 ? 512 : 384;
+  static constexpr uint32_t S0 = 0, S1 = KT < 128 ? 64 : 128, O0 = D == 128 ? 256 : 0, O1 = 384;
+
+
+  static_assert(SMEM <= 232448, "shared memory");
+};
+
+struct TcParams {
+  PagedAttnArgs a;
+  UnitShape u;
+  uint32_t box, ppt;  // positions of a page box, boxes per tile
+  uint32_t join_rows;
+};
+
+struct alignas(16) TcInfo {
+  uint32_t R0, rows, kvh, tile0, ntiles, len;
+  int32_t lim_base;
+  uint32_t dest, row0;
+};
+constexpr uint32_t kDirect = 0xffffffffu, kRowBuf = 0xfffffffeu;
+
+// 16-byte chunk `ch` (8 f16) of row r in a 128B-swizzled K-major operand tile of R rows
+template <int R>
+__device__ __forceinline__ uint32_t sw_off(int r, int ch) {
+  return (uint32_t)((ch >> 3) * (R * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+}
+
+// eight values as f16 and what the rounding left over
+__device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 p = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    const float2 f = __half22float2(p);
+    h[i] = *reinterpret_cast<const uint32_t *>(&p);
+    l[i] = pack_half2(x[2 * i] - f.x, x[2 * i + 1] - f.y);
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
+template <int D, bool Q8, bool LO, int NQT>
+__global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
+    paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                    const __grid_constant__ TcParams p) {
+  using C = TcCfg<D, Q8, LO, NQT>;
+  constexpr int KT = C::KT, NQ = C::NQ, NK = C::NK;
+  static_assert(D == 128, "two streams need two O tiles of 128 columns");
+  extern __shared__ __align__(1024) unsigned char smem[];
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::oB);
+  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;
+  uint64_t *q_full = bars + 8, *q_free = bars + 9, *info_free = bars + 10;
+  uint64_t *s_full = bars + 11, *p_full = bars + 13, *o_done = bars + 15, *o_free = bars + 17;
+  uint64_t *b_done = bars + 19, *mma_done = bars + 20, *tail = bars + 21;
+  uint32_t *tmem_at = reinterpret_cast<uint32_t *>(bars + 22);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 23);
+  TcInfo *info = reinterpret_cast<TcInfo *>(smem + C::oInfo);
+  float2 *ml_s = reinterpret_cast<float2 *>(smem + C::oML);
+  const PagedAttnArgs &a = p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (smem_u32(smem) & 1023) {
+    atomicExch(&g_device_error, BG_ELAUNCH);
+    return;
+  }
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], Q8 ? 4 : 1);
+      mbar_init(&v_full[i], Q8 ? 4 : 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_done[i], 1);
+      mbar_init(&o_free[i], 128);
+    }
+    mbar_init(q_full, 64);
+    mbar_init(q_free, 1);
+    mbar_init(info_free, 8);
+    mbar_init(b_done, 128);
+    mbar_init(mma_done, 1);
+    mbar_init(tail, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    if (!Q8) {
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+    }
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  tc_fence_before();
+  const TileSpan span = block_span<C::THREADS>(a.bv, p.u, a.kv.page_size, a.min_tiles,
+                                               reinterpret_cast<uint32_t *>(smem + C::oScan));
+  tc_fence_after();
+  const uint32_t tmem = *tmem_at;
+  const uint32_t sQ = smem_u32(smem + C::oQ), sK = smem_u32(smem + C::oK), sV = smem_u32(smem + C::oV);
+  const uint32_t ps = a.kv.page_size;
+
+  // registers: 384 threads: 128*72 + 256*216 = 384*168; 512: 128*72 + 256*168 + 128*104 = 512*128
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
+  if (warp == 0) {
+    // ---------------- TMA producer (f16 pool) ----------------
+    if constexpr (!Q8) {
+      PieceWalk walk;
+      walk.init(span, a.bv, p.u, ps);
+      Piece pc;
+      bool ok = true;
+      int it = 0, tails = 0, kdone = 0, vdone = 0;
+      while (ok && walk.next(pc, a.bv, p.u, ps)) {
+        auto page_of = [&](uint32_t tile) -> uint32_t {
+          const uint32_t pos = (pc.tile0 + tile) * KT + lane * p.box;
+          if ((uint32_t)lane >= p.ppt || tile >= pc.ntiles || pos >= pc.len) return a.kv.num_pages;
+          const uint32_t pg = (uint32_t)__ldg(pc.pages + pos / ps);
+          if (pg < a.kv.num_pages) return pg;
+          atomicExch(&g_device_error, BG_EINVAL);
+          return a.kv.num_pages;
+        };
+        uint32_t pg_next = page_of(0);
+        for (uint32_t t = 0; ok && t < pc.ntiles; ++t, ++it) {
+          const uint32_t pg = pg_next;
+          pg_next = page_of(t + 1);
+          const int s = it & 1;
+          const uint32_t pos0 = (pc.tile0 + t) * KT, par = ((it >> 1) - 1) & 1;
+          const int y = (int)((pos0 + lane * p.box) % ps);
+          if (it >= 2) ok = mbar_wait_warp(&k_empty[s], par);
+          if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
+          if (lane == 0) mbar_expect_tx(&k_full[s], C::KVT);
+          __syncwarp();
+          if ((uint32_t)lane < p.ppt)
+            for (int cb = 0; cb < D / 64; ++cb)
+              tma_load_4d(smem + C::oK + s * C::KVT + cb * KT * 128 + lane * p.box * 128, &tmK, &k_full[s], cb * 64,
+                          (int)pc.kvh, y, (int)pg);
+          kdone = it + 1;
+          if (it >= 2) ok = mbar_wait_warp(&v_empty[s], par);
+          if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
+          // slots of the last page behind the length may hold NaN, and 0 * NaN is NaN: such a tile
+          // arrives on its own barrier, its rows behind the length are cleared, then it is handed on
+          const bool last = pos0 + KT > pc.len && pc.len > pos0 && pc.len % p.box;
+          uint64_t *bar = last ? tail : &v_full[s];
+          if (lane == 0) mbar_expect_tx(bar, C::KVT);
+          __syncwarp();
+          unsigned char *dst = smem + C::oV + s * C::KVT;
+          if ((uint32_t)lane < p.ppt)
+            for (int cb = 0; cb < D / 64; ++cb)
+              tma_load_4d(dst + cb * KT * 128 + lane * p.box * 128, &tmV, bar, cb * 64, (int)pc.kvh, y, (int)pg);
+          if (last) {
+            ok = mbar_wait_warp(tail, tails++ & 1);
+            if (!ok) break;
+            const uint32_t r0 = pc.len - pos0, r1 = (r0 + p.box - 1) / p.box * p.box, n = (r1 - r0) * 8;
+            for (uint32_t i = lane; i < n * (D / 64); i += 32) {
+              const uint32_t cb = i / n, x = i % n;
+              *reinterpret_cast<uint4 *>(dst + cb * KT * 128 + r0 * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[s]);
+          }
+          vdone = it + 1;
+        }
+      }
+      if (!ok && lane == 0) *abort_flag = 1;
+      // no copy may still be in flight when the block exits
+      if (lane == 0) {
+        for (int i = max(0, kdone - 2); i < kdone; ++i) mbar_wait(&k_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, vdone - 2); i < vdone; ++i) mbar_wait(&v_full[i & 1], (i >> 1) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      constexpr uint32_t idS = idesc_f16(KT, false), idO = idesc_f16(D, true);
+      auto one_s = [&](uint32_t slot, uint32_t q, uint32_t k, bool acc) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t da = umma_desc_sw128(q + (kk >> 2) * (kM * 128) + (kk & 3) * 32, 16, 1024);
+          const uint64_t db = umma_desc_sw128(k + (kk >> 2) * (KT * 128) + (kk & 3) * 32, 16, 1024);
+          umma_ss(tmem + slot, da, db, idS, acc || kk > 0);
+        }
+      };
+      // S = Q K^T: small products first, so that they are added up among themselves
+      auto issue_s = [&](int t, int s) {
+        const uint32_t slot = t ? C::S1 : C::S0;
+        const uint32_t q = sQ + (NQT == 2 ? t : 0) * NQ * C::QT, k = sK + s * NK * C::KVT;
+        bool acc = false;
+        if constexpr (LO) {
+          one_s(slot, q + C::QT, k, acc);
+          acc = true;
+        }
+        if constexpr (Q8) {
+          one_s(slot, q, k + C::KVT, acc);
+          acc = true;
+        }
+        one_s(slot, q, k, acc);
+      };
+      auto one_pv = [&](uint32_t o, uint32_t pa, uint32_t v, bool acc) {
+#pragma unroll
+        for (int kk = 0; kk < KT / 16; ++kk) {
+          const uint64_t dv = umma_desc_sw128(v + kk * 16 * 128, KT * 128, 1024);
+          umma_ts(tmem + o, tmem + pa + kk * 8, dv, idO, (acc || kk > 0) ? 1u : 0u);
+        }
+      };
+      auto issue_pv = [&](int t, int s, bool acc) {
+        const uint32_t slot = t ? C::S1 : C::S0, o = t ? C::O1 : C::O0, v = sV + s * NK * C::KVT;
+        if constexpr (LO) {
+          one_pv(o, slot + KT / 2, v, acc);
+          acc = true;
+        }
+        if constexpr (Q8) {
+          one_pv(o, slot, v + C::KVT, acc);
+          acc = true;
+        }
+        one_pv(o, slot, v, acc);
+      };
+      bool ok = true;
+      int it = 0;               // tiles of all pieces before this one
+      uint32_t np[2] = {0, 0};  // P tiles consumed per stream
+      for (uint32_t piece = 0; ok; ++piece) {
+        if (!mbar_wait(q_full, piece & 1)) { ok = false; break; }
+        const int n = (int)info->ntiles;
+        if (n == 0) break;
+        tc_fence_after();
+        auto wait_k = [&](int i) { return mbar_wait(&k_full[(it + i) & 1], ((it + i) >> 1) & 1); };
+        auto wait_v = [&](int i) { return mbar_wait(&v_full[(it + i) & 1], ((it + i) >> 1) & 1); };
+        auto wait_o = [&](int t) { return piece == 0 || mbar_wait(&o_free[NQT == 2 ? t : 0], (piece - 1) & 1); };
+        if constexpr (NQT == 2) {
+          ok = wait_k(0);
+          if (!ok) break;
+          tc_fence_after();
+          for (int t = 0; t < 2; ++t) {
+            issue_s(t, it & 1);
+            umma_commit(&s_full[t]);
+          }
+          umma_commit(&k_empty[it & 1]);
+          if (n == 1) umma_commit(q_free);
+          for (int i = 0; ok && i < n; ++i) {
+            for (int t = 0; ok && t < 2; ++t) {
+              ok = mbar_wait(&p_full[t], np[t]++ & 1) && (i > 0 || wait_o(t)) && (t > 0 || wait_v(i));
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv(t, (it + i) & 1, i > 0);
+              if (t == 1) umma_commit(&v_empty[(it + i) & 1]);
+              if (i + 1 < n) {
+                if (t == 0) ok = wait_k(i + 1);
+                if (!ok) break;
+                tc_fence_after();
+                issue_s(t, (it + i + 1) & 1);
+                umma_commit(&s_full[t]);
+                if (t == 1) {
+                  umma_commit(&k_empty[(it + i + 1) & 1]);
+                  if (i + 2 == n) umma_commit(q_free);
+                }
+              } else {
+                umma_commit(&o_done[t]);
+              }
+            }
+          }
+        } else {
+          for (int i = 0; ok && i < 2 && i < n; ++i) {
+            ok = wait_k(i);
+            if (!ok) break;
+            tc_fence_after();
+            issue_s(i, (it + i) & 1);
+            umma_commit(&s_full[i]);
+            umma_commit(&k_empty[(it + i) & 1]);
+            if (i + 1 == n) umma_commit(q_free);
+          }
+          for (int i = 0; ok && i < n; ++i) {
+            const int t = i & 1;
+            ok = mbar_wait(&p_full[t], np[t]++ & 1) && (i > 1 || wait_o(t)) && wait_v(i);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(t, (it + i) & 1, i > 1);
+            umma_commit(&v_empty[(it + i) & 1]);
+            if (i + 2 < n) {
+              ok = wait_k(i + 2);
+              if (!ok) break;
+              tc_fence_after();
+              issue_s(t, (it + i) & 1);
+              umma_commit(&s_full[t]);
+              umma_commit(&k_empty[(it + i) & 1]);
+              if (i + 3 == n) umma_commit(q_free);
+            } else {
+              umma_commit(&o_done[t]);
+            }
+          }
+        }
+        it += n;
+      }
+      if (!ok) *abort_flag = 1;
+      // every MMA must complete before the block frees its TMEM
+      umma_commit(mma_done);
+      mbar_wait(mma_done, 0);
+    }
+  } else {
+    // ---------------- query rows and descriptions ----------------
+    const int gt = (warp - 2) * 32 + lane;
+    PieceWalk walk;
+    walk.init(span, a.bv, p.u, ps);
+    Piece pc;
+    bool ok = true;
+    if (a.cuts && gt == 0) a.cuts[blockIdx.x].npieces = 0;
+    for (uint32_t piece = 0; ok; ++piece) {
+      const bool more = walk.next(pc, a.bv, p.u, ps);
+      if (piece > 0) {
+        ok = mbar_wait_warp(q_free, (piece - 1) & 1) && mbar_wait_warp(info_free, (piece - 1) & 1);
+        if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) break;
+      }
+      if (!more) {
+        if (gt == 0) info->ntiles = 0;
+        mbar_arrive(q_full);
+        break;
+      }
+      const bool whole = pc.npieces == 1;
+      const uint32_t slot = a.slot0 + (2 * blockIdx.x + (pc.starts ? 1 : 0)) * p.u.RU;
+      const uint32_t row0 = pc.own ? a.own_row0 : a.pre_row0;
+      if (gt == 0) {
+        info->R0 = pc.R0;
+        info->rows = pc.rows;
+        info->kvh = pc.kvh;
+        info->tile0 = pc.tile0;
+        info->ntiles = pc.ntiles;
+        info->len = pc.len;
+        info->lim_base = pc.lim_base;
+        info->dest = !whole ? slot : p.join_rows ? kRowBuf : kDirect;
+        info->row0 = row0;
+        if (!p.join_rows && !whole && pc.starts) a.cuts[blockIdx.x] = CutUnit{pc.R0, pc.rows, pc.kvh, pc.npieces};
+      }
+      if (p.join_rows && pc.starts) {
+        RowPieces *rp = (pc.own ? a.own_pieces : a.pre_pieces) + (uint64_t)pc.kvh * a.bv.T * a.G + pc.R0;
+        for (uint32_t r = gt; r < pc.rows; r += 64) {
+          const uint32_t R = pc.R0 + r;
+          rp[r] = RowPieces{whole ? row0 + R / a.G * a.H + pc.kvh * a.G + R % a.G : slot + r, pc.npieces, p.u.RU, 0};
+        }
+      }
+      constexpr int CPR = D / 8;  // chunks of 8 values per row
+      constexpr int NIT = NQT * kM * CPR / 64;
+      if constexpr (!LO) {
+#pragma unroll 4
+        for (int i = 0; i < NIT; ++i) {
+          const uint32_t idx = gt + i * 64, r = idx / CPR, c = idx % CPR, R = pc.R0 + r;
+          const bool there = r < pc.rows;
+          const uint64_t off = there ? ((uint64_t)(R / a.G) * a.H + pc.kvh * a.G + R % a.G) * CPR + c : 0;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sQ + (r >> 7) * C::QT + sw_off<kM>(r & 127, c)),
+                       "l"(static_cast<const uint4 *>(a.q) + off), "r"(there ? 16u : 0u)
+                       : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+      } else {
+#pragma unroll 1
+        for (int i0 = 0; i0 < NIT; i0 += 4) {
+          float x[4][8];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint32_t idx = gt + (i0 + u) * 64, r = idx / CPR, c = idx % CPR, R = pc.R0 + r;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[u][j] = 0.f;
+            if (r < pc.rows) {
+              const uint64_t off = ((uint64_t)(R / a.G) * a.H + pc.kvh * a.G + R % a.G) * D + c * 8;
+              if (a.q_f16) load_f16<8>(static_cast<const __half *>(a.q) + off, x[u]);
+              else load_f32<8>(static_cast<const float *>(a.q) + off, x[u]);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const uint32_t idx = gt + (i0 + u) * 64, r = idx / CPR, c = idx % CPR;
+            uint4 hi, lo;
+            split8(x[u], hi, lo);
+            unsigned char *d = smem + C::oQ + (r >> 7) * NQ * C::QT + sw_off<kM>(r & 127, c);
+            *reinterpret_cast<uint4 *>(d) = hi;
+            *reinterpret_cast<uint4 *>(d + C::QT) = lo;
+          }
+        }
+      }
+      fence_async_smem();
+      mbar_arrive(q_full);
+    }
+    if (!ok) *abort_flag = 1;
+  }
+  } else if (warp < 12) {
+    // ---------------- softmax (one row per thread) ----------------
+    if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;" ::: "memory");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
+    const int t = (warp - 4) >> 2;                // stream
+    const int row = ((warp & 3) << 5) + lane;     // TMEM lane
+    const uint32_t lane_off = (uint32_t)((warp & 3) << 5) << 16;
+    const uint32_t sbase = (tmem + (t ? C::S1 : C::S0)) | lane_off;
+    const uint32_t obase = (tmem + (t ? C::O1 : C::O0)) | lane_off;
+    const float sl2 = a.sl2;
+    bool ok = true;
+    uint32_t ns = 0, nd = 0;  // score tiles and finished outputs of this stream
+    uint32_t nd1 = 0;         // finished outputs of stream 1, counted by stream 0 (NQT = 1)
+    for (uint32_t piece = 0;; ++piece) {
+      if (!mbar_wait_warp(q_full, piece & 1)) { ok = false; break; }
+      const TcInfo in = *info;
+      __syncwarp();
+      if (in.ntiles == 0) break;
+      if (lane == 0) mbar_arrive(info_free);
+      const uint32_t r = (NQT == 2 ? t * kM : 0) + row;
+      const uint32_t R = in.R0 + min(r, in.rows - 1);
+      const int lim = min(in.lim_base + (int)(R / a.G), (int)in.len - 1);
+      float m_used = kNegBig, l = 0.f;
+      const int step = NQT == 2 ? 1 : 2;
+      const int first = NQT == 2 ? 0 : t;
+      for (int j = first; j < (int)in.ntiles; j += step) {
+        if (!mbar_wait_warp(&s_full[t], ns++ & 1)) { ok = false; break; }
+        tc_fence_after();
+        const int key0 = (int)(in.tile0 + j) * KT;
+        const int nvalid = min(KT, max(0, lim - key0 + 1));
+        uint32_t x[KT / 32][32];  // the whole score row: one TMEM wait per tile
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) tmem_ld32(sbase + c * 32, x[c]);
+        tmem_wait_ld();
+        if (nvalid < KT) {
+#pragma unroll
+          for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= nvalid) x[c][i] = __float_as_uint(-INFINITY);
+        }
+        float mx8[8];  // eight independent chains
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mx8[k] = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const int k = (c * 16 + i / 2) & 7;
+            mx8[k] = fmax3(mx8[k], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+          }
+        const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], fmaxf(mx8[5], fmaxf(mx8[6], mx8[7]))));
+        const float mt = mx * sl2;
+        // lazy rescale: the whole warp takes the TMEM round trip when any of its rows moved far; rows
+        // that did not use the factor 1.  PV of the tile before has completed (its commit is behind S).
+        const bool need = mt > m_used + kRescale;
+        if (__any_sync(0xffffffffu, need)) {
+          if (j > first) {
+            const float f = need ? ex2_approx(m_used - mt) : 1.0f;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(obase + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st32(obase + c * 32, o);
+            }
+            l *= f;
+          }
+          if (need) m_used = mt;
+        }
+        const float mneg = kUp - m_used;
+        float ls0 = 0.f, ls1 = 0.f;
+#pragma unroll
+        for (int c = 0; c < KT / 32; ++c) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float p0 = ex2_approx(fmaf(__uint_as_float(x[c][2 * i]), sl2, mneg));
+            const float p1 = ex2_approx(fmaf(__uint_as_float(x[c][2 * i + 1]), sl2, mneg));
+            ls0 += p0;
+            ls1 += p1;
+            hi[i] = pack_half2(p0, p1);
+            if constexpr (LO) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
+              lo[i] = pack_half2(p0 - f.x, p1 - f.y);
+            }
+          }
+          tmem_st16(sbase + c * 16, hi);
+          if constexpr (LO) tmem_st16(sbase + KT / 2 + c * 16, lo);
+        }
+        l += ls0 + ls1;
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      // ---- the piece's rows ----
+      const bool some = first < (int)in.ntiles;
+      if (some) {
+        ok = mbar_wait_warp(&o_done[t], nd++ & 1);
+        if (!ok) break;
+      }
+      float f0 = 1.f, f1 = 0.f, M = m_used, L = l;
+      if constexpr (NQT == 1) {
+        if (t == 1) {
+          // stream 0 still reads the last piece's (m, l) until it frees O
+          if (piece > 0 && !mbar_wait_warp(&o_free[0], (piece - 1) & 1)) { ok = false; break; }
+          ml_s[row] = make_float2(m_used, some ? l : 0.f);
+          mbar_arrive(b_done);
+          continue;
+        }
+        if (!mbar_wait_warp(b_done, piece & 1)) { ok = false; break; }
+        if (in.ntiles > 1 && !mbar_wait_warp(&o_done[1], nd1++ & 1)) { ok = false; break; }
+        const float2 ml = ml_s[row];
+        M = fmaxf(m_used, ml.x);
+        f0 = ex2_approx(m_used - M);
+        f1 = in.ntiles > 1 ? ex2_approx(ml.x - M) : 0.f;
+        L = l * f0 + ml.y * f1;
+      }
+      tc_fence_after();
+      const bool valid = r < in.rows;
+      const uint64_t orow = (uint64_t)(R / a.G) * a.H + in.kvh * a.G + R % a.G;
+      const uint64_t prow = in.dest == kRowBuf ? in.row0 + orow : in.dest + r;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(obase + c * 32, o);
+        tmem_wait_ld();
+        if constexpr (NQT == 1) {
+          if (in.ntiles > 1) {  // uniform: O_1 holds something
+            uint32_t o1[32];
+            tmem_ld32(((tmem + C::O1) | lane_off) + c * 32, o1);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(o1[i]) * f1);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f0);
+          }
+        }
+        if (!valid) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float v[4] = {__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                              __uint_as_float(o[4 * i + 3])};
+          if (in.dest == kDirect) write_out4(a.out, a.out_f16, a.gate, orow * D + c * 32 + i * 4, v, L);
+          else *reinterpret_cast<float4 *>(a.part_o + prow * D + c * 32 + i * 4) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      if (valid && in.dest != kDirect) a.part_ml[prow] = make_float2(M - kUp, L);
+      tc_fence_before();
+      mbar_arrive(&o_free[NQT == 2 ? t : 0]);
+    }
+    if (!ok) *abort_flag = 1;
+  } else {
+    // ---------------- dequantising producer (q8 pool) ----------------
+    if constexpr (Q8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;" ::: "memory");
+      const int gt = tid - 384;
+      constexpr int CPR = D / 16;                // 16-code chunks per row
+      constexpr int NCH = KT * CPR / 128;        // chunks per thread of one tile
+      PieceWalk walk;
+      walk.init(span, a.bv, p.u, ps);
+      Piece pc;
+      uint32_t t = 0;
+      bool have = walk.next(pc, a.bv, p.u, ps), ok = true;
+      uint4 w[2][NCH];
+      float sc[2][NCH];
+      auto fetch = [&](uint32_t tile) {  // codes and block scales of K and V; zeros behind the length
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          const uint32_t idx = gt + i * 128, r = idx / CPR, c = idx % CPR, pos = (pc.tile0 + tile) * KT + r;
+          int64_t row = -1;
+          if (pos < pc.len) {
+            row = paged_row(a.kv, pc.pages, pos);
+            if (row < 0) atomicExch(&g_device_error, BG_EINVAL);
+          }
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            w[v][i] = make_uint4(0, 0, 0, 0);
+            sc[v][i] = 0.f;
+            if (row >= 0) {
+              const uint64_t at = (uint64_t)row * a.kv.KV + pc.kvh;
+              w[v][i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(v ? a.kv.V : a.kv.K) + at * D + c * 16));
+              sc[v][i] = __ldg((v ? a.kv.Vs : a.kv.Ks) + at * (D / 32) + c / 2);
+            }
+          }
+        }
+      };
+      if (have) fetch(0);
+      for (int it = 0; have; ++it) {
+        const int s = it & 1;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          if (it >= 2) ok = mbar_wait_warp(v ? &v_empty[s] : &k_empty[s], ((it >> 1) - 1) & 1);
+          if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
+          unsigned char *dst = smem + (v ? C::oV : C::oK) + s * 2 * C::KVT;
+#pragma unroll
+          for (int i = 0; i < NCH; ++i) {
+            const uint32_t idx = gt + i * 128, r = idx / CPR, c = idx % CPR;
+            const uint32_t in[4] = {w[v][i].x, w[v][i].y, w[v][i].z, w[v][i].w};
+            const float s127 = sc[v][i] * (1.0f / 127.0f);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float x[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) x[k] = (float)(int8_t)(in[2 * h + k / 4] >> (8 * (k % 4))) * s127;
+              uint4 hi, lo;
+              split8(x, hi, lo);
+              unsigned char *d = dst + sw_off<KT>(r, 2 * c + h);
+              *reinterpret_cast<uint4 *>(d) = hi;
+              *reinterpret_cast<uint4 *>(d + C::KVT) = lo;
+            }
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v ? &v_full[s] : &k_full[s]);
+        }
+        if (!ok) break;
+        if (++t == pc.ntiles) {
+          t = 0;
+          have = walk.next(pc, a.bv, p.u, ps);
+        }
+        if (have) fetch(t);
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+template <int D, bool Q8, bool LO, int NQT>
+int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_lo, bool prefix, cudaStream_t st) {
+  using C = TcCfg<D, Q8, LO, NQT>;
+  const uint32_t ps = a.kv.page_size;
+  TcParams p;
+  p.a = a;
+  // a launch has either the prefix's units or the sequences' own
+  p.u = UnitShape{a.G, a.kv.KV, NQT * kM, C::KT, prefix ? 0xffffffffu : rows_lo, 0xffffffffu, prefix};
+  p.box = page_box(ps, C::KT);
+  p.ppt = C::KT / p.box;
+  p.join_rows = a.own_pieces != nullptr;
+  CUtensorMap tk = {}, tv = {};
+  if (!Q8) {
+    const uint64_t rb = (uint64_t)D * 2;
+    const uint64_t dims[4] = {D, a.kv.KV, ps, a.kv.num_pages};
+    const uint64_t strides[3] = {rb, rb * a.kv.KV, rb * a.kv.KV * ps};
+    const uint32_t box[4] = {64, 1, p.box, 1};
+    if (make_tmap_4d(&tk, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.kv.K, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        make_tmap_4d(&tv, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.kv.V, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return BG_EUNSUPPORTED;
+  }
+  auto kern = paged_tc_kernel<D, Q8, LO, NQT>;
+  static unsigned long long allowed = 0;
+  if (!allow_smem(kern, C::SMEM, allowed)) return BG_ELAUNCH;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, tk, tv, p) == cudaSuccess ? BG_OK : BG_ELAUNCH;
+}
+
+template <bool Q8>
+int launch_q(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_lo, bool prefix, cudaStream_t st) {
+  if (!(a.q_f16 && a.out_f16)) return launch_cfg<128, Q8, true, 1>(a, blocks, rows_lo, prefix, st);
+  return ru == 256 ? launch_cfg<128, Q8, false, 2>(a, blocks, rows_lo, prefix, st)
+                   : launch_cfg<128, Q8, false, 1>(a, blocks, rows_lo, prefix, st);
+}
+
+}  // namespace
+
+// Page boxes of at least 8 positions keep the 128-byte swizzle's pattern.
+bool paged_tc_supported(int mode, uint32_t D, uint32_t page_size) {
+  return (mode == BG_KV_F16 || mode == BG_KV_Q8) && D == 128 && page_size % 8 == 0;
+}
+
+// Rows of a unit: two query tiles where there are rows for them and shared memory for both (f16 rows).
+uint32_t paged_tc_rows(bool lo, uint64_t rows) { return !lo && rows > kM ? 2 * kM : kM; }
+
+int launch_paged_tc(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_lo, bool prefix, cudaStream_t st) {
+  return a.mode == BG_KV_Q8 ? launch_q<true>(a, blocks, ru, rows_lo, prefix, st)
+                            : launch_q<false>(a, blocks, ru, rows_lo, prefix, st);
+}
+
+int poll_device_error_paged_tc() {
+  int v = 0, z = 0;
+  if (cudaMemcpyFromSymbol(&v, g_device_error, sizeof(int)) != cudaSuccess) return BG_ELAUNCH;
+  if (v) cudaMemcpyToSymbol(g_device_error, &z, sizeof(int));
+  return v;
+}
+
+}  // namespace bg

@@ -43,10 +43,17 @@ def test_decode_lengths(ops, mode, D, io):
 
 
 @pytest.mark.parametrize("mode", ["f16", "q8"])
-@pytest.mark.parametrize("page", [1, 5, 16, 32, 48, 64, 128, 256])
+@pytest.mark.parametrize("page", [1, 5, 8, 16, 24, 32, 48, 64, 128, 192, 256])
 def test_page_sizes(ops, mode, page):
     lens = [3, 200, 65, 513]
     run(ops, Ragged(lens, [1] * 4, page=page, mode=mode, seed=page), what=f"page {page}")
+
+
+@pytest.mark.parametrize("mode", ["f16", "q8"])
+@pytest.mark.parametrize("page", [5, 8, 24, 48, 64, 192, 256])
+def test_page_sizes_prefill(ops, mode, page):
+    run(ops, Ragged([213, 100, 515], [80, 100, 33], page=page, mode=mode, prefix=77, seed=page), torch.float16,
+        torch.float16, what=f"page {page}")
 
 
 @pytest.mark.parametrize("G", [1, 2, 3, 6, 8, 12, 16, 20])
