@@ -76,6 +76,8 @@ __device__ __forceinline__ int64_t paged_row(const PagedView &kv, const int32_t 
 // c goes on with in slot 2c.  Only a block's first and last piece can be cut, so two slots suffice.
 struct UnitShape {
   uint32_t G, KV, RU, KT;
+  uint32_t tokens;  // RU / G where that is whole, else 0
+  uint32_t shift;   // log2(KT)
   uint32_t rows_lo, rows_hi;  // own sequences of rows_lo < n*G <= rows_hi rows (others are another kernel's)
   int prefix;                 // whether the prefix's units are this kernel's
 };
@@ -87,6 +89,12 @@ struct TileSpan {
   uint32_t off0;                // its index among that sequence's tiles
 };
 
+inline UnitShape unit_shape(uint32_t G, uint32_t KV, uint32_t RU, uint32_t KT, uint32_t rows_lo, uint32_t rows_hi, bool prefix) {
+  UnitShape u{G, KV, RU, KT, RU % G ? 0 : RU / G, 0, rows_lo, rows_hi, prefix};
+  while ((1u << u.shift) < KT) ++u.shift;
+  return u;
+}
+
 // An upper bound of all tiles of a call, from what the host knows.
 inline uint64_t most_tiles(const UnitShape &u, uint64_t tokens, uint64_t batch, uint64_t capacity, uint64_t prefix) {
   const uint64_t units = tokens * u.G / u.RU + batch + 1;
@@ -95,9 +103,9 @@ inline uint64_t most_tiles(const UnitShape &u, uint64_t tokens, uint64_t batch, 
 
 // Positions that the last row of chunk ch attends (own part of a sequence), and the chunk's tiles.
 __device__ __forceinline__ uint32_t chunk_tiles(const SeqRange &s, const UnitShape &u, uint32_t ch) {
-  const uint32_t rows = s.n * u.G, last = (min((ch + 1) * u.RU, rows) - 1) / u.G;
-  const int32_t m = min(s.len, max(0, s.len - (int32_t)s.n + (int32_t)last + 1));
-  return max(1u, ((uint32_t)m + u.KT - 1) / u.KT);
+  const uint32_t end = u.tokens ? min((ch + 1) * u.tokens, s.n) : (min((ch + 1) * u.RU, s.n * u.G) - 1) / u.G + 1;
+  const int32_t m = min(s.len, max(0, s.len - (int32_t)s.n + (int32_t)end));
+  return max(1u, ((uint32_t)m + u.KT - 1) >> u.shift);
 }
 
 // Tiles of one kv head of a sequence's own units (0: none of this kernel's).
@@ -150,7 +158,7 @@ __device__ __forceinline__ TileSpan block_span(const BatchView &bv, const UnitSh
   s.pre = 0;
   if (u.prefix && bv.prefix_len) {
     const uint32_t nch = (batch_rows(bv, u.G) + u.RU - 1) / u.RU;
-    s.pre = u.KV * nch * ((bv.prefix_len + u.KT - 1) / u.KT);
+    s.pre = u.KV * nch * ((bv.prefix_len + u.KT - 1) >> u.shift);
   }
   s.total = s.pre + own;
   const uint32_t even = s.total / gridDim.x + (s.total % gridDim.x != 0);
@@ -223,7 +231,7 @@ struct PieceWalk {
     uint32_t a, n;
     if (cur < pre) {
       const uint32_t rows = batch_rows(bv, u.G), nch = (rows + u.RU - 1) / u.RU;
-      n = (bv.prefix_len + u.KT - 1) / u.KT;
+      n = (bv.prefix_len + u.KT - 1) >> u.shift;
       const uint32_t unit = cur / n;
       a = unit * n;
       p.kvh = unit / nch;

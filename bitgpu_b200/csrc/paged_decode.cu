@@ -596,7 +596,7 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_hi, bool p
   const uint32_t ps = a.kv.page_size;
   DecodeParams p;
   p.a = a;
-  p.u = UnitShape{a.G, a.kv.KV, 8 * NT, kTile, 0, rows_hi, prefix};
+  p.u = unit_shape(a.G, a.kv.KV, 8 * NT, kTile, 0, rows_hi, prefix);
   p.box = page_box(ps, kTile);
   p.ppt = kTile / p.box;
   p.join_rows = a.own_pieces != nullptr;

@@ -27,6 +27,25 @@ __global__ void __launch_bounds__(128) join_cuts_kernel(PagedAttnArgs a, uint32_
       a.gate, off);
 }
 
+// The same for units of many rows and few pieces (tcgen05 kernel): one warp per row.
+template <int D>
+__global__ void __launch_bounds__(128) join_cuts_wide_kernel(PagedAttnArgs a, uint32_t ru) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint32_t lane = threadIdx.x & 31, r = blockIdx.y * kWarps + (threadIdx.x >> 5);
+  const uint4 d = __ldcg(reinterpret_cast<const uint4 *>(a.cuts + blockIdx.x));
+  const CutUnit c{d.x, d.y, d.z, d.w};
+  if (c.npieces == 0 || r >= c.rows) return;
+  const uint32_t R = c.R0 + r, t = R / a.G, idx0 = a.slot0 + (2 * blockIdx.x + 1) * ru + r;
+  const uint64_t off = ((uint64_t)t * a.H + c.kvh * a.G + R % a.G) * D;
+  constexpr int NJ = (D + 127) / 128;
+  float acc[NJ][4], M, L;
+  join_pieces<D>(
+      a.part_o, a.part_ml, 0, 1, min(c.npieces, gridDim.x - blockIdx.x), lane,
+      [&](uint32_t k) { return (uint64_t)piece_index(idx0, ru, k); }, acc, M, L);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) write_out4(a.out, a.out_f16, a.gate, off + 4 * lane + 128 * j, acc[j], L);
+}
+
 template <int D>
 __global__ void __launch_bounds__(128) join_rows_kernel(PagedAttnArgs a) {
   __shared__ __align__(16) float sm[kWarps * (D + 2)];
@@ -60,6 +79,11 @@ int launch_dependent(K kern, dim3 grid, cudaStream_t st, A... args) {
 }  // namespace
 
 int launch_paged_join_cuts(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, cudaStream_t st) {
+  if (ru >= 128) {
+    const dim3 wide(blocks, ru / kWarps);
+    if (a.D == 128) return launch_dependent(join_cuts_wide_kernel<128>, wide, st, a, ru);
+    return BG_EUNSUPPORTED;
+  }
   const dim3 grid(blocks, ru);
   if (a.D == 128) return launch_dependent(join_cuts_kernel<128>, grid, st, a, ru);
   if (a.D == 256) return launch_dependent(join_cuts_kernel<256>, grid, st, a, ru);

@@ -29,6 +29,8 @@
 #include <cuda.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "paged.h"
 #include "paged_merge.cuh"
 #include "umma.cuh"
@@ -61,6 +63,8 @@ struct TcParams {
   UnitShape u;
   uint32_t box, ppt;  // positions of a page box, boxes per tile
   uint32_t join_rows;
+  uint32_t q_tma;     // f16 rows whose group divides 128: query tiles come by TMA
+  uint32_t wide;      // out and the partial rows start on 32-byte boundaries
 };
 
 struct alignas(16) TcInfo {
@@ -90,10 +94,28 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
+// N consecutive words of one row.  A row belongs to one thread, so a store instruction touches 32 rows:
+// 32-byte stores fill whole sectors (16-byte ones write every sector twice: 5.5 -> 2.5 us per 256 rows).
+template <int N>
+__device__ __forceinline__ void store_words(void *dst, const uint32_t (&w)[N], uint32_t wide) {
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<uint32_t *>(dst) + i),
+                   "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]),
+                   "r"(w[i + 7])
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<uint4 *>(static_cast<uint32_t *>(dst) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  }
+}
+
 template <int D, bool Q8, bool LO, int NQT>
 __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                    const __grid_constant__ TcParams p) {
+                    const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ TcParams p) {
   using C = TcCfg<D, Q8, LO, NQT>;
   constexpr int KT = C::KT, NQ = C::NQ, NK = C::NK;
   static_assert(D == 128, "two streams need two O tiles of 128 columns");
@@ -125,7 +147,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       mbar_init(&o_done[i], 1);
       mbar_init(&o_free[i], 128);
     }
-    mbar_init(q_full, 64);
+    mbar_init(q_full, !LO && p.q_tma ? 1 : 64);
     mbar_init(q_free, 1);
     mbar_init(info_free, 8);
     mbar_init(b_done, 128);
@@ -225,47 +247,36 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     // ---------------- MMA issuer ----------------
     if (lane == 0) {
       constexpr uint32_t idS = idesc_f16(KT, false), idO = idesc_f16(D, true);
-      auto one_s = [&](uint32_t slot, uint32_t q, uint32_t k, bool acc) {
+      constexpr uint32_t kHi = umma_desc_hi(1024);
+      const uint32_t q_lo = umma_desc_lo(sQ, 16), k_lo = umma_desc_lo(sK, 16), v_lo = umma_desc_lo(sV, KT * 128);
+      // one product over D (K steps of 16 values, 32 bytes of a 128-byte swizzle row)
+      auto one_s = [&](uint32_t slot, uint32_t q, uint32_t k, auto acc) {
+        umma_ss_lo<kHi, decltype(acc)::value>(slot, q, k, idS);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t da = umma_desc_sw128(q + (kk >> 2) * (kM * 128) + (kk & 3) * 32, 16, 1024);
-          const uint64_t db = umma_desc_sw128(k + (kk >> 2) * (KT * 128) + (kk & 3) * 32, 16, 1024);
-          umma_ss(tmem + slot, da, db, idS, acc || kk > 0);
-        }
+        for (int kk = 1; kk < D / 16; ++kk)
+          umma_ss_lo<kHi, true>(slot, q + ((kk >> 2) * (kM * 128) + (kk & 3) * 32) / 16,
+                                k + ((kk >> 2) * (KT * 128) + (kk & 3) * 32) / 16, idS);
       };
       // S = Q K^T: small products first, so that they are added up among themselves
       auto issue_s = [&](int t, int s) {
-        const uint32_t slot = t ? C::S1 : C::S0;
-        const uint32_t q = sQ + (NQT == 2 ? t : 0) * NQ * C::QT, k = sK + s * NK * C::KVT;
-        bool acc = false;
-        if constexpr (LO) {
-          one_s(slot, q + C::QT, k, acc);
-          acc = true;
-        }
-        if constexpr (Q8) {
-          one_s(slot, q, k + C::KVT, acc);
-          acc = true;
-        }
-        one_s(slot, q, k, acc);
+        const uint32_t slot = tmem + (t ? C::S1 : C::S0);
+        const uint32_t q = q_lo + (NQT == 2 ? t : 0) * (NQ * C::QT / 16), k = k_lo + s * (NK * C::KVT / 16);
+        if constexpr (LO) one_s(slot, q + C::QT / 16, k, std::false_type{});
+        if constexpr (Q8) one_s(slot, q, k + C::KVT / 16, std::bool_constant<LO>{});
+        one_s(slot, q, k, std::bool_constant<LO || Q8>{});
       };
       auto one_pv = [&](uint32_t o, uint32_t pa, uint32_t v, bool acc) {
+        if (acc) umma_ts_lo<kHi, true>(o, pa, v, idO);
+        else umma_ts_lo<kHi, false>(o, pa, v, idO);
 #pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk) {
-          const uint64_t dv = umma_desc_sw128(v + kk * 16 * 128, KT * 128, 1024);
-          umma_ts(tmem + o, tmem + pa + kk * 8, dv, idO, (acc || kk > 0) ? 1u : 0u);
-        }
+        for (int kk = 1; kk < KT / 16; ++kk) umma_ts_lo<kHi, true>(o, pa + kk * 8, v + kk * (16 * 128 / 16), idO);
       };
+      // O += P V (P from TMEM)
       auto issue_pv = [&](int t, int s, bool acc) {
-        const uint32_t slot = t ? C::S1 : C::S0, o = t ? C::O1 : C::O0, v = sV + s * NK * C::KVT;
-        if constexpr (LO) {
-          one_pv(o, slot + KT / 2, v, acc);
-          acc = true;
-        }
-        if constexpr (Q8) {
-          one_pv(o, slot, v + C::KVT, acc);
-          acc = true;
-        }
-        one_pv(o, slot, v, acc);
+        const uint32_t slot = tmem + (t ? C::S1 : C::S0), o = tmem + (t ? C::O1 : C::O0), v = v_lo + s * (NK * C::KVT / 16);
+        if constexpr (LO) one_pv(o, slot + KT / 2, v, acc);
+        if constexpr (Q8) one_pv(o, slot, v + C::KVT / 16, LO || acc);
+        one_pv(o, slot, v, LO || Q8 || acc);
       };
       bool ok = true;
       int it = 0;               // tiles of all pieces before this one
@@ -354,6 +365,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     walk.init(span, a.bv, p.u, ps);
     Piece pc;
     bool ok = true;
+    uint32_t loaded = 0;  // pieces whose query tile was asked for
     if (a.cuts && gt == 0) a.cuts[blockIdx.x].npieces = 0;
     for (uint32_t piece = 0; ok; ++piece) {
       const bool more = walk.next(pc, a.bv, p.u, ps);
@@ -363,7 +375,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       }
       if (!more) {
         if (gt == 0) info->ntiles = 0;
-        mbar_arrive(q_full);
+        if (LO || !p.q_tma || gt == 0) mbar_arrive(q_full);
         break;
       }
       const bool whole = pc.npieces == 1;
@@ -388,40 +400,66 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
           rp[r] = RowPieces{whole ? row0 + R / a.G * a.H + pc.kvh * a.G + R % a.G : slot + r, pc.npieces, p.u.RU, 0};
         }
       }
+      if (!LO && p.q_tma) {
+        // rows behind the unit's are other sequences' (or zeros): computed along, never written
+        loaded = piece + 1;
+        if (gt == 0) {
+          mbar_expect_tx(q_full, NQT * C::QT);
+          const int tok = (int)(pc.R0 / a.G), per = kM / (int)a.G;
+          for (int q = 0; q < NQT; ++q)
+            for (int cb = 0; cb < D / 64; ++cb)
+              tma_load_4d(smem + C::oQ + q * C::QT + cb * kM * 128, &tmQ, q_full, cb * 64, 0, (int)pc.kvh, tok + q * per);
+        }
+        continue;
+      }
+      // a thread has one 16-byte column of every fourth row; (token, head) step along without divisions
       constexpr int CPR = D / 8;  // chunks of 8 values per row
-      constexpr int NIT = NQT * kM * CPR / 64;
+      constexpr int RS = 64 / CPR, NIT = NQT * kM / RS;
+      const uint32_t c = gt % CPR, up_t = RS / a.G, up_g = RS % a.G;
+      uint32_t r = gt / CPR, tok = (pc.R0 + r) / a.G, g = (pc.R0 + r) % a.G;
+      auto step = [&]() {
+        r += RS;
+        tok += up_t;
+        g += up_g;
+        if (g >= a.G) {
+          g -= a.G;
+          ++tok;
+        }
+      };
+      const uint32_t head0 = pc.kvh * a.G;
       if constexpr (!LO) {
 #pragma unroll 4
         for (int i = 0; i < NIT; ++i) {
-          const uint32_t idx = gt + i * 64, r = idx / CPR, c = idx % CPR, R = pc.R0 + r;
           const bool there = r < pc.rows;
-          const uint64_t off = there ? ((uint64_t)(R / a.G) * a.H + pc.kvh * a.G + R % a.G) * CPR + c : 0;
+          const uint64_t off = there ? ((uint64_t)tok * a.H + head0 + g) * CPR + c : 0;
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sQ + (r >> 7) * C::QT + sw_off<kM>(r & 127, c)),
                        "l"(static_cast<const uint4 *>(a.q) + off), "r"(there ? 16u : 0u)
                        : "memory");
+          step();
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
       } else {
 #pragma unroll 1
         for (int i0 = 0; i0 < NIT; i0 += 4) {
           float x[4][8];
+          const uint32_t r0 = r;
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const uint32_t idx = gt + (i0 + u) * 64, r = idx / CPR, c = idx % CPR, R = pc.R0 + r;
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[u][j] = 0.f;
             if (r < pc.rows) {
-              const uint64_t off = ((uint64_t)(R / a.G) * a.H + pc.kvh * a.G + R % a.G) * D + c * 8;
+              const uint64_t off = ((uint64_t)tok * a.H + head0 + g) * D + c * 8;
               if (a.q_f16) load_f16<8>(static_cast<const __half *>(a.q) + off, x[u]);
               else load_f32<8>(static_cast<const float *>(a.q) + off, x[u]);
             }
+            step();
           }
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const uint32_t idx = gt + (i0 + u) * 64, r = idx / CPR, c = idx % CPR;
             uint4 hi, lo;
             split8(x[u], hi, lo);
-            unsigned char *d = smem + C::oQ + (r >> 7) * NQ * C::QT + sw_off<kM>(r & 127, c);
+            const uint32_t rr = r0 + u * RS;
+            unsigned char *d = smem + C::oQ + (rr >> 7) * NQ * C::QT + sw_off<kM>(rr & 127, c);
             *reinterpret_cast<uint4 *>(d) = hi;
             *reinterpret_cast<uint4 *>(d + C::QT) = lo;
           }
@@ -430,7 +468,11 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       fence_async_smem();
       mbar_arrive(q_full);
     }
-    if (!ok) *abort_flag = 1;
+    if (!ok) {
+      *abort_flag = 1;
+      // no query tile may still be in flight when the block exits (otherwise q_free is behind it)
+      if (!LO && p.q_tma && gt == 0 && loaded) mbar_wait(q_full, (loaded - 1) & 1);
+    }
   }
   } else if (warp < 12) {
     // ---------------- softmax (one row per thread) ----------------
@@ -554,6 +596,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         L = l * f0 + ml.y * f1;
       }
       tc_fence_after();
+      const float inv = L != 0.f ? 1.0f / L : 0.f;  // a row that attends nothing is zero
       const bool valid = r < in.rows;
       const uint64_t orow = (uint64_t)(R / a.G) * a.H + in.kvh * a.G + R % a.G;
       const uint64_t prow = in.dest == kRowBuf ? in.row0 + orow : in.dest + r;
@@ -576,12 +619,30 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
           }
         }
         if (!valid) continue;
+        if (in.dest != kDirect) {
+          store_words<32>(a.part_o + prow * D + c * 32, o, p.wide);
+          continue;
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float v[4] = {__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
-                              __uint_as_float(o[4 * i + 3])};
-          if (in.dest == kDirect) write_out4(a.out, a.out_f16, a.gate, orow * D + c * 32 + i * 4, v, L);
-          else *reinterpret_cast<float4 *>(a.part_o + prow * D + c * 32 + i * 4) = make_float4(v[0], v[1], v[2], v[3]);
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+        if (a.gate) {
+          const float4 *g = reinterpret_cast<const float4 *>(a.gate + orow * D + c * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 x = __ldg(g + i);
+            o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) / (1.0f + expf(-x.x)));
+            o[4 * i + 1] = __float_as_uint(__uint_as_float(o[4 * i + 1]) / (1.0f + expf(-x.y)));
+            o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) / (1.0f + expf(-x.z)));
+            o[4 * i + 3] = __float_as_uint(__uint_as_float(o[4 * i + 3]) / (1.0f + expf(-x.w)));
+          }
+        }
+        if (a.out_f16) {
+          uint32_t h[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) h[i] = pack_half2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+          store_words<16>(static_cast<__half *>(a.out) + orow * D + c * 32, h, p.wide);
+        } else {
+          store_words<32>(static_cast<float *>(a.out) + orow * D + c * 32, o, p.wide);
         }
       }
       if (valid && in.dest != kDirect) a.part_ml[prow] = make_float2(M - kUp, L);
@@ -676,11 +737,19 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_lo, bool p
   TcParams p;
   p.a = a;
   // a launch has either the prefix's units or the sequences' own
-  p.u = UnitShape{a.G, a.kv.KV, NQT * kM, C::KT, prefix ? 0xffffffffu : rows_lo, 0xffffffffu, prefix};
+  p.u = unit_shape(a.G, a.kv.KV, NQT * kM, C::KT, prefix ? 0xffffffffu : rows_lo, 0xffffffffu, prefix);
   p.box = page_box(ps, C::KT);
   p.ppt = C::KT / p.box;
   p.join_rows = a.own_pieces != nullptr;
-  CUtensorMap tk = {}, tv = {};
+  CUtensorMap tk = {}, tv = {}, tq = {};
+  p.q_tma = !LO && kM % a.G == 0;
+  p.wide = (((uintptr_t)a.out | (uintptr_t)a.part_o) & 31) == 0;
+  if (p.q_tma) {
+    const uint64_t dims[4] = {D, a.G, a.kv.KV, a.bv.T};
+    const uint64_t strides[3] = {D * 2, (uint64_t)a.G * D * 2, (uint64_t)a.H * D * 2};
+    const uint32_t box[4] = {64, a.G, 1, kM / a.G};
+    if (make_tmap_4d(&tq, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return BG_EUNSUPPORTED;
+  }
   if (!Q8) {
     const uint64_t rb = (uint64_t)D * 2;
     const uint64_t dims[4] = {D, a.kv.KV, ps, a.kv.num_pages};
@@ -703,7 +772,7 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_lo, bool p
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, tk, tv, p) == cudaSuccess ? BG_OK : BG_ELAUNCH;
+  return cudaLaunchKernelEx(&cfg, kern, tk, tv, tq, p) == cudaSuccess ? BG_OK : BG_ELAUNCH;
 }
 
 template <bool Q8>

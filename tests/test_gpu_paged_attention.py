@@ -16,6 +16,7 @@ def ops():
 
 def run(ops, r, q_dtype=torch.float32, out_dtype=torch.float32, gated=False, scale=0.0, max_q=None, what=""):
     q = r.queries(q_dtype)
+    q[r.cu[-1]:] = float("nan")
     gate = torch.randn(q.shape, generator=r.g) if gated else None
     want = r.attention(q, gate, scale or None)
     out = torch.full(q.shape, 7.0, dtype=out_dtype, device="cuda")
@@ -121,6 +122,8 @@ def test_prefix_tokens(ops, io):
 def test_padding_rows(ops):
     run(ops, Ragged([33, 70], [2, 3], pad=7, seed=1))
     run(ops, Ragged([33, 70], [2, 3], pad=300, prefix=65, seed=1))
+    for io in DT.values():
+        run(ops, Ragged([190, 70], [90, 33], pad=40, prefix=165, seed=1), io, io)
 
 
 @pytest.mark.parametrize("io", ["f32", "f16"])
