@@ -10,8 +10,9 @@
 //   NQT = 2 (256 rows): stream t is rows [128 t, 128 t + 128) and both use every K/V tile;
 //   NQT = 1 (128 rows): the streams take even and odd K/V tiles of the same rows, and their outputs are
 //           joined at the end (stream 0 reads both from TMEM).
-// The MMA thread issues PV_t(i) and right behind it the next S_t, which overwrites the columns that P_t was
-// read from: MMAs of one thread execute in order, and the commit behind S_t covers PV_t too.
+// Each stream has two score slots of 64 columns, so that the next scores are there when a softmax step ends.
+// The MMA thread issues PV_t and right behind it the S_t that takes over its slot (P overwrote the scores in
+// place): MMAs of one thread execute in order.
 //
 // Precision, by the types of the call:
 //   f16 rows, f16 pool: operands are exact, P is rounded once to f16 (kept 2^6 up, away from subnormals);
@@ -21,9 +22,10 @@
 //           error of f16 rows; the extra products cost less than that here, because the softmax warps
 //           and not the tensor pipe set the pace of the single-product form.)
 //
-// Warp roles: warp 0 TMA producer of K and V (f16 pool; page boxes, 128-byte swizzle), warp 1 MMA issuer,
-// warps 2-3 load the next unit's query rows as soon as the last S of the current one is done, warps 4-11
-// softmax (one row per thread), warps 12-15 (q8 pool) dequantise, one tile ahead in registers.
+// Warp roles: warp 0 TMA producer of K and V (f16 pool; page boxes, 128-byte swizzle), warp 1 MMA issue of
+// stream 0, warps 2-3 bring the next unit's query rows as soon as the last S of the current one is done,
+// warps 4-11 softmax (one row per thread).  MMA issue of stream 1: warp 12, or with a q8 pool warp 0, where
+// warps 12-15 dequantise, one tile ahead in registers.
 // All waits are bounded; on expiry the block records BG_ETIMEOUT, stops issuing, waits for what it issued,
 // frees its TMEM and exits.
 #include <cuda.h>
@@ -46,15 +48,15 @@ template <int D, bool Q8, bool LO, int NQT>
 struct TcCfg {
   static constexpr int NQ = LO ? 2 : 1, NK = Q8 ? 2 : 1;     // operand halves
   static constexpr int QT = kM * D * 2;                      // bytes of one f16 query tile
-  static constexpr int KT = D == 128 ? (Q8 ? 64 : 128) : (Q8 || LO ? 32 : 64);
+  static constexpr int KT = 64;
   static constexpr int KVT = KT * D * 2;                     // bytes of one f16 K (or V) tile
-  static constexpr int oQ = 0, oK = NQT * NQ * QT, oV = oK + 2 * NK * KVT, oB = oV + 2 * NK * KVT;
-  static constexpr int oInfo = oB + 256, oML = oInfo + 64, oScan = oML + kM * 8;
+  static constexpr int NST = Q8 ? 2 : 4;                     // ring stages of K and of V
+  static constexpr int oQ = 0, oK = NQT * NQ * QT, oV = oK + NST * NK * KVT, oB = oV + NST * NK * KVT;
+  static constexpr int oInfo = oB + 384, oML = oInfo + 64, oScan = oML + kM * 8;
   static constexpr int SMEM = oScan + 20 * 8;
-  static constexpr int THREADS = Q8 ? 512 : 384;
-  static constexpr uint32_t S0 = 0, S1 = KT < 128 ? 64 : 128, O0 = D == 128 ? 256 : 0, O1 = 384;
-
-
+  static constexpr int THREADS = 512;
+  // TMEM columns: score slot u of stream t at (2t + u) * KT, outputs behind them
+  static constexpr uint32_t O0 = 256, O1 = 384;
   static_assert(SMEM <= 232448, "shared memory");
 };
 
@@ -94,6 +96,35 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
+// Codes of one block scale s as two f16 halves of code * s / 127, in packed f16 arithmetic.  With
+// s / 127 = m 2^e and m = mh + ml in f16:  c' = code 2^e is exact (byte + 128 under the pattern 0x64xx is
+// 1152 + code, and one fused multiply-add removes the 1152 and applies 2^e);  hi = c' mh rounded;
+// c' mh - hi is exact in f16, so  lo = c' ml + (c' mh - hi)  carries the rest to 2^-22 of the value.
+struct CodeScale {
+  __half2 p2, bias, mh, ml;
+  __device__ __forceinline__ explicit CodeScale(float s) {
+    const float x = s * (1.0f / 127.0f);
+    const int e = min(4, max(-20, (int)((__float_as_uint(x) >> 23) & 255) - 127));
+    const float m = x * __uint_as_float((uint32_t)(127 - e) << 23), f = __uint_as_float((uint32_t)(127 + e) << 23);
+    p2 = __float2half2_rn(f);
+    bias = __float2half2_rn(-1152.0f * f);
+    mh = __float2half2_rn(m);
+    ml = __float2half2_rn(m - __low2float(mh));
+  }
+  // the four codes of a word, in order
+  __device__ __forceinline__ void split4(uint32_t w, uint32_t &h0, uint32_t &h1, uint32_t &l0, uint32_t &l1) const {
+    const uint32_t b = w ^ 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t x = __byte_perm(b, 0x64646464u, i ? 0x4342 : 0x4140);
+      const __half2 c = __hfma2(*reinterpret_cast<const __half2 *>(&x), p2, bias);
+      const __half2 h = __hmul2(c, mh), r = __hfma2(c, mh, __hneg2(h)), l = __hfma2(c, ml, r);
+      (i ? h1 : h0) = *reinterpret_cast<const uint32_t *>(&h);
+      (i ? l1 : l0) = *reinterpret_cast<const uint32_t *>(&l);
+    }
+  }
+};
+
 // N consecutive words of one row.  A row belongs to one thread, so a store instruction touches 32 rows:
 // 32-byte stores fill whole sectors (16-byte ones write every sector twice: 5.5 -> 2.5 us per 256 rows).
 template <int N>
@@ -121,12 +152,13 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   static_assert(D == 128, "two streams need two O tiles of 128 columns");
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::oB);
-  uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;
-  uint64_t *q_full = bars + 8, *q_free = bars + 9, *info_free = bars + 10;
-  uint64_t *s_full = bars + 11, *p_full = bars + 13, *o_done = bars + 15, *o_free = bars + 17;
-  uint64_t *b_done = bars + 19, *mma_done = bars + 20, *tail = bars + 21;
-  uint32_t *tmem_at = reinterpret_cast<uint32_t *>(bars + 22);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 23);
+  uint64_t *k_full = bars, *k_empty = bars + 4, *v_full = bars + 8, *v_empty = bars + 12;
+  uint64_t *q_full = bars + 16, *q_free = bars + 17, *info_free = bars + 18;
+  uint64_t *s_full = bars + 19, *p_full = bars + 23;  // per score slot 2t + u
+  uint64_t *pv_done = bars + 27, *o_free = bars + 29; // per stream
+  uint64_t *b_done = bars + 31, *tail = bars + 32, *mma_done = bars + 33;
+  uint32_t *tmem_at = reinterpret_cast<uint32_t *>(bars + 35);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 36);
   TcInfo *info = reinterpret_cast<TcInfo *>(smem + C::oInfo);
   float2 *ml_s = reinterpret_cast<float2 *>(smem + C::oML);
   const PagedAttnArgs &a = p.a;
@@ -137,21 +169,23 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   }
 
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&k_full[i], Q8 ? 4 : 1);
       mbar_init(&v_full[i], Q8 ? 4 : 1);
-      mbar_init(&k_empty[i], 1);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&k_empty[i], NQT);  // streams that read the tile
+      mbar_init(&v_empty[i], NQT);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 128);
-      mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&pv_done[i], 1);
       mbar_init(&o_free[i], 128);
+      mbar_init(&mma_done[i], 1);
     }
     mbar_init(q_full, !LO && p.q_tma ? 1 : 64);
-    mbar_init(q_free, 1);
+    mbar_init(q_free, 2);
     mbar_init(info_free, 8);
     mbar_init(b_done, 128);
-    mbar_init(mma_done, 1);
     mbar_init(tail, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -173,12 +207,122 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   const uint32_t sQ = smem_u32(smem + C::oQ), sK = smem_u32(smem + C::oK), sV = smem_u32(smem + C::oV);
   const uint32_t ps = a.kv.page_size;
 
-  // registers: 384 threads: 128*72 + 256*216 = 384*168; 512: 128*72 + 256*168 + 128*104 = 512*128
+  // ---------------- MMA issue of stream t (one warp per stream) ----------------
+  // The whole warp runs the loop and one elected lane issues: so the compiler knows every operand to be
+  // uniform (run by one lane under a branch, each MMA first moves its descriptors to uniform registers).
+  // One warp per stream: a warp needs ~100 cycles for each barrier that it looks at, done or not, and the
+  // queue of the tensor pipe is too short to bridge that; the other stream's MMAs do.
+  auto mma_loop = [&](auto stream) {
+    constexpr int t = decltype(stream)::value;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+    constexpr uint32_t idS = idesc_f16(KT, false), idO = idesc_f16(D, true);
+    constexpr uint32_t kHi = umma_desc_hi(1024);
+    const uint32_t q_lo = umma_desc_lo(sQ, 16) + (NQT == 2 ? t : 0) * (NQ * C::QT / 16);
+    const uint32_t k_lo = umma_desc_lo(sK, 16), v_lo = umma_desc_lo(sV, KT * 128), o = tmem + (t ? C::O1 : C::O0);
+    // one product over D (K steps of 16 values, 32 bytes of a 128-byte swizzle row)
+    auto one_s = [&](uint32_t slot, uint32_t q, uint32_t k, auto acc) {
+      umma_ss_lo<kHi, decltype(acc)::value>(slot, q, k, idS);
+#pragma unroll
+      for (int kk = 1; kk < D / 16; ++kk)
+        umma_ss_lo<kHi, true>(slot, q + ((kk >> 2) * (kM * 128) + (kk & 3) * 32) / 16,
+                              k + ((kk >> 2) * (KT * 128) + (kk & 3) * 32) / 16, idS);
+    };
+    // S = Q K^T into slot u: small products first, so that they are added up among themselves
+    auto issue_s = [&](int u, int s) {
+      const uint32_t slot = tmem + (2 * t + u) * KT, k = k_lo + s * (NK * C::KVT / 16);
+      if constexpr (LO) one_s(slot, q_lo + C::QT / 16, k, std::false_type{});
+      if constexpr (Q8) one_s(slot, q_lo, k + C::KVT / 16, std::bool_constant<LO>{});
+      one_s(slot, q_lo, k, std::bool_constant<LO || Q8>{});
+    };
+    auto one_pv = [&](uint32_t pa, uint32_t v, bool acc) {
+      if (acc) umma_ts_lo<kHi, true>(o, pa, v, idO);
+      else umma_ts_lo<kHi, false>(o, pa, v, idO);
+#pragma unroll
+      for (int kk = 1; kk < KT / 16; ++kk) umma_ts_lo<kHi, true>(o, pa + kk * 8, v + kk * (16 * 128 / 16), idO);
+    };
+    // O_t += P V (P from the slot's columns)
+    auto issue_pv = [&](int u, int s, bool acc) {
+      const uint32_t slot = tmem + (2 * t + u) * KT, v = v_lo + s * (NK * C::KVT / 16);
+      if constexpr (LO) one_pv(slot + KT / 2, v, acc);
+      if constexpr (Q8) one_pv(slot, v + C::KVT / 16, LO || acc);
+      one_pv(slot, v, LO || Q8 || acc);
+    };
+    constexpr int STEP = 3 - NQT, FIRST = NQT == 2 ? 0 : t;  // this stream's tiles: FIRST, FIRST + STEP, ...
+    bool ok = true;
+    int it = 0;         // tiles of all pieces before this one
+    uint32_t pp = 0;    // next phase parity of p_full, one bit per slot
+    for (uint32_t piece = 0; ok; ++piece) {
+      if (!mbar_wait_warp(q_full, piece & 1)) { ok = false; break; }
+      const int n = (int)__shfl_sync(0xffffffffu, info->ntiles, 0);
+      if (n == 0) break;
+      tc_fence_after();
+      auto stage = [&](int i) { return (it + i) % C::NST; };
+      auto wait_k = [&](int i) { return mbar_wait_warp(&k_full[stage(i)], ((it + i) / C::NST) & 1); };
+      auto wait_v = [&](int i) { return mbar_wait_warp(&v_full[stage(i)], ((it + i) / C::NST) & 1); };
+      auto after_s = [&](int i, int u) {
+        umma_commit(&s_full[2 * t + u]);
+        umma_commit(&k_empty[stage(i)]);
+        if (i + STEP >= n) umma_commit(q_free);  // this stream's last S of the piece
+      };
+      if (FIRST >= n && elect_one()) umma_commit(q_free);  // no tile for this stream
+      __syncwarp();
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const int i = FIRST + a * STEP;
+        if (!ok || i >= n) break;
+        ok = wait_k(i);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_s(a, stage(i));
+          after_s(i, a);
+        }
+        __syncwarp();
+      }
+      // PV(i), and behind it the S that takes over its slot: in-order execution keeps P safe
+      for (int i = FIRST, u = 0; ok && i < n; i += STEP, u ^= 1) {
+        const bool more = i + 2 * STEP < n;
+        ok = wait_v(i);
+        if (ok && i == FIRST && piece > 0) ok = mbar_wait_warp(&o_free[NQT == 2 ? t : 0], (piece - 1) & 1);
+        ok = ok && mbar_wait_warp(&p_full[2 * t + u], (pp >> u) & 1);
+        if (!ok) break;
+        pp ^= 1u << u;
+        tc_fence_after();
+        if (elect_one()) {
+          issue_pv(u, stage(i), i > FIRST);
+          umma_commit(&pv_done[t]);
+          umma_commit(&v_empty[stage(i)]);
+        }
+        __syncwarp();
+        if (more) {
+          // (only now: the ring may not hold this K before V(i) has been used)
+          ok = wait_k(i + 2 * STEP);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            issue_s(u, stage(i + 2 * STEP));
+            after_s(i + 2 * STEP, u);
+          }
+          __syncwarp();
+        }
+      }
+      it += n;
+    }
+    if (!ok) *abort_flag = 1;
+    // every MMA must complete before the block frees its TMEM
+    if (elect_one()) umma_commit(&mma_done[t]);
+    __syncwarp();
+    mbar_wait_warp(&mma_done[t], 0);
+  };
+
+  // registers: 128*72 + 256*168 + 128*104 = 512*128
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
   if (warp == 0) {
     // ---------------- TMA producer (f16 pool) ----------------
-    if constexpr (!Q8) {
+    if constexpr (Q8) {
+      mma_loop(std::integral_constant<int, 1>{});
+    } else {
       PieceWalk walk;
       walk.init(span, a.bv, p.u, ps);
       Piece pc;
@@ -197,10 +341,10 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         for (uint32_t t = 0; ok && t < pc.ntiles; ++t, ++it) {
           const uint32_t pg = pg_next;
           pg_next = page_of(t + 1);
-          const int s = it & 1;
-          const uint32_t pos0 = (pc.tile0 + t) * KT, par = ((it >> 1) - 1) & 1;
+          const int s = it % C::NST;
+          const uint32_t pos0 = (pc.tile0 + t) * KT, par = ((it / C::NST) - 1) & 1;
           const int y = (int)((pos0 + lane * p.box) % ps);
-          if (it >= 2) ok = mbar_wait_warp(&k_empty[s], par);
+          if (it >= C::NST) ok = mbar_wait_warp(&k_empty[s], par);
           if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
           if (lane == 0) mbar_expect_tx(&k_full[s], C::KVT);
           __syncwarp();
@@ -209,7 +353,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
               tma_load_4d(smem + C::oK + s * C::KVT + cb * KT * 128 + lane * p.box * 128, &tmK, &k_full[s], cb * 64,
                           (int)pc.kvh, y, (int)pg);
           kdone = it + 1;
-          if (it >= 2) ok = mbar_wait_warp(&v_empty[s], par);
+          if (it >= C::NST) ok = mbar_wait_warp(&v_empty[s], par);
           if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
           // slots of the last page behind the length may hold NaN, and 0 * NaN is NaN: such a tile
           // arrives on its own barrier, its rows behind the length are cleared, then it is handed on
@@ -239,125 +383,12 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       if (!ok && lane == 0) *abort_flag = 1;
       // no copy may still be in flight when the block exits
       if (lane == 0) {
-        for (int i = max(0, kdone - 2); i < kdone; ++i) mbar_wait(&k_full[i & 1], (i >> 1) & 1);
-        for (int i = max(0, vdone - 2); i < vdone; ++i) mbar_wait(&v_full[i & 1], (i >> 1) & 1);
+        for (int i = max(0, kdone - C::NST); i < kdone; ++i) mbar_wait(&k_full[i % C::NST], (i / C::NST) & 1);
+        for (int i = max(0, vdone - C::NST); i < vdone; ++i) mbar_wait(&v_full[i % C::NST], (i / C::NST) & 1);
       }
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0) {
-      constexpr uint32_t idS = idesc_f16(KT, false), idO = idesc_f16(D, true);
-      constexpr uint32_t kHi = umma_desc_hi(1024);
-      const uint32_t q_lo = umma_desc_lo(sQ, 16), k_lo = umma_desc_lo(sK, 16), v_lo = umma_desc_lo(sV, KT * 128);
-      // one product over D (K steps of 16 values, 32 bytes of a 128-byte swizzle row)
-      auto one_s = [&](uint32_t slot, uint32_t q, uint32_t k, auto acc) {
-        umma_ss_lo<kHi, decltype(acc)::value>(slot, q, k, idS);
-#pragma unroll
-        for (int kk = 1; kk < D / 16; ++kk)
-          umma_ss_lo<kHi, true>(slot, q + ((kk >> 2) * (kM * 128) + (kk & 3) * 32) / 16,
-                                k + ((kk >> 2) * (KT * 128) + (kk & 3) * 32) / 16, idS);
-      };
-      // S = Q K^T: small products first, so that they are added up among themselves
-      auto issue_s = [&](int t, int s) {
-        const uint32_t slot = tmem + (t ? C::S1 : C::S0);
-        const uint32_t q = q_lo + (NQT == 2 ? t : 0) * (NQ * C::QT / 16), k = k_lo + s * (NK * C::KVT / 16);
-        if constexpr (LO) one_s(slot, q + C::QT / 16, k, std::false_type{});
-        if constexpr (Q8) one_s(slot, q, k + C::KVT / 16, std::bool_constant<LO>{});
-        one_s(slot, q, k, std::bool_constant<LO || Q8>{});
-      };
-      auto one_pv = [&](uint32_t o, uint32_t pa, uint32_t v, bool acc) {
-        if (acc) umma_ts_lo<kHi, true>(o, pa, v, idO);
-        else umma_ts_lo<kHi, false>(o, pa, v, idO);
-#pragma unroll
-        for (int kk = 1; kk < KT / 16; ++kk) umma_ts_lo<kHi, true>(o, pa + kk * 8, v + kk * (16 * 128 / 16), idO);
-      };
-      // O += P V (P from TMEM)
-      auto issue_pv = [&](int t, int s, bool acc) {
-        const uint32_t slot = tmem + (t ? C::S1 : C::S0), o = tmem + (t ? C::O1 : C::O0), v = v_lo + s * (NK * C::KVT / 16);
-        if constexpr (LO) one_pv(o, slot + KT / 2, v, acc);
-        if constexpr (Q8) one_pv(o, slot, v + C::KVT / 16, LO || acc);
-        one_pv(o, slot, v, LO || Q8 || acc);
-      };
-      bool ok = true;
-      int it = 0;               // tiles of all pieces before this one
-      uint32_t np[2] = {0, 0};  // P tiles consumed per stream
-      for (uint32_t piece = 0; ok; ++piece) {
-        if (!mbar_wait(q_full, piece & 1)) { ok = false; break; }
-        const int n = (int)info->ntiles;
-        if (n == 0) break;
-        tc_fence_after();
-        auto wait_k = [&](int i) { return mbar_wait(&k_full[(it + i) & 1], ((it + i) >> 1) & 1); };
-        auto wait_v = [&](int i) { return mbar_wait(&v_full[(it + i) & 1], ((it + i) >> 1) & 1); };
-        auto wait_o = [&](int t) { return piece == 0 || mbar_wait(&o_free[NQT == 2 ? t : 0], (piece - 1) & 1); };
-        if constexpr (NQT == 2) {
-          ok = wait_k(0);
-          if (!ok) break;
-          tc_fence_after();
-          for (int t = 0; t < 2; ++t) {
-            issue_s(t, it & 1);
-            umma_commit(&s_full[t]);
-          }
-          umma_commit(&k_empty[it & 1]);
-          if (n == 1) umma_commit(q_free);
-          for (int i = 0; ok && i < n; ++i) {
-            for (int t = 0; ok && t < 2; ++t) {
-              ok = mbar_wait(&p_full[t], np[t]++ & 1) && (i > 0 || wait_o(t)) && (t > 0 || wait_v(i));
-              if (!ok) break;
-              tc_fence_after();
-              issue_pv(t, (it + i) & 1, i > 0);
-              if (t == 1) umma_commit(&v_empty[(it + i) & 1]);
-              if (i + 1 < n) {
-                if (t == 0) ok = wait_k(i + 1);
-                if (!ok) break;
-                tc_fence_after();
-                issue_s(t, (it + i + 1) & 1);
-                umma_commit(&s_full[t]);
-                if (t == 1) {
-                  umma_commit(&k_empty[(it + i + 1) & 1]);
-                  if (i + 2 == n) umma_commit(q_free);
-                }
-              } else {
-                umma_commit(&o_done[t]);
-              }
-            }
-          }
-        } else {
-          for (int i = 0; ok && i < 2 && i < n; ++i) {
-            ok = wait_k(i);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(i, (it + i) & 1);
-            umma_commit(&s_full[i]);
-            umma_commit(&k_empty[(it + i) & 1]);
-            if (i + 1 == n) umma_commit(q_free);
-          }
-          for (int i = 0; ok && i < n; ++i) {
-            const int t = i & 1;
-            ok = mbar_wait(&p_full[t], np[t]++ & 1) && (i > 1 || wait_o(t)) && wait_v(i);
-            if (!ok) break;
-            tc_fence_after();
-            issue_pv(t, (it + i) & 1, i > 1);
-            umma_commit(&v_empty[(it + i) & 1]);
-            if (i + 2 < n) {
-              ok = wait_k(i + 2);
-              if (!ok) break;
-              tc_fence_after();
-              issue_s(t, (it + i) & 1);
-              umma_commit(&s_full[t]);
-              umma_commit(&k_empty[(it + i) & 1]);
-              if (i + 3 == n) umma_commit(q_free);
-            } else {
-              umma_commit(&o_done[t]);
-            }
-          }
-        }
-        it += n;
-      }
-      if (!ok) *abort_flag = 1;
-      // every MMA must complete before the block frees its TMEM
-      umma_commit(mma_done);
-      mbar_wait(mma_done, 0);
-    }
+    mma_loop(std::integral_constant<int, 0>{});
   } else {
     // ---------------- query rows and descriptions ----------------
     const int gt = (warp - 2) * 32 + lane;
@@ -476,17 +507,15 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   }
   } else if (warp < 12) {
     // ---------------- softmax (one row per thread) ----------------
-    if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;" ::: "memory");
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;" ::: "memory");
     const int t = (warp - 4) >> 2;                // stream
     const int row = ((warp & 3) << 5) + lane;     // TMEM lane
     const uint32_t lane_off = (uint32_t)((warp & 3) << 5) << 16;
-    const uint32_t sbase = (tmem + (t ? C::S1 : C::S0)) | lane_off;
     const uint32_t obase = (tmem + (t ? C::O1 : C::O0)) | lane_off;
     const float sl2 = a.sl2;
     bool ok = true;
-    uint32_t ns = 0, nd = 0;  // score tiles and finished outputs of this stream
-    uint32_t nd1 = 0;         // finished outputs of stream 1, counted by stream 0 (NQT = 1)
+    uint32_t sp = 0;           // next phase parity of s_full, one bit per slot of this stream
+    uint32_t nv = 0;           // this stream's PVs of the pieces before
     for (uint32_t piece = 0;; ++piece) {
       if (!mbar_wait_warp(q_full, piece & 1)) { ok = false; break; }
       const TcInfo in = *info;
@@ -500,8 +529,11 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       const int step = NQT == 2 ? 1 : 2;
       const int first = NQT == 2 ? 0 : t;
       for (int j = first; j < (int)in.ntiles; j += step) {
-        if (!mbar_wait_warp(&s_full[t], ns++ & 1)) { ok = false; break; }
+        const int u = (NQT == 2 ? j : j >> 1) & 1, jj = NQT == 2 ? j : j >> 1;
+        if (!mbar_wait_warp(&s_full[2 * t + u], (sp >> u) & 1)) { ok = false; break; }
+        sp ^= 1u << u;
         tc_fence_after();
+        const uint32_t sbase = (tmem + (2 * t + u) * KT) | lane_off;
         const int key0 = (int)(in.tile0 + j) * KT;
         const int nvalid = min(KT, max(0, lim - key0 + 1));
         uint32_t x[KT / 32][32];  // the whole score row: one TMEM wait per tile
@@ -528,10 +560,17 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], fmaxf(mx8[5], fmaxf(mx8[6], mx8[7]))));
         const float mt = mx * sl2;
         // lazy rescale: the whole warp takes the TMEM round trip when any of its rows moved far; rows
-        // that did not use the factor 1.  PV of the tile before has completed (its commit is behind S).
+        // that did not use the factor 1.  The PV before must have completed: the one before that has
+        // (its commit lies in front of this S), so its phase is the current one or the one just done.
+        // Phases of pv_done are only ever waited for before this tile's P is handed over (or, after the
+        // last one, by the wait below): the barrier cannot have moved on by two.
+        bool waited = jj == 0;
         const bool need = mt > m_used + kRescale;
         if (__any_sync(0xffffffffu, need)) {
-          if (j > first) {
+          if (jj > 0) {
+            if (!mbar_wait_warp(&pv_done[t], (nv + jj - 1) & 1)) { ok = false; break; }
+            waited = true;
+            tc_fence_after();
             const float f = need ? ex2_approx(m_used - mt) : 1.0f;
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -568,27 +607,29 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         }
         l += ls0 + ls1;
         tmem_wait_st();
+        if (j + step >= (int)in.ntiles && !waited && !mbar_wait_warp(&pv_done[t], (nv + jj - 1) & 1)) { ok = false; break; }
         tc_fence_before();
-        mbar_arrive(&p_full[t]);
+        mbar_arrive(&p_full[2 * t + u]);
       }
       if (!ok) break;
       // ---- the piece's rows ----
-      const bool some = first < (int)in.ntiles;
-      if (some) {
-        ok = mbar_wait_warp(&o_done[t], nd++ & 1);
-        if (!ok) break;
-      }
+      const int mine = NQT == 2 ? (int)in.ntiles : ((int)in.ntiles + 1 - t) >> 1;  // this stream's tiles
+      const bool some = mine > 0;
+      if (some && !mbar_wait_warp(&pv_done[t], (nv + mine - 1) & 1)) { ok = false; break; }
+      nv += mine;
       float f0 = 1.f, f1 = 0.f, M = m_used, L = l;
       if constexpr (NQT == 1) {
         if (t == 1) {
           // stream 0 still reads the last piece's (m, l) until it frees O
+          tc_fence_after();
           if (piece > 0 && !mbar_wait_warp(&o_free[0], (piece - 1) & 1)) { ok = false; break; }
           ml_s[row] = make_float2(m_used, some ? l : 0.f);
+          tc_fence_before();
           mbar_arrive(b_done);
           continue;
         }
         if (!mbar_wait_warp(b_done, piece & 1)) { ok = false; break; }
-        if (in.ntiles > 1 && !mbar_wait_warp(&o_done[1], nd1++ & 1)) { ok = false; break; }
+        // (stream 1 has seen its last PV done before it counted in)
         const float2 ml = ml_s[row];
         M = fmaxf(m_used, ml.x);
         f0 = ex2_approx(m_used - M);
@@ -652,8 +693,8 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     if (!ok) *abort_flag = 1;
   } else {
     // ---------------- dequantising producer (q8 pool) ----------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;" ::: "memory");
     if constexpr (Q8) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 104;" ::: "memory");
       const int gt = tid - 384;
       constexpr int CPR = D / 16;                // 16-code chunks per row
       constexpr int NCH = KT * CPR / 128;        // chunks per thread of one tile
@@ -687,24 +728,22 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       };
       if (have) fetch(0);
       for (int it = 0; have; ++it) {
-        const int s = it & 1;
+        const int s = it % C::NST;
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
-          if (it >= 2) ok = mbar_wait_warp(v ? &v_empty[s] : &k_empty[s], ((it >> 1) - 1) & 1);
+          if (it >= C::NST) ok = mbar_wait_warp(v ? &v_empty[s] : &k_empty[s], ((it / C::NST) - 1) & 1);
           if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
           unsigned char *dst = smem + (v ? C::oV : C::oK) + s * 2 * C::KVT;
 #pragma unroll
           for (int i = 0; i < NCH; ++i) {
             const uint32_t idx = gt + i * 128, r = idx / CPR, c = idx % CPR;
             const uint32_t in[4] = {w[v][i].x, w[v][i].y, w[v][i].z, w[v][i].w};
-            const float s127 = sc[v][i] * (1.0f / 127.0f);
+            const CodeScale cs(sc[v][i]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float x[8];
-#pragma unroll
-              for (int k = 0; k < 8; ++k) x[k] = (float)(int8_t)(in[2 * h + k / 4] >> (8 * (k % 4))) * s127;
               uint4 hi, lo;
-              split8(x, hi, lo);
+              cs.split4(in[2 * h], hi.x, hi.y, lo.x, lo.y);
+              cs.split4(in[2 * h + 1], hi.z, hi.w, lo.z, lo.w);
               unsigned char *d = dst + sw_off<KT>(r, 2 * c + h);
               *reinterpret_cast<uint4 *>(d) = hi;
               *reinterpret_cast<uint4 *>(d + C::KVT) = lo;
@@ -722,6 +761,8 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         if (have) fetch(t);
       }
       if (!ok) *abort_flag = 1;
+    } else if (warp == 12) {
+      mma_loop(std::integral_constant<int, 1>{});
     }
   }
   tc_fence_before();

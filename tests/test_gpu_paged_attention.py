@@ -113,6 +113,24 @@ def test_prefix_many_rows(ops, mode, D, io, B):
     run(ops, Ragged(lens, [1] * B, KV=2, G=4, D=D, mode=mode, prefix=777, page=32, seed=B), DT[io], DT[io])
 
 
+@pytest.mark.parametrize("mode", ["f16", "q8"])
+@pytest.mark.parametrize("io", ["f32", "f16"])
+@pytest.mark.parametrize("B,G", [(24, 4), (40, 4), (67, 4), (30, 3)])
+def test_prefix_many_tiles(ops, mode, io, B, G):
+    """A prefix long enough that every block of the matrix kernels walks a dozen tiles of a unit, with
+    one unit of rows and with several."""
+    lens = [(11 * i) % 70 + 1 for i in range(B)]
+    run(ops, Ragged(lens, [1] * B, KV=8, G=G, mode=mode, prefix=13001, page=64, seed=B), DT[io], DT[io])
+
+
+@pytest.mark.parametrize("mode", ["f16", "q8"])
+@pytest.mark.parametrize("io", ["f32", "f16"])
+@pytest.mark.parametrize("n", [33, 129, 257])
+def test_prefill_many_tiles(ops, mode, io, n):
+    """Prompts behind long contexts: units of many tiles in every block, cut ones among them."""
+    run(ops, Ragged([9000, 7001, 1500], [n, n // 2, 1], KV=8, G=4, mode=mode, page=16, seed=n), DT[io], DT[io])
+
+
 @pytest.mark.parametrize("io", ["f32", "f16"])
 def test_prefix_tokens(ops, io):
     """Several tokens each behind a prefix (verification and prompts), padding behind them."""
