@@ -74,10 +74,13 @@ __device__ __forceinline__ int64_t paged_row(const PagedView &kv, const int32_t 
 // work whatever the lengths, decided on the device from the lengths of this very call.  A unit that a
 // border cuts leaves partial rows: the piece that starts in block c in slot 2c+1, the piece that block
 // c goes on with in slot 2c.  Only a block's first and last piece can be cut, so two slots suffice.
+// A unit also costs its queries, its first scores and its epilogue: `lead` tiles' time, counted as empty
+// tiles in front of its own, so that blocks with many short units get fewer tiles.
 struct UnitShape {
   uint32_t G, KV, RU, KT;
   uint32_t tokens;  // RU / G where that is whole, else 0
   uint32_t shift;   // log2(KT)
+  uint32_t lead;
   uint32_t rows_lo, rows_hi;  // own sequences of rows_lo < n*G <= rows_hi rows (others are another kernel's)
   int prefix;                 // whether the prefix's units are this kernel's
 };
@@ -89,8 +92,9 @@ struct TileSpan {
   uint32_t off0;                // its index among that sequence's tiles
 };
 
-inline UnitShape unit_shape(uint32_t G, uint32_t KV, uint32_t RU, uint32_t KT, uint32_t rows_lo, uint32_t rows_hi, bool prefix) {
-  UnitShape u{G, KV, RU, KT, RU % G ? 0 : RU / G, 0, rows_lo, rows_hi, prefix};
+inline UnitShape unit_shape(uint32_t G, uint32_t KV, uint32_t RU, uint32_t KT, uint32_t lead, uint32_t rows_lo,
+                            uint32_t rows_hi, bool prefix) {
+  UnitShape u{G, KV, RU, KT, RU % G ? 0 : RU / G, 0, lead, rows_lo, rows_hi, prefix};
   while ((1u << u.shift) < KT) ++u.shift;
   return u;
 }
@@ -98,7 +102,7 @@ inline UnitShape unit_shape(uint32_t G, uint32_t KV, uint32_t RU, uint32_t KT, u
 // An upper bound of all tiles of a call, from what the host knows.
 inline uint64_t most_tiles(const UnitShape &u, uint64_t tokens, uint64_t batch, uint64_t capacity, uint64_t prefix) {
   const uint64_t units = tokens * u.G / u.RU + batch + 1;
-  return u.KV * units * ((capacity + u.KT - 1) / u.KT + 1 + (prefix + u.KT - 1) / u.KT);
+  return u.KV * units * ((capacity + u.KT - 1) / u.KT + 1 + u.lead + (prefix + u.KT - 1) / u.KT);
 }
 
 // Positions that the last row of chunk ch attends (own part of a sequence), and the chunk's tiles.
@@ -108,12 +112,12 @@ __device__ __forceinline__ uint32_t chunk_tiles(const SeqRange &s, const UnitSha
   return max(1u, ((uint32_t)m + u.KT - 1) >> u.shift);
 }
 
-// Tiles of one kv head of a sequence's own units (0: none of this kernel's).
+// Tiles of one kv head of a sequence's own units, their leads among them (0: none of this kernel's).
 __device__ __forceinline__ uint32_t seq_tiles(const SeqRange &s, const UnitShape &u) {
   const uint32_t rows = s.n * u.G;
   if (rows <= u.rows_lo || rows > u.rows_hi) return 0;
   uint32_t n = 0;
-  for (uint32_t ch = 0; ch * u.RU < rows; ++ch) n += chunk_tiles(s, u, ch);
+  for (uint32_t ch = 0; ch * u.RU < rows; ++ch) n += u.lead + chunk_tiles(s, u, ch);
   return n;
 }
 
@@ -158,7 +162,7 @@ __device__ __forceinline__ TileSpan block_span(const BatchView &bv, const UnitSh
   s.pre = 0;
   if (u.prefix && bv.prefix_len) {
     const uint32_t nch = (batch_rows(bv, u.G) + u.RU - 1) / u.RU;
-    s.pre = u.KV * nch * ((bv.prefix_len + u.KT - 1) >> u.shift);
+    s.pre = u.KV * nch * (u.lead + ((bv.prefix_len + u.KT - 1) >> u.shift));
   }
   s.total = s.pre + own;
   const uint32_t even = s.total / gridDim.x + (s.total % gridDim.x != 0);
@@ -196,7 +200,7 @@ struct Piece {
 
 struct PieceWalk {
   uint32_t cur, t1, per, pre;  // next tile, end of the span
-  uint32_t b, kvh, ch, in;           // own part: sequence, kv head, chunk, tiles before `cur` in the unit
+  uint32_t b, kvh, ch, in;           // own part: sequence, kv head, chunk, tiles (and lead) before `cur` in the unit
   SeqRange sr;
 
   __device__ __forceinline__ void seek(const BatchView &bv, const UnitShape &u, uint32_t page_size, uint32_t off) {
@@ -207,7 +211,7 @@ struct PieceWalk {
     uint32_t x = off % s;
     ch = 0;
     for (;;) {
-      const uint32_t n = chunk_tiles(sr, u, ch);
+      const uint32_t n = u.lead + chunk_tiles(sr, u, ch);
       if (x < n) break;
       x -= n;
       ++ch;
@@ -227,56 +231,67 @@ struct PieceWalk {
   }
 
   __device__ __forceinline__ bool next(Piece &p, const BatchView &bv, const UnitShape &u, uint32_t page_size) {
-    if (cur >= t1) return false;
-    uint32_t a, n;
-    if (cur < pre) {
-      const uint32_t rows = batch_rows(bv, u.G), nch = (rows + u.RU - 1) / u.RU;
-      n = (bv.prefix_len + u.KT - 1) >> u.shift;
-      const uint32_t unit = cur / n;
-      a = unit * n;
-      p.kvh = unit / nch;
-      p.R0 = unit % nch * u.RU;
-      p.rows = min(u.RU, rows - p.R0);
-      p.tile0 = cur - a;
-      p.len = bv.prefix_len;
-      p.lim_base = 0x40000000;
-      p.pages = bv.prefix_pages;
-      p.own = false;
-      p.ntiles = min(n - p.tile0, t1 - cur);
-    } else {
-      const uint32_t rows = sr.n * u.G;
-      n = chunk_tiles(sr, u, ch);
-      a = cur - in;
-      p.kvh = kvh;
-      p.R0 = sr.begin * u.G + ch * u.RU;
-      p.rows = min(u.RU, rows - ch * u.RU);
-      p.tile0 = in;
-      p.len = (uint32_t)sr.len;
-      p.lim_base = sr.len - (int32_t)sr.n - (int32_t)sr.begin;
-      p.pages = bv.table + (uint64_t)b * bv.table_stride;
-      p.own = true;
-      p.ntiles = min(n - in, t1 - cur);
-      in += p.ntiles;
-      if (in == n) {  // on to the next unit: chunk, kv head, sequence
-        in = 0;
-        if (++ch * u.RU >= rows) {
-          ch = 0;
-          if (++kvh == u.KV) {
-            kvh = 0;
-            if (cur + p.ntiles < t1) {
-              do {
-                ++b;
-                sr = seq_range(bv, b, page_size);
-              } while (seq_tiles(sr, u) == 0);
+    {
+      if (cur >= t1) return false;
+      uint32_t at, n, done;  // where the unit's first tile lies, its tiles, those before this block's
+      if (cur < pre) {
+        const uint32_t rows = batch_rows(bv, u.G), nch = (rows + u.RU - 1) / u.RU;
+        n = (bv.prefix_len + u.KT - 1) >> u.shift;
+        const uint32_t unit = cur / (n + u.lead);
+        at = unit * (n + u.lead) + u.lead;
+        p.kvh = unit / nch;
+        p.R0 = unit % nch * u.RU;
+        p.rows = min(u.RU, rows - p.R0);
+        p.len = bv.prefix_len;
+        p.lim_base = 0x40000000;
+        p.pages = bv.prefix_pages;
+        p.own = false;
+        if (cur < at) cur = min(at, t1);
+        if (cur >= t1) return false;  // only (some of) the lead is this block's
+        done = cur - at;
+        p.ntiles = min(n - done, t1 - cur);
+      } else {
+        const uint32_t rows = sr.n * u.G;
+        n = chunk_tiles(sr, u, ch);
+        if (in < u.lead) {
+          const uint32_t skip = min(u.lead - in, t1 - cur);
+          cur += skip;
+          in += skip;
+          if (cur >= t1) return false;
+        }
+        done = in - u.lead;
+        at = cur - done;
+        p.kvh = kvh;
+        p.R0 = sr.begin * u.G + ch * u.RU;
+        p.rows = min(u.RU, rows - ch * u.RU);
+        p.len = (uint32_t)sr.len;
+        p.lim_base = sr.len - (int32_t)sr.n - (int32_t)sr.begin;
+        p.pages = bv.table + (uint64_t)b * bv.table_stride;
+        p.own = true;
+        p.ntiles = min(n - done, t1 - cur);
+        in += p.ntiles;
+        if (done + p.ntiles == n) {  // on to the next unit: chunk, kv head, sequence
+          in = 0;
+          if (++ch * u.RU >= rows) {
+            ch = 0;
+            if (++kvh == u.KV) {
+              kvh = 0;
+              if (cur + p.ntiles < t1) {
+                do {
+                  ++b;
+                  sr = seq_range(bv, b, page_size);
+                } while (seq_tiles(sr, u) == 0);
+              }
             }
           }
         }
       }
+      p.tile0 = done;
+      p.npieces = (at + n - 1) / per - at / per + 1;
+      p.starts = done == 0;
+      cur += p.ntiles;
+      return true;
     }
-    p.npieces = (a + n - 1) / per - a / per + 1;
-    p.starts = p.tile0 == 0;
-    cur += p.ntiles;
-    return true;
   }
 };
 

@@ -64,7 +64,7 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
   const uint64_t cap = (uint64_t)b->table_stride * kv->page_size;
   p.rows = (uint64_t)b->tokens * H;
   p.join = b->prefix_len > 0;
-  const UnitShape small = unit_shape(G, KV, 8, 64, 0, 0, false);  // the most units and tiles that any kernel may count
+  const UnitShape small = unit_shape(G, KV, 8, 64, 4, 0, 0, false);  // the most units and tiles that any kernel may count
   p.fast = fast && paged_decode_supported((int)kv->mode, D, kv->page_size) && p.rows < 0x10000000ull &&
            most_tiles(small, b->tokens, b->batch, cap, b->prefix_len) < 0xffffffffull;
   if (!p.fast) {

@@ -36,6 +36,7 @@ constexpr int kTile = 64;    // positions per tile
 constexpr int kConsumers = 4;
 constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kUnits = 2;    // staged units
+constexpr int kLead = 0;     // tiles' time that a unit costs beside its tiles
 
 struct DecodeParams {
   PagedAttnArgs a;
@@ -596,7 +597,7 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_hi, bool p
   const uint32_t ps = a.kv.page_size;
   DecodeParams p;
   p.a = a;
-  p.u = unit_shape(a.G, a.kv.KV, 8 * NT, kTile, 0, rows_hi, prefix);
+  p.u = unit_shape(a.G, a.kv.KV, 8 * NT, kTile, kLead, 0, rows_hi, prefix);
   p.box = page_box(ps, kTile);
   p.ppt = kTile / p.box;
   p.join_rows = a.own_pieces != nullptr;

@@ -10,9 +10,10 @@
 //   NQT = 2 (256 rows): stream t is rows [128 t, 128 t + 128) and both use every K/V tile;
 //   NQT = 1 (128 rows): the streams take even and odd K/V tiles of the same rows, and their outputs are
 //           joined at the end (stream 0 reads both from TMEM).
-// Each stream has two score slots of 64 columns, so that the next scores are there when a softmax step ends.
-// The MMA thread issues PV_t and right behind it the S_t that takes over its slot (P overwrote the scores in
-// place): MMAs of one thread execute in order.
+// Softmax works in steps of 64 columns and hands each part of P over at once, so PV of the first part runs
+// under the softmax of the second (f16 pool: tiles of 128 positions, one score tile per stream; q8: tiles of
+// 64, two score tiles).  PV_t and, behind it, the S_t that takes over its columns (P overwrote the scores in
+// place) come from one warp: MMAs of one thread execute in order.
 //
 // Precision, by the types of the call:
 //   f16 rows, f16 pool: operands are exact, P is rounded once to f16 (kept 2^6 up, away from subnormals);
@@ -22,10 +23,9 @@
 //           error of f16 rows; the extra products cost less than that here, because the softmax warps
 //           and not the tensor pipe set the pace of the single-product form.)
 //
-// Warp roles: warp 0 TMA producer of K and V (f16 pool; page boxes, 128-byte swizzle), warp 1 MMA issue of
-// stream 0, warps 2-3 bring the next unit's query rows as soon as the last S of the current one is done,
-// warps 4-11 softmax (one row per thread).  MMA issue of stream 1: warp 12, or with a q8 pool warp 0, where
-// warps 12-15 dequantise, one tile ahead in registers.
+// Warp roles: warp 0 TMA producer of K and V (f16 pool; page boxes, 128-byte swizzle), warp 1 MMA issuer,
+// warps 2-3 bring the next unit's query rows as soon as the last S of the current one is done, warps 4-11
+// softmax (one row per thread), warps 12-15 (q8 pool) dequantise, one tile ahead in registers.
 // All waits are bounded; on expiry the block records BG_ETIMEOUT, stops issuing, waits for what it issued,
 // frees its TMEM and exits.
 #include <cuda.h>
@@ -48,14 +48,16 @@ template <int D, bool Q8, bool LO, int NQT>
 struct TcCfg {
   static constexpr int NQ = LO ? 2 : 1, NK = Q8 ? 2 : 1;     // operand halves
   static constexpr int QT = kM * D * 2;                      // bytes of one f16 query tile
-  static constexpr int KT = 64;
+  static constexpr int KT = Q8 ? 64 : 128;                   // positions of a K/V tile
+  static constexpr int PARTS = KT / 64, SLOTS = 3 - PARTS;   // 64-column parts of a score tile; score tiles per stream
   static constexpr int KVT = KT * D * 2;                     // bytes of one f16 K (or V) tile
-  static constexpr int NST = Q8 ? 2 : 4;                     // ring stages of K and of V
+  static constexpr int LEAD = Q8 ? 2 : 1;                    // a unit's own cost, in tiles
+  static constexpr int NST = 2;                              // ring stages of K and of V
   static constexpr int oQ = 0, oK = NQT * NQ * QT, oV = oK + NST * NK * KVT, oB = oV + NST * NK * KVT;
   static constexpr int oInfo = oB + 384, oML = oInfo + 64, oScan = oML + kM * 8;
   static constexpr int SMEM = oScan + 20 * 8;
-  static constexpr int THREADS = 512;
-  // TMEM columns: score slot u of stream t at (2t + u) * KT, outputs behind them
+  static constexpr int THREADS = Q8 ? 512 : 384;
+  // TMEM columns: part x of stream t at (2t + x) * 64, outputs behind them
   static constexpr uint32_t O0 = 256, O1 = 384;
   static_assert(SMEM <= 232448, "shared memory");
 };
@@ -65,6 +67,7 @@ struct TcParams {
   UnitShape u;
   uint32_t box, ppt;  // positions of a page box, boxes per tile
   uint32_t join_rows;
+  uint32_t page_shift;  // log2(page_size), or 32
   uint32_t q_tma;     // f16 rows whose group divides 128: query tiles come by TMA
   uint32_t wide;      // out and the partial rows start on 32-byte boundaries
 };
@@ -172,20 +175,20 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     for (int i = 0; i < 4; ++i) {
       mbar_init(&k_full[i], Q8 ? 4 : 1);
       mbar_init(&v_full[i], Q8 ? 4 : 1);
-      mbar_init(&k_empty[i], NQT);  // streams that read the tile
-      mbar_init(&v_empty[i], NQT);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[i], 4);  // one arrival per warp: 128 single ones on one word are serialised
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&pv_done[i], 1);
-      mbar_init(&o_free[i], 128);
-      mbar_init(&mma_done[i], 1);
+      mbar_init(&o_free[i], 4);
     }
     mbar_init(q_full, !LO && p.q_tma ? 1 : 64);
-    mbar_init(q_free, 2);
+    mbar_init(q_free, 1);
+    mbar_init(mma_done, 1);
     mbar_init(info_free, 8);
-    mbar_init(b_done, 128);
+    mbar_init(b_done, 4);
     mbar_init(tail, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -207,122 +210,12 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   const uint32_t sQ = smem_u32(smem + C::oQ), sK = smem_u32(smem + C::oK), sV = smem_u32(smem + C::oV);
   const uint32_t ps = a.kv.page_size;
 
-  // ---------------- MMA issue of stream t (one warp per stream) ----------------
-  // The whole warp runs the loop and one elected lane issues: so the compiler knows every operand to be
-  // uniform (run by one lane under a branch, each MMA first moves its descriptors to uniform registers).
-  // One warp per stream: a warp needs ~100 cycles for each barrier that it looks at, done or not, and the
-  // queue of the tensor pipe is too short to bridge that; the other stream's MMAs do.
-  auto mma_loop = [&](auto stream) {
-    constexpr int t = decltype(stream)::value;
-    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
-    constexpr uint32_t idS = idesc_f16(KT, false), idO = idesc_f16(D, true);
-    constexpr uint32_t kHi = umma_desc_hi(1024);
-    const uint32_t q_lo = umma_desc_lo(sQ, 16) + (NQT == 2 ? t : 0) * (NQ * C::QT / 16);
-    const uint32_t k_lo = umma_desc_lo(sK, 16), v_lo = umma_desc_lo(sV, KT * 128), o = tmem + (t ? C::O1 : C::O0);
-    // one product over D (K steps of 16 values, 32 bytes of a 128-byte swizzle row)
-    auto one_s = [&](uint32_t slot, uint32_t q, uint32_t k, auto acc) {
-      umma_ss_lo<kHi, decltype(acc)::value>(slot, q, k, idS);
-#pragma unroll
-      for (int kk = 1; kk < D / 16; ++kk)
-        umma_ss_lo<kHi, true>(slot, q + ((kk >> 2) * (kM * 128) + (kk & 3) * 32) / 16,
-                              k + ((kk >> 2) * (KT * 128) + (kk & 3) * 32) / 16, idS);
-    };
-    // S = Q K^T into slot u: small products first, so that they are added up among themselves
-    auto issue_s = [&](int u, int s) {
-      const uint32_t slot = tmem + (2 * t + u) * KT, k = k_lo + s * (NK * C::KVT / 16);
-      if constexpr (LO) one_s(slot, q_lo + C::QT / 16, k, std::false_type{});
-      if constexpr (Q8) one_s(slot, q_lo, k + C::KVT / 16, std::bool_constant<LO>{});
-      one_s(slot, q_lo, k, std::bool_constant<LO || Q8>{});
-    };
-    auto one_pv = [&](uint32_t pa, uint32_t v, bool acc) {
-      if (acc) umma_ts_lo<kHi, true>(o, pa, v, idO);
-      else umma_ts_lo<kHi, false>(o, pa, v, idO);
-#pragma unroll
-      for (int kk = 1; kk < KT / 16; ++kk) umma_ts_lo<kHi, true>(o, pa + kk * 8, v + kk * (16 * 128 / 16), idO);
-    };
-    // O_t += P V (P from the slot's columns)
-    auto issue_pv = [&](int u, int s, bool acc) {
-      const uint32_t slot = tmem + (2 * t + u) * KT, v = v_lo + s * (NK * C::KVT / 16);
-      if constexpr (LO) one_pv(slot + KT / 2, v, acc);
-      if constexpr (Q8) one_pv(slot, v + C::KVT / 16, LO || acc);
-      one_pv(slot, v, LO || Q8 || acc);
-    };
-    constexpr int STEP = 3 - NQT, FIRST = NQT == 2 ? 0 : t;  // this stream's tiles: FIRST, FIRST + STEP, ...
-    bool ok = true;
-    int it = 0;         // tiles of all pieces before this one
-    uint32_t pp = 0;    // next phase parity of p_full, one bit per slot
-    for (uint32_t piece = 0; ok; ++piece) {
-      if (!mbar_wait_warp(q_full, piece & 1)) { ok = false; break; }
-      const int n = (int)__shfl_sync(0xffffffffu, info->ntiles, 0);
-      if (n == 0) break;
-      tc_fence_after();
-      auto stage = [&](int i) { return (it + i) % C::NST; };
-      auto wait_k = [&](int i) { return mbar_wait_warp(&k_full[stage(i)], ((it + i) / C::NST) & 1); };
-      auto wait_v = [&](int i) { return mbar_wait_warp(&v_full[stage(i)], ((it + i) / C::NST) & 1); };
-      auto after_s = [&](int i, int u) {
-        umma_commit(&s_full[2 * t + u]);
-        umma_commit(&k_empty[stage(i)]);
-        if (i + STEP >= n) umma_commit(q_free);  // this stream's last S of the piece
-      };
-      if (FIRST >= n && elect_one()) umma_commit(q_free);  // no tile for this stream
-      __syncwarp();
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const int i = FIRST + a * STEP;
-        if (!ok || i >= n) break;
-        ok = wait_k(i);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          issue_s(a, stage(i));
-          after_s(i, a);
-        }
-        __syncwarp();
-      }
-      // PV(i), and behind it the S that takes over its slot: in-order execution keeps P safe
-      for (int i = FIRST, u = 0; ok && i < n; i += STEP, u ^= 1) {
-        const bool more = i + 2 * STEP < n;
-        ok = wait_v(i);
-        if (ok && i == FIRST && piece > 0) ok = mbar_wait_warp(&o_free[NQT == 2 ? t : 0], (piece - 1) & 1);
-        ok = ok && mbar_wait_warp(&p_full[2 * t + u], (pp >> u) & 1);
-        if (!ok) break;
-        pp ^= 1u << u;
-        tc_fence_after();
-        if (elect_one()) {
-          issue_pv(u, stage(i), i > FIRST);
-          umma_commit(&pv_done[t]);
-          umma_commit(&v_empty[stage(i)]);
-        }
-        __syncwarp();
-        if (more) {
-          // (only now: the ring may not hold this K before V(i) has been used)
-          ok = wait_k(i + 2 * STEP);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            issue_s(u, stage(i + 2 * STEP));
-            after_s(i + 2 * STEP, u);
-          }
-          __syncwarp();
-        }
-      }
-      it += n;
-    }
-    if (!ok) *abort_flag = 1;
-    // every MMA must complete before the block frees its TMEM
-    if (elect_one()) umma_commit(&mma_done[t]);
-    __syncwarp();
-    mbar_wait_warp(&mma_done[t], 0);
-  };
-
-  // registers: 128*72 + 256*168 + 128*104 = 512*128
+  // registers: 384 threads: 128*72 + 256*216 = 384*168; 512: 128*72 + 256*168 + 128*104 = 512*128
   if (warp < 4) {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
   if (warp == 0) {
     // ---------------- TMA producer (f16 pool) ----------------
-    if constexpr (Q8) {
-      mma_loop(std::integral_constant<int, 1>{});
-    } else {
+    if constexpr (!Q8) {
       PieceWalk walk;
       walk.init(span, a.bv, p.u, ps);
       Piece pc;
@@ -388,7 +281,126 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       }
     }
   } else if (warp == 1) {
-    mma_loop(std::integral_constant<int, 0>{});
+    // ---------------- MMA issuer ----------------
+    // The whole warp runs the loop and one elected lane issues: so the compiler knows every operand to be
+    // uniform (run by one lane under a branch, each MMA first moves its descriptors to uniform registers:
+    // 2900 -> 1720 cycles for a tile's 24 MMAs and their barriers).  One warp for both streams on purpose:
+    // it serves them in turn, which keeps them half a step apart, one on the tensor pipe under the other's
+    // softmax.  (With a warp each they fall into step, wait for the pipe together and then for the exp unit.)
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+    constexpr uint32_t idS = idesc_f16(KT, false), idO = idesc_f16(D, true);
+    constexpr uint32_t kHi = umma_desc_hi(1024);
+    const uint32_t q_lo = umma_desc_lo(sQ, 16), k_lo = umma_desc_lo(sK, 16), v_lo = umma_desc_lo(sV, KT * 128);
+    // one product over D (K steps of 16 values, 32 bytes of a 128-byte swizzle row)
+    auto one_s = [&](uint32_t slot, uint32_t q, uint32_t k, auto acc) {
+      umma_ss_lo<kHi, decltype(acc)::value>(slot, q, k, idS);
+#pragma unroll
+      for (int kk = 1; kk < D / 16; ++kk)
+        umma_ss_lo<kHi, true>(slot, q + ((kk >> 2) * (kM * 128) + (kk & 3) * 32) / 16,
+                              k + ((kk >> 2) * (KT * 128) + (kk & 3) * 32) / 16, idS);
+    };
+    // S = Q K^T into score tile u: small products first, so that they are added up among themselves
+    auto issue_s = [&](int t, int u, int s) {
+      const uint32_t slot = tmem + (2 * t + u) * 64, k = k_lo + s * (NK * C::KVT / 16);
+      const uint32_t q = q_lo + (NQT == 2 ? t : 0) * (NQ * C::QT / 16);
+      if constexpr (LO) one_s(slot, q + C::QT / 16, k, std::false_type{});
+      if constexpr (Q8) one_s(slot, q, k + C::KVT / 16, std::bool_constant<LO>{});
+      one_s(slot, q, k, std::bool_constant<LO || Q8>{});
+    };
+    auto one_pv = [&](uint32_t o, uint32_t pa, uint32_t v, bool acc) {
+      if (acc) umma_ts_lo<kHi, true>(o, pa, v, idO);
+      else umma_ts_lo<kHi, false>(o, pa, v, idO);
+#pragma unroll
+      for (int kk = 1; kk < 4; ++kk) umma_ts_lo<kHi, true>(o, pa + kk * 8, v + kk * (16 * 128 / 16), idO);
+    };
+    // O_t += P V for 64 positions, part h of a tile (P from the columns of part x)
+    auto issue_pv = [&](int t, int x, int s, int h, bool acc) {
+      const uint32_t slot = tmem + (2 * t + x) * 64, v = v_lo + s * (NK * C::KVT / 16) + h * (64 * 128 / 16);
+      const uint32_t o = tmem + (t ? C::O1 : C::O0);
+      if constexpr (LO) one_pv(o, slot + 32, v, acc);
+      if constexpr (Q8) one_pv(o, slot, v + C::KVT / 16, LO || acc);
+      one_pv(o, slot, v, LO || Q8 || acc);
+    };
+    // a stream's tiles are STEP apart; AHEAD tiles' S come before the first PV, as far as the ring holds their K
+    constexpr int STEP = 3 - NQT, AHEAD = C::SLOTS * STEP < C::NST ? C::SLOTS * STEP : C::NST;
+    static_assert(AHEAD % STEP == 0, "the next S belongs to the same stream");
+    bool ok = true;
+    int it = 0;         // tiles of all pieces before this one
+    uint32_t pp = 0;    // next phase parity of p_full, one bit per part
+    for (uint32_t piece = 0; ok; ++piece) {
+      if (!mbar_wait_warp(q_full, piece & 1)) { ok = false; break; }
+      const int n = (int)__shfl_sync(0xffffffffu, info->ntiles, 0);
+      if (n == 0) break;
+      auto stage = [&](int i) { return (it + i) % C::NST; };
+      auto wait_k = [&](int i) { return mbar_wait_warp(&k_full[stage(i)], ((it + i) / C::NST) & 1); };
+      auto wait_v = [&](int i) { return mbar_wait_warp(&v_full[stage(i)], ((it + i) / C::NST) & 1); };
+      // S of stream t, tile i; the last reader of K_i frees it, the last S of the piece frees Q
+      auto send_s = [&](int t, int u, int i) {
+        tc_fence_after();
+        if (elect_one()) {
+          issue_s(t, u, stage(i));
+          umma_commit(&s_full[2 * t + u]);
+          if (NQT == 1 || t == 1) {
+            umma_commit(&k_empty[stage(i)]);
+            if (i + 1 == n) umma_commit(q_free);
+          }
+        }
+        __syncwarp();
+      };
+      for (int i = 0; ok && i < AHEAD && i < n; ++i) {
+        ok = wait_k(i);
+        if (!ok) break;
+        const int u = (i / STEP) % C::SLOTS;
+        if (NQT == 2) {
+          send_s(0, u, i);
+          send_s(1, u, i);
+        } else {
+          send_s(i & 1, u, i);
+        }
+      }
+      // the PVs of stream t, tile i, and behind them the S that takes over its columns: in-order execution
+      // keeps P safe
+      auto step = [&](int t, int i, int u) {
+        if (NQT == 1 || t == 0) ok = wait_v(i);
+        if (ok && i < STEP && piece > 0) ok = mbar_wait_warp(&o_free[NQT == 2 ? t : 0], (piece - 1) & 1);
+#pragma unroll
+        for (int h = 0; h < C::PARTS; ++h) {
+          const int x = C::PARTS == 2 ? h : u, b = 2 * t + x;
+          ok = ok && mbar_wait_warp(&p_full[b], (pp >> b) & 1);
+          if (!ok) return;
+          pp ^= 1u << b;
+          tc_fence_after();
+          if (elect_one()) {
+            issue_pv(t, x, stage(i), h, i >= STEP || h > 0);
+            umma_commit(&pv_done[t]);
+            if (h == C::PARTS - 1 && (NQT == 1 || t == 1)) umma_commit(&v_empty[stage(i)]);
+          }
+          __syncwarp();
+        }
+        if (i + AHEAD < n) {
+          // (only now: the ring may not hold this K before V(i) has been used)
+          if (NQT == 1 || t == 0) ok = wait_k(i + AHEAD);
+          if (ok) send_s(t, ((i + AHEAD) / STEP) % C::SLOTS, i + AHEAD);
+        }
+      };
+      for (int i = 0; ok && i < n; ++i) {
+        const int u = (i / STEP) % C::SLOTS;
+        if (NQT == 2) {
+          step(0, i, u);
+          if (ok) step(1, i, u);
+        } else if (i & 1) {
+          step(1, i, u);
+        } else {
+          step(0, i, u);
+        }
+      }
+      it += n;
+    }
+    if (!ok) *abort_flag = 1;
+    // every MMA must complete before the block frees its TMEM
+    if (elect_one()) umma_commit(mma_done);
+    __syncwarp();
+    mbar_wait_warp(mma_done, 0);
   } else {
     // ---------------- query rows and descriptions ----------------
     const int gt = (warp - 2) * 32 + lane;
@@ -507,7 +519,8 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   }
   } else if (warp < 12) {
     // ---------------- softmax (one row per thread) ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;" ::: "memory");
+    if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;" ::: "memory");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
     const int t = (warp - 4) >> 2;                // stream
     const int row = ((warp & 3) << 5) + lane;     // TMEM lane
     const uint32_t lane_off = (uint32_t)((warp & 3) << 5) << 16;
@@ -529,20 +542,26 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       const int step = NQT == 2 ? 1 : 2;
       const int first = NQT == 2 ? 0 : t;
       for (int j = first; j < (int)in.ntiles; j += step) {
-        const int u = (NQT == 2 ? j : j >> 1) & 1, jj = NQT == 2 ? j : j >> 1;
-        if (!mbar_wait_warp(&s_full[2 * t + u], (sp >> u) & 1)) { ok = false; break; }
-        sp ^= 1u << u;
-        tc_fence_after();
-        const uint32_t sbase = (tmem + (2 * t + u) * KT) | lane_off;
-        const int key0 = (int)(in.tile0 + j) * KT;
-        const int nvalid = min(KT, max(0, lim - key0 + 1));
-        uint32_t x[KT / 32][32];  // the whole score row: one TMEM wait per tile
+       const int jj = NQT == 2 ? j : j >> 1;  // tile of this stream
+#pragma unroll 1
+       for (int h = 0; h < C::PARTS; ++h) {
+        const int g = jj * C::PARTS + h, part = g & 1;  // 64-column step of this stream, and where it lies
+        if (h == 0) {
+          const int u = C::PARTS == 2 ? 0 : part;
+          if (!mbar_wait_warp(&s_full[2 * t + u], (sp >> u) & 1)) { ok = false; break; }
+          sp ^= 1u << u;
+          tc_fence_after();
+        }
+        const uint32_t sbase = (tmem + (2 * t + part) * 64) | lane_off;
+        const int key0 = (int)(in.tile0 + j) * KT + h * 64;
+        const int nvalid = min(64, max(0, lim - key0 + 1));
+        uint32_t x[2][32];  // the step's scores of the row: one TMEM wait
 #pragma unroll
-        for (int c = 0; c < KT / 32; ++c) tmem_ld32(sbase + c * 32, x[c]);
+        for (int c = 0; c < 2; ++c) tmem_ld32(sbase + c * 32, x[c]);
         tmem_wait_ld();
-        if (nvalid < KT) {
+        if (nvalid < 64) {
 #pragma unroll
-          for (int c = 0; c < KT / 32; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (c * 32 + i >= nvalid) x[c][i] = __float_as_uint(-INFINITY);
@@ -551,7 +570,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
 #pragma unroll
         for (int k = 0; k < 8; ++k) mx8[k] = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < KT / 32; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             const int k = (c * 16 + i / 2) & 7;
@@ -560,15 +579,14 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], fmaxf(mx8[5], fmaxf(mx8[6], mx8[7]))));
         const float mt = mx * sl2;
         // lazy rescale: the whole warp takes the TMEM round trip when any of its rows moved far; rows
-        // that did not use the factor 1.  The PV before must have completed: the one before that has
-        // (its commit lies in front of this S), so its phase is the current one or the one just done.
+        // that did not use the factor 1.  The PV before must have completed.
         // Phases of pv_done are only ever waited for before this tile's P is handed over (or, after the
         // last one, by the wait below): the barrier cannot have moved on by two.
-        bool waited = jj == 0;
+        bool waited = g == 0;
         const bool need = mt > m_used + kRescale;
         if (__any_sync(0xffffffffu, need)) {
-          if (jj > 0) {
-            if (!mbar_wait_warp(&pv_done[t], (nv + jj - 1) & 1)) { ok = false; break; }
+          if (g > 0) {
+            if (!mbar_wait_warp(&pv_done[t], (nv + g - 1) & 1)) { ok = false; break; }
             waited = true;
             tc_fence_after();
             const float f = need ? ex2_approx(m_used - mt) : 1.0f;
@@ -586,16 +604,17 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
           if (need) m_used = mt;
         }
         const float mneg = kUp - m_used;
-        float ls0 = 0.f, ls1 = 0.f;
+        const uint64_t sl2x2 = pack2(sl2, sl2), mneg2 = pack2(mneg, mneg);
+        uint64_t sums[2] = {0, 0};
 #pragma unroll
-        for (int c = 0; c < KT / 32; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float p0 = ex2_approx(fmaf(__uint_as_float(x[c][2 * i]), sl2, mneg));
-            const float p1 = ex2_approx(fmaf(__uint_as_float(x[c][2 * i + 1]), sl2, mneg));
-            ls0 += p0;
-            ls1 += p1;
+            const float2 e = unpack2(fma2(pack2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), sl2x2, mneg2));
+            const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
+            const uint64_t pp = pack2(p0, p1);
+            sums[i & 1] = add2(sums[i & 1], pp);
             hi[i] = pack_half2(p0, p1);
             if constexpr (LO) {
               const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
@@ -603,20 +622,24 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
             }
           }
           tmem_st16(sbase + c * 16, hi);
-          if constexpr (LO) tmem_st16(sbase + KT / 2 + c * 16, lo);
+          if constexpr (LO) tmem_st16(sbase + 32 + c * 16, lo);
         }
-        l += ls0 + ls1;
+        const float2 sum = unpack2(add2(sums[0], sums[1]));
+        l += sum.x + sum.y;
         tmem_wait_st();
-        if (j + step >= (int)in.ntiles && !waited && !mbar_wait_warp(&pv_done[t], (nv + jj - 1) & 1)) { ok = false; break; }
+        if (j + step >= (int)in.ntiles && h == C::PARTS - 1 && !waited && !mbar_wait_warp(&pv_done[t], (nv + g - 1) & 1)) { ok = false; break; }
         tc_fence_before();
-        mbar_arrive(&p_full[2 * t + u]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * t + part]);
+       }
+       if (!ok) break;
       }
       if (!ok) break;
       // ---- the piece's rows ----
       const int mine = NQT == 2 ? (int)in.ntiles : ((int)in.ntiles + 1 - t) >> 1;  // this stream's tiles
       const bool some = mine > 0;
-      if (some && !mbar_wait_warp(&pv_done[t], (nv + mine - 1) & 1)) { ok = false; break; }
-      nv += mine;
+      if (some && !mbar_wait_warp(&pv_done[t], (nv + mine * C::PARTS - 1) & 1)) { ok = false; break; }
+      nv += mine * C::PARTS;
       float f0 = 1.f, f1 = 0.f, M = m_used, L = l;
       if constexpr (NQT == 1) {
         if (t == 1) {
@@ -625,7 +648,8 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
           if (piece > 0 && !mbar_wait_warp(&o_free[0], (piece - 1) & 1)) { ok = false; break; }
           ml_s[row] = make_float2(m_used, some ? l : 0.f);
           tc_fence_before();
-          mbar_arrive(b_done);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(b_done);
           continue;
         }
         if (!mbar_wait_warp(b_done, piece & 1)) { ok = false; break; }
@@ -688,7 +712,8 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       }
       if (valid && in.dest != kDirect) a.part_ml[prow] = make_float2(M - kUp, L);
       tc_fence_before();
-      mbar_arrive(&o_free[NQT == 2 ? t : 0]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_free[NQT == 2 ? t : 0]);
     }
     if (!ok) *abort_flag = 1;
   } else {
@@ -701,68 +726,99 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       PieceWalk walk;
       walk.init(span, a.bv, p.u, ps);
       Piece pc;
-      uint32_t t = 0;
-      bool have = walk.next(pc, a.bv, p.u, ps), ok = true;
+      constexpr uint32_t kNone = 0xffffffffu;
       uint4 w[2][NCH];
       float sc[2][NCH];
-      auto fetch = [&](uint32_t tile) {  // codes and block scales of K and V; zeros behind the length
+      uint32_t ahead[NCH];  // pool rows of this thread's chunks, of the tile that K is fetched for (32 bits hold any pool's)
+      uint32_t t = 0;
+      bool have = walk.next(pc, a.bv, p.u, ps), ok = true;
+      auto locate = [&]() {  // the walk's current tile (kNone: behind the length), and on to the next
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-          const uint32_t idx = gt + i * 128, r = idx / CPR, c = idx % CPR, pos = (pc.tile0 + tile) * KT + r;
-          int64_t row = -1;
+          const uint32_t pos = (pc.tile0 + t) * KT + (gt + i * 128) / CPR;
+          ahead[i] = kNone;
           if (pos < pc.len) {
-            row = paged_row(a.kv, pc.pages, pos);
-            if (row < 0) atomicExch(&g_device_error, BG_EINVAL);
-          }
-#pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            w[v][i] = make_uint4(0, 0, 0, 0);
-            sc[v][i] = 0.f;
-            if (row >= 0) {
-              const uint64_t at = (uint64_t)row * a.kv.KV + pc.kvh;
-              w[v][i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(v ? a.kv.V : a.kv.K) + at * D + c * 16));
-              sc[v][i] = __ldg((v ? a.kv.Vs : a.kv.Ks) + at * (D / 32) + c / 2);
-            }
+            const uint32_t pg = (uint32_t)__ldg(pc.pages + (p.page_shift < 32 ? pos >> p.page_shift : pos / ps));
+            const uint32_t at = p.page_shift < 32 ? pos & (ps - 1) : pos % ps;
+            if (pg < a.kv.num_pages) ahead[i] = (pg * ps + at) * a.kv.KV + pc.kvh;
+            else atomicExch(&g_device_error, BG_EINVAL);
           }
         }
-      };
-      if (have) fetch(0);
-      for (int it = 0; have; ++it) {
-        const int s = it % C::NST;
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-          if (it >= C::NST) ok = mbar_wait_warp(v ? &v_empty[s] : &k_empty[s], ((it / C::NST) - 1) & 1);
-          if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
-          unsigned char *dst = smem + (v ? C::oV : C::oK) + s * 2 * C::KVT;
-#pragma unroll
-          for (int i = 0; i < NCH; ++i) {
-            const uint32_t idx = gt + i * 128, r = idx / CPR, c = idx % CPR;
-            const uint32_t in[4] = {w[v][i].x, w[v][i].y, w[v][i].z, w[v][i].w};
-            const CodeScale cs(sc[v][i]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint4 hi, lo;
-              cs.split4(in[2 * h], hi.x, hi.y, lo.x, lo.y);
-              cs.split4(in[2 * h + 1], hi.z, hi.w, lo.z, lo.w);
-              unsigned char *d = dst + sw_off<KT>(r, 2 * c + h);
-              *reinterpret_cast<uint4 *>(d) = hi;
-              *reinterpret_cast<uint4 *>(d + C::KVT) = lo;
-            }
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(v ? &v_full[s] : &k_full[s]);
-        }
-        if (!ok) break;
         if (++t == pc.ntiles) {
           t = 0;
           have = walk.next(pc, a.bv, p.u, ps);
         }
-        if (have) fetch(t);
+      };
+      auto fetch = [&](int v, const uint32_t (&rows)[NCH]) {  // codes and block scales of K (0) or V (1)
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          const uint32_t c = (gt + i * 128) % CPR;
+          w[v][i] = make_uint4(0, 0, 0, 0);
+          sc[v][i] = 0.f;
+          if (rows[i] != kNone) {
+            w[v][i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(v ? a.kv.V : a.kv.K) +
+                                                            (uint64_t)rows[i] * D + c * 16));
+            sc[v][i] = __ldg((v ? a.kv.Vs : a.kv.Ks) + (uint64_t)rows[i] * (D / 32) + c / 2);
+          }
+        }
+      };
+      auto convert = [&](int v, int it) {
+        const int s = it % C::NST;
+        if (it >= C::NST) ok = mbar_wait_warp(v ? &v_empty[s] : &k_empty[s], ((it / C::NST) - 1) & 1);
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) ok = false;
+        if (!ok) return;
+        unsigned char *dst = smem + (v ? C::oV : C::oK) + s * 2 * C::KVT;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          const uint32_t idx = gt + i * 128, r = idx / CPR, c = idx % CPR;
+          const uint32_t in[4] = {w[v][i].x, w[v][i].y, w[v][i].z, w[v][i].w};
+          const CodeScale cs(sc[v][i]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint4 hi, lo;
+            cs.split4(in[2 * h], hi.x, hi.y, lo.x, lo.y);
+            cs.split4(in[2 * h + 1], hi.z, hi.w, lo.z, lo.w);
+            unsigned char *d = dst + sw_off<KT>(r, 2 * c + h);
+            *reinterpret_cast<uint4 *>(d) = hi;
+            *reinterpret_cast<uint4 *>(d + C::KVT) = lo;
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v ? &v_full[s] : &k_full[s]);
+      };
+      // K runs one tile ahead of V (K0 K1 V0 K2 V1 ...: S of a tile comes a softmax before its PV), and each
+      // is fetched for its next tile as soon as its registers are free, to travel while the other is converted.
+      if (have) {
+        locate();
+        fetch(0, ahead);
+        fetch(1, ahead);
+        convert(0, 0);
+        bool k_more = have;  // K of tile it + 1 has been (or is to be) fetched
+        if (k_more) {
+          locate();
+          fetch(0, ahead);
+        }
+        for (int it = 0; ok; ++it) {
+          const bool v_more = k_more;
+          uint32_t v_row[NCH];
+#pragma unroll
+          for (int i = 0; i < NCH; ++i) v_row[i] = ahead[i];  // of tile it + 1
+          if (k_more) {
+            convert(0, it + 1);
+            if (!ok) break;
+            k_more = have;
+            if (k_more) {
+              locate();
+              fetch(0, ahead);
+            }
+          }
+          convert(1, it);
+          if (!ok || !v_more) break;
+          fetch(1, v_row);
+        }
       }
       if (!ok) *abort_flag = 1;
-    } else if (warp == 12) {
-      mma_loop(std::integral_constant<int, 1>{});
     }
   }
   tc_fence_before();
@@ -778,9 +834,12 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_lo, bool p
   TcParams p;
   p.a = a;
   // a launch has either the prefix's units or the sequences' own
-  p.u = unit_shape(a.G, a.kv.KV, NQT * kM, C::KT, prefix ? 0xffffffffu : rows_lo, 0xffffffffu, prefix);
+  p.u = unit_shape(a.G, a.kv.KV, NQT * kM, C::KT, C::LEAD, prefix ? 0xffffffffu : rows_lo, 0xffffffffu, prefix);
   p.box = page_box(ps, C::KT);
   p.ppt = C::KT / p.box;
+  p.page_shift = 32;
+  for (uint32_t i = 0; i < 31; ++i)
+    if (1u << i == ps) p.page_shift = i;
   p.join_rows = a.own_pieces != nullptr;
   CUtensorMap tk = {}, tv = {}, tq = {};
   p.q_tma = !LO && kM % a.G == 0;
