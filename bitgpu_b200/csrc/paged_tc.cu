@@ -765,20 +765,21 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       auto convert = [&](int v, int it) {
         const int s = it % C::NST;
         if (it >= C::NST) ok = mbar_wait_warp(v ? &v_empty[s] : &k_empty[s], ((it / C::NST) - 1) & 1);
-        if (__any_sync(0xffffffffu, *abort_flag != 0)) ok = false;
         if (!ok) return;
         unsigned char *dst = smem + (v ? C::oV : C::oK) + s * 2 * C::KVT;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
           const uint32_t idx = gt + i * 128, r = idx / CPR, c = idx % CPR;
-          const uint32_t in[4] = {w[v][i].x, w[v][i].y, w[v][i].z, w[v][i].w};
           const CodeScale cs(sc[v][i]);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            // the lanes of a row's second half take their two chunks in the other order: a quarter warp's
+            // stores then fall on all banks
+            const uint32_t hh = h ^ (c >> 2);
             uint4 hi, lo;
-            cs.split4(in[2 * h], hi.x, hi.y, lo.x, lo.y);
-            cs.split4(in[2 * h + 1], hi.z, hi.w, lo.z, lo.w);
-            unsigned char *d = dst + sw_off<KT>(r, 2 * c + h);
+            cs.split4(hh ? w[v][i].z : w[v][i].x, hi.x, hi.y, lo.x, lo.y);
+            cs.split4(hh ? w[v][i].w : w[v][i].y, hi.z, hi.w, lo.z, lo.w);
+            unsigned char *d = dst + sw_off<KT>(r, 2 * c + hh);
             *reinterpret_cast<uint4 *>(d) = hi;
             *reinterpret_cast<uint4 *>(d + C::KVT) = lo;
           }
