@@ -78,8 +78,9 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
   p.tc_own = tc && group > 16;
   p.tc_pre = tc && p.join && all > 32;
   p.decode = !p.tc_own || (p.join && !p.tc_pre) || b->tokens < (uint64_t)b->batch * b->max_q;
-  // rows of a unit: 8 where a sequence's rows (or, behind a prefix, all rows) fill no more
-  p.ru = !p.tc_own && group <= 8 && !(p.join && !p.tc_pre && all > 8) ? 8 : 16;
+  // rows of a unit: as many as a sequence's rows (or, behind a prefix, all rows) fill; f32 rows have a form for 4
+  const uint64_t fill = p.tc_own ? 16 : p.join && !p.tc_pre ? (all > group ? all : group) : group;
+  p.ru = fill <= 4 && lo ? 4 : fill <= 8 ? 8 : 16;
   p.blocks = paged_decode_blocks((int)kv->mode, D, p.ru);
   p.ru_own = paged_tc_rows(lo, group);
   p.ru_pre = paged_tc_rows(lo, all);

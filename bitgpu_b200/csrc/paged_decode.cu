@@ -14,8 +14,9 @@
 //   * four consumer warps take 16 positions of a tile each.  Scores are computed transposed (m16n8k16
 //     with positions on M, up to 8 query rows on N), and so is the output, O^T = V^T P^T; P reaches the
 //     B operand in registers through movmatrix;
-//   * f32 rows (LO): q and p are split into two f16 operands (22 bits) and both products run twice;
-//     f16 rows: q is exact and p is rounded once to f16, which costs about as much as the rounding of
+//   * f32 rows (LO): q and p are split into two f16 operands (22 bits).  Up to four rows a unit (PK; one
+//     token of a group of four heads) the halves share one product, hi in columns 0-3 and lo in 4-7 of the
+//     MMA's eight; otherwise both products run twice.  f16 rows: q is exact and p is rounded once to f16, which costs about as much as the rounding of
 //     the result.  p carries a factor 2^14 (q8: 2^6, since V's block scale is folded into p), which
 //     cancels in the quotient and keeps small weights out of f16's subnormals;
 //   * q8 codes enter the products as exact f16 integers: byte + 128 under the f16 pattern 0x64xx is
@@ -79,11 +80,13 @@ struct DecCfg {
   static constexpr int SMEM = oB + 384;
 };
 
-template <int MODE, int D, int NT, bool LO>
+template <int MODE, int D, int NT, bool LO, bool PK>
 __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, DecodeParams p) {
   using C = DecCfg<MODE, D, NT>;
   constexpr int NST = C::NST, NB = C::NB, KS = D / 16, NN = C::NN;
+  static_assert(!PK || (LO && NT == 1), "packed halves");
+  constexpr bool TWO = LO && !PK;  // the low halves have products of their own
   constexpr float kShift = MODE == BG_KV_F16 ? 14.f : 6.f;  // log2 of the factor that p carries
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::oB);
@@ -181,6 +184,8 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
       }
       ++un;
       // ---- its tiles ----
+      // A sequence's own K and V are read once and leave L2 first (64 streams of up to 32768: 640 -> 628 us).
+      const uint64_t policy = l2_policy(pc.own);
       for (uint32_t t = 0; t < pc.ntiles; ++t, ++it) {
         const uint32_t pg = pg_next;
         pg_next = page_of(t + 1);
@@ -196,8 +201,9 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           unsigned char *dst = st + lane * p.box * 128;
 #pragma unroll
           for (int cb = 0; cb < C::NCB; ++cb) {
-            tma_load_4d(dst + cb * kTile * 128, &tmK, &full[s], cb * (128 / C::ES), (int)pc.kvh, slot_y, (int)pg);
-            tma_load_4d(dst + C::KVT + cb * kTile * 128, &tmV, &full[s], cb * (128 / C::ES), (int)pc.kvh, slot_y, (int)pg);
+            tma_load_4d_hint(dst + cb * kTile * 128, &tmK, &full[s], cb * (128 / C::ES), (int)pc.kvh, slot_y, (int)pg, policy);
+            tma_load_4d_hint(dst + C::KVT + cb * kTile * 128, &tmV, &full[s], cb * (128 / C::ES), (int)pc.kvh, slot_y, (int)pg,
+                             policy);
           }
         }
         if constexpr (MODE == BG_KV_Q8) {
@@ -262,11 +268,11 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
     if (ui.ntiles == 0) return;
 
     // Q^T operand fragments (B of m16n8k16): column n = lane / 4, k pairs
-    uint32_t qh[NT][KS][2], ql[LO ? NT : 1][LO ? KS : 1][2];
+    uint32_t qh[NT][KS][2], ql[TWO ? NT : 1][TWO ? KS : 1][2];
     int32_t lim[NT][2];  // last attended position of the lane's score columns
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const uint32_t r = nt * 8 + (lane >> 2);
+      const uint32_t r = PK ? (lane >> 2) & 3 : nt * 8 + (lane >> 2);
       const unsigned char *qr = smem + C::oQ + us * C::QSLOT + r * (a.q_f16 ? D * 2 + 16 : C::QROW);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -276,22 +282,24 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           // fragments, dims 4j,4j+1 (half 0) and 4j+2,4j+3 (half 1), j = lane % 4
           const int d = MODE == BG_KV_Q8 ? ks * 16 + 4 * (lane & 3) + 2 * half : ks * 16 + 2 * (lane & 3) + 8 * half;
           if (a.q_f16) {
-            qh[nt][ks][half] = *reinterpret_cast<const uint32_t *>(qr + d * 2);
-            if constexpr (LO) ql[nt][ks][half] = 0;
+            qh[nt][ks][half] = PK && lane >= 16 ? 0u : *reinterpret_cast<const uint32_t *>(qr + d * 2);
+            if constexpr (TWO) ql[nt][ks][half] = 0;
           } else {
             const float2 v = *reinterpret_cast<const float2 *>(qr + d * 4);
             const uint32_t h = pack_f16(v.x, v.y);
             qh[nt][ks][half] = h;
             if constexpr (LO) {
               const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-              ql[nt][ks][half] = pack_f16(v.x - f.x, v.y - f.y);
+              const uint32_t lo = pack_f16(v.x - f.x, v.y - f.y);
+              if constexpr (TWO) ql[nt][ks][half] = lo;
+              else if (lane >= 16) qh[nt][ks][half] = lo;
             }
           }
         }
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint32_t rc = min((uint32_t)(nt * 8 + 2 * (lane & 3) + j), ui.rows - 1);
+        const uint32_t col = nt * 8 + 2 * (lane & 3) + j, rc = min(PK ? col & 3 : col, ui.rows - 1);
         lim[nt][j] = min(ui.lim_base + (int32_t)((ui.R0 + rc) / a.G), (int32_t)ui.len - 1);
       }
     }
@@ -331,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           ldsm_x4(f, swz<kTile>(kb, row0 + lrow, 2 * ks + lhi));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            if constexpr (LO) {
+            if constexpr (TWO) {
               mma16816(acc[nt], f, qh[nt][ks][0], qh[nt][ks][1]);
               mma16816(acl[nt], f, ql[nt][ks][0], ql[nt][ks][1]);
             } else {
@@ -342,7 +350,10 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[nt][i] = (acc[nt][i] + acl[nt][i]) * sl2;
+          for (int i = 0; i < 4; ++i) {
+            sc[nt][i] = (acc[nt][i] + acl[nt][i]) * sl2;
+            if constexpr (PK) sc[nt][i] += __shfl_xor_sync(0xffffffffu, sc[nt][i], 2);
+          }
       } else {
         const float *ksc = reinterpret_cast<const float *>(smem + s * C::STAGE + 2 * C::KVT);
         const __half2 bias = __float2half2_rn(1152.f);
@@ -370,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
             mma16816(acc, a0, qh[nt][2 * bk][0], qh[nt][2 * bk][1]);
             mma16816(acc, a1, qh[nt][2 * bk + 1][0], qh[nt][2 * bk + 1][1]);
-            if constexpr (LO) {
+            if constexpr (TWO) {
               mma16816(acc, a0, ql[nt][2 * bk][0], ql[nt][2 * bk][1]);
               mma16816(acc, a1, ql[nt][2 * bk + 1][0], ql[nt][2 * bk + 1][1]);
             }
@@ -379,6 +390,10 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
             sc[nt][2] = fmaf(acc[2], sb, sc[nt][2]);
             sc[nt][3] = fmaf(acc[3], sb, sc[nt][3]);
           }
+        }
+        if constexpr (PK) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[0][i] += __shfl_xor_sync(0xffffffffu, sc[0][i], 2);
         }
       }
 
@@ -420,12 +435,14 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
 
       // ---- O^T += V^T . P^T ----
       auto split = [&](float x, float y, uint32_t &hi, uint32_t &lo) {
-        const uint32_t h = pack_f16(x, y);
-        hi = movm_t(h);
+        uint32_t h = pack_f16(x, y);
         if constexpr (LO) {
           const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
-          lo = movm_t(pack_f16(x - f.x, y - f.y));
+          const uint32_t l = pack_f16(x - f.x, y - f.y);
+          if constexpr (TWO) lo = movm_t(l);
+          else if (lane & 2) h = l;  // columns 4-7
         }
+        hi = movm_t(h);
       };
       if constexpr (MODE == BG_KV_F16) {
         uint32_t pb0[NT], pb1[NT], pl0[NT], pl1[NT];
@@ -456,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           for (int nt = 0; nt < NT; ++nt) {
             if constexpr (LO) {
               float acc[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816(acc, f, pl0[nt], pl1[nt]);
+              if constexpr (TWO) mma16816(acc, f, pl0[nt], pl1[nt]);
               mma16816(acc, f, pb0[nt], pb1[nt]);
 #pragma unroll
               for (int i = 0; i < 4; ++i) oacc[nt][mt][i] = fmaf(oacc[nt][mt][i], cr[nt][i & 1], acc[i]);
@@ -493,8 +510,10 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           for (int nt = 0; nt < NT; ++nt) {
             if constexpr (LO) {
               float x0[4] = {0.f, 0.f, 0.f, 0.f}, x1[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816(x0, a0, pl0[nt], pl1[nt]);
-              mma16816(x1, a1, pl0[nt], pl1[nt]);
+              if constexpr (TWO) {
+                mma16816(x0, a0, pl0[nt], pl1[nt]);
+                mma16816(x1, a1, pl0[nt], pl1[nt]);
+              }
               mma16816(x0, a0, pb0[nt], pb1[nt]);
               mma16816(x1, a1, pb0[nt], pb1[nt]);
 #pragma unroll
@@ -574,7 +593,15 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
       const uint32_t n = idx / (D / 4), d = idx % (D / 4) * 4;
       const float4 x = *reinterpret_cast<const float4 *>(e0 + n * C::DP + d);
       const float4 y = *reinterpret_cast<const float4 *>(e1 + n * C::DP + d);
-      const float o[4] = {x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w};
+      float o[4] = {x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w};
+      if constexpr (PK) {  // the low halves' columns
+        const float4 z = *reinterpret_cast<const float4 *>(e0 + (n + 4) * C::DP + d);
+        const float4 w = *reinterpret_cast<const float4 *>(e1 + (n + 4) * C::DP + d);
+        o[0] += z.x + w.x;
+        o[1] += z.y + w.y;
+        o[2] += z.z + w.z;
+        o[3] += z.w + w.w;
+      }
       const uint32_t R = ui.R0 + n;
       const uint64_t row = (uint64_t)(R / a.G) * a.H + ui.kvh * a.G + R % a.G;
       if (ui.dest == kDirect) {
@@ -591,13 +618,13 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
   }
 }
 
-template <int MODE, int D, int NT, bool LO>
+template <int MODE, int D, int NT, bool LO, bool PK = false>
 int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_hi, bool prefix, cudaStream_t st) {
   using C = DecCfg<MODE, D, NT>;
   const uint32_t ps = a.kv.page_size;
   DecodeParams p;
   p.a = a;
-  p.u = unit_shape(a.G, a.kv.KV, 8 * NT, kTile, kLead, 0, rows_hi, prefix);
+  p.u = unit_shape(a.G, a.kv.KV, PK ? 4 : 8 * NT, kTile, kLead, 0, rows_hi, prefix);
   p.box = page_box(ps, kTile);
   p.ppt = kTile / p.box;
   p.join_rows = a.own_pieces != nullptr;
@@ -607,9 +634,12 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_hi, bool p
   const uint64_t strides[3] = {rb, rb * a.kv.KV, rb * a.kv.KV * ps};
   const uint32_t box[4] = {128 / C::ES, 1, p.box, 1};
   const CUtensorMapDataType dt = MODE == BG_KV_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  if (make_tmap_4d(&tk, dt, a.kv.K, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return BG_EUNSUPPORTED;
-  if (make_tmap_4d(&tv, dt, a.kv.V, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return BG_EUNSUPPORTED;
-  auto kern = paged_decode_kernel<MODE, D, NT, LO>;
+  // L2 fetches no more than a head's row: promoted to 256 bytes, a 128-byte q8 row brings its neighbour head's,
+  // whose block comes by much later (32 streams: 423 MB read for caches of 321 MB)
+  const auto fetch = rb >= 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B;
+  if (make_tmap_4d(&tk, dt, a.kv.K, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, fetch)) return BG_EUNSUPPORTED;
+  if (make_tmap_4d(&tv, dt, a.kv.V, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, fetch)) return BG_EUNSUPPORTED;
+  auto kern = paged_decode_kernel<MODE, D, NT, LO, PK>;
   static unsigned long long allowed = 0;
   if (!allow_smem(kern, C::SMEM, allowed)) return BG_ELAUNCH;
   cudaLaunchConfig_t cfg = {};
@@ -628,6 +658,7 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_hi, bool p
 template <int MODE, int D>
 int launch_md(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_hi, bool prefix, cudaStream_t st) {
   const bool lo = !(a.q_f16 && a.out_f16);
+  if (ru == 4) return launch_cfg<MODE, D, 1, true, true>(a, blocks, rows_hi, prefix, st);
   if (ru == 8)
     return lo ? launch_cfg<MODE, D, 1, true>(a, blocks, rows_hi, prefix, st)
               : launch_cfg<MODE, D, 1, false>(a, blocks, rows_hi, prefix, st);
@@ -643,7 +674,7 @@ bool paged_decode_supported(int mode, uint32_t D, uint32_t page_size) {
 }
 
 uint32_t paged_decode_blocks(int mode, uint32_t D, uint32_t ru) {
-  return 148 * (D == 256 ? 1 : mode == BG_KV_Q8 && ru == 8 ? 3 : 2);
+  return 148 * (D == 256 ? 1 : mode == BG_KV_Q8 && ru <= 8 ? 3 : 2);
 }
 
 int launch_paged_decode(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_hi, bool prefix,

@@ -73,6 +73,22 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, u
       : "memory");
 }
 
+// The same with an L2 eviction priority (a createpolicy value).
+__device__ __forceinline__ void tma_load_4d_hint(void *dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z,
+                                                 int w, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, "
+      "%5, %6}], [%2], %7;" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ uint64_t l2_policy(bool evict_first) {
+  uint64_t first, normal;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first));
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(normal));
+  return evict_first ? first : normal;
+}
+
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -80,6 +96,7 @@ __device__ __forceinline__ void prefetch_tmap(const CUtensorMap *map) {
 // Host: encode a rank-4 tiled tensor map (driver entry point fetched through the runtime, so the
 // library does not link libcuda).  dims/strides in elements/bytes as cuTensorMapEncodeTiled.
 int make_tmap_4d(CUtensorMap *m, CUtensorMapDataType dt, const void *base, const uint64_t dims[4],
-                 const uint64_t strides_bytes[3], const uint32_t box[4], CUtensorMapSwizzle swz);
+                 const uint64_t strides_bytes[3], const uint32_t box[4], CUtensorMapSwizzle swz,
+                 CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 
 }  // namespace bg

@@ -30,7 +30,8 @@ EncodeTiledFn encode_fn() {
 }  // namespace
 
 int make_tmap_4d(CUtensorMap *m, CUtensorMapDataType dt, const void *base, const uint64_t dims[4],
-                 const uint64_t strides_bytes[3], const uint32_t box[4], CUtensorMapSwizzle swz) {
+                 const uint64_t strides_bytes[3], const uint32_t box[4], CUtensorMapSwizzle swz,
+                 CUtensorMapL2promotion promotion) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return -1;
   cuuint64_t gd[4] = {dims[0], dims[1], dims[2], dims[3]};
@@ -38,7 +39,7 @@ int make_tmap_4d(CUtensorMap *m, CUtensorMapDataType dt, const void *base, const
   cuuint32_t bx[4] = {box[0], box[1], box[2], box[3]};
   cuuint32_t es[4] = {1, 1, 1, 1};
   CUresult r = fn(m, dt, 4, const_cast<void *>(base), gd, gs, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -1;
 }
 
