@@ -98,6 +98,17 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
   return p;
 }
 
+// Enough for either kind of kernel and either type of rows, so that what a caller needs does not change with
+// bg_force_generic or with the types of one call.
+size_t workspace_bytes_for(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, uint32_t KV, uint32_t D) {
+  size_t n = 0;
+  for (int i = 0; i < 3; ++i) {
+    const size_t m = make_plan(kv, b, H, KV, D, i < 2, i == 1).bytes;
+    n = m > n ? m : n;
+  }
+  return n;
+}
+
 }  // namespace
 
 namespace bg {
@@ -153,14 +164,7 @@ int bg_paged_append(const bg_paged_cache *kv, const bg_paged_batch *batch, uint3
 size_t bg_paged_attention_workspace_size(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV,
                                          uint32_t D) {
   if (check_paged(kv, batch, KV, D) || H == 0 || H % KV || batch->batch == 0 || batch->tokens == 0) return 0;
-  // enough for either kind of kernel, so that bg_force_generic does not change what a caller needs
-  // (and for either type of rows)
-  size_t n = 0;
-  for (int i = 0; i < 3; ++i) {
-    const size_t m = make_plan(kv, batch, H, KV, D, i < 2, i == 1).bytes;
-    n = m > n ? m : n;
-  }
-  return n;
+  return workspace_bytes_for(kv, batch, H, KV, D);
 }
 
 int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV, uint32_t D,
@@ -171,7 +175,8 @@ int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, ui
   if (batch->batch == 0 || batch->tokens == 0) return BG_OK;
   if (!q || !out || !aligned16(q) || !aligned16(out) || !aligned16(gate) || !aligned16(workspace)) return BG_EINVAL;
   const Plan plan = make_plan(kv, batch, H, KV, D, !generic_forced(), !(q_dtype == BG_DT_F16 && out_dtype == BG_DT_F16));
-  if (plan.bytes && (!workspace || workspace_bytes < plan.bytes)) return BG_ENOMEM;
+  const size_t need = workspace_bytes_for(kv, batch, H, KV, D);
+  if (need && (!workspace || workspace_bytes < need)) return BG_ENOMEM;
   cudaStream_t st = (cudaStream_t)stream;
   PagedAttnArgs a = {};
   a.kv = view(kv, KV);

@@ -372,7 +372,7 @@ class PagedKVCache:
                     raise ValueError(f"{name} must be [num_pages, page_size, kv_heads, head_dim / 32] beside K")
         self.K, self.V, self.Ks, self.Vs = K, V, Ks, Vs
         self.num_pages, self.page_size, self.KV, self.D = K.shape
-        self.device = K.device
+        self.device, self.index = K.device, K.get_device()
         self._desc = PagedCacheDesc(K.data_ptr(), V.data_ptr(), Ks.data_ptr() if Ks is not None else None,
                                     Vs.data_ptr() if Vs is not None else None, self.num_pages, self.page_size,
                                     MODES[self.mode])
@@ -420,7 +420,7 @@ class PagedBatch:
             raise ValueError("prefix_len needs prefix_pages")
         self.page_table, self.kv_len, self.cu_q, self.prefix_pages = page_table, kv_len, cu_q, prefix_pages
         self.batch, self.tokens, self.max_q, self.prefix_len = B, tokens, max_q, prefix_len
-        self.device = page_table.device
+        self.device, self.index = page_table.device, page_table.get_device()
         self._desc = PagedBatchDesc(_ptr(cu_q), kv_len.data_ptr(), page_table.data_ptr(), _ptr(prefix_pages), B, tokens,
                                     max_q, width, prefix_len)
         self._ref = C.byref(self._desc)
@@ -430,7 +430,7 @@ class PagedBatch:
         return self._desc
 
     def _fits(self, cache):
-        if cache.device != self.device:
+        if cache.index != self.index:
             raise ValueError("the cache and the batch must be on one device")
         if self.prefix_len and self.prefix_pages.numel() * cache.page_size < self.prefix_len:
             raise ValueError("prefix_pages holds fewer than prefix_len positions")
@@ -455,11 +455,12 @@ def _on(device, fn, *args):
         return fn(*args, _raw_stream(index))
 
 
-def _rows(t, name, T, heads, D, dtype, device):
-    if t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be {dtype} on {device}")
-    if t.dim() != 3 or t.shape[0] != T or t.shape[2] != D or (heads and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [tokens, heads, head_dim] = [{T}, {heads or 'H'}, {D}]")
+def _rows(t, name, shape, dtype, index):
+    """Rows of a projection for the C call: any token and head stride, contiguous values."""
+    if t.dtype is not dtype or t.get_device() != index:
+        raise ValueError(f"{name} must be {dtype} on the cache's device")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be [tokens, heads, head_dim] = {list(shape)}, got {list(t.shape)}")
     st, sh, sd = t.stride()
     if sd != 1 or st < 0 or sh < 0:
         raise ValueError(f"the values of a {name} row must be contiguous")
@@ -478,40 +479,46 @@ def paged_append(cache, batch, k, v, cos=None, sin=None, k_gamma=None, eps=1e-6,
     ``[tokens, heads, head_dim]`` (``q_out``, or new in ``q_dtype``; padding rows are not written),
     or None without q."""
     T, KV, D, dev = batch.tokens, cache.KV, cache.D, cache.device
+    index, dtype = cache.index, k.dtype
     batch._fits(cache)
-    if k.dtype not in _DT:
-        raise ValueError(f"k must be float32 or float16, got {k.dtype}")
-    kr, vr = _rows(k, "k", T, KV, D, k.dtype, dev), _rows(v, "v", T, KV, D, k.dtype, dev)
+    if dtype not in _DT:
+        raise ValueError(f"k must be float32 or float16, got {dtype}")
+    kv_shape = (T, KV, D)
+    kr, vr = _rows(k, "k", kv_shape, dtype, index), _rows(v, "v", kv_shape, dtype, index)
     rot = positions = 0
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
     if cos is not None:
         _need(cos, torch.float32, "cos")
         _need(sin, torch.float32, "sin")
-        if cos.dim() != 2 or cos.shape != sin.shape or cos.device != dev or sin.device != dev:
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.get_device() != index or sin.get_device() != index:
             raise ValueError("cos and sin must be [positions, rot] on the cache's device")
         positions, rot = cos.shape
     for g, name in ((k_gamma, "k_gamma"), (q_gamma, "q_gamma")):
         if g is not None:
             _need(g, torch.float32, name)
-            if g.numel() != D or g.device != dev:
+            if g.numel() != D or g.get_device() != index:
                 raise ValueError(f"{name} must be [head_dim] on the cache's device")
     qr, H = None, 0
     if q is not None:
-        qr, H = _rows(q, "q", T, 0, D, k.dtype, dev), q.shape[1]
+        if q.dim() != 3:
+            raise ValueError("q must be [tokens, heads, head_dim]")
+        H = q.shape[1]
+        q_shape = (T, H, D)
+        qr = _rows(q, "q", q_shape, dtype, index)
         if q_out is None:
-            q_out = torch.empty((T, H, D), dtype=q_dtype, device=dev)
+            q_out = torch.empty_like(q, dtype=q_dtype, memory_format=torch.contiguous_format)
         else:
             _need(q_out, name="q_out")
-            if q_out.shape != (T, H, D) or q_out.device != dev:
+            if q_out.shape != q_shape or q_out.get_device() != index:
                 raise ValueError("q_out must be [tokens, heads, head_dim] on the cache's device")
         if q_out.dtype not in _DT:
             raise ValueError(f"q_out must be float32 or float16, got {q_out.dtype}")
     else:
         q_out = None
-    rc = _on(dev, lib().bg_paged_append, cache._ref, batch._ref, H, KV, D, qr, kr, vr, _DT[k.dtype], _ptr(q_gamma),
+    rc = _on(dev, lib().bg_paged_append, cache._ref, batch._ref, H, KV, D, qr, kr, vr, _DT[dtype], _ptr(q_gamma),
              _ptr(k_gamma), eps, _ptr(cos), _ptr(sin), rot, positions, _ptr(q_out),
-             _DT[q_out.dtype] if q is not None else 0)
+             _DT[q_out.dtype] if q_out is not None else 0)
     if rc:
         check("bg_paged_append", rc)
     return q_out
@@ -525,22 +532,22 @@ def paged_attention(q, cache, batch, scale=0.0, gate=None, out_dtype=torch.float
     _need(q, name="q")
     if q.dtype not in _DT:
         raise ValueError(f"q must be float32 or float16, got {q.dtype}")
-    dev = cache.device
-    if q.dim() != 3 or q.shape[0] != batch.tokens or q.shape[2] != cache.D or q.device != dev:
+    dev, index, shape = cache.device, cache.index, q.shape
+    if len(shape) != 3 or shape[0] != batch.tokens or shape[2] != cache.D or q.get_device() != index:
         raise ValueError("q must be [tokens, heads, head_dim] on the cache's device")
     batch._fits(cache)
-    H = q.shape[1]
+    H = shape[1]
     if out is None:
         out = torch.empty_like(q, dtype=out_dtype)
     else:
         _need(out, name="out")
-        if out.shape != q.shape or out.device != dev:
+        if out.shape != shape or out.get_device() != index:
             raise ValueError("out must have the shape and device of q")
     if out.dtype not in _DT:
         raise ValueError(f"out must be float32 or float16, got {out.dtype}")
     if gate is not None:
         _need(gate, torch.float32, "gate")
-        if gate.shape != q.shape or gate.device != dev:
+        if gate.shape != shape or gate.get_device() != index:
             raise ValueError("gate must have the shape and device of q")
     key = (H, cache.KV, cache.D, cache.mode, cache.page_size)
     nbytes = batch._ws.get(key)
