@@ -25,7 +25,7 @@
 //
 // Warp roles: warp 0 TMA producer of K and V (f16 pool; page boxes, 128-byte swizzle), warp 1 MMA issuer,
 // warps 2-3 bring the next unit's query rows as soon as the last S of the current one is done, warps 4-11
-// softmax (one row per thread), warps 12-15 (q8 pool) dequantise, one tile ahead in registers.
+// softmax (one row per thread), warps 12-15 and 16-19 (q8 pool) dequantise K and V, a tile ahead in registers.
 // All waits are bounded; on expiry the block records BG_ETIMEOUT, stops issuing, waits for what it issued,
 // frees its TMEM and exits.
 #include <cuda.h>
@@ -55,8 +55,8 @@ struct TcCfg {
   static constexpr int NST = 2;                              // ring stages of K and of V
   static constexpr int oQ = 0, oK = NQT * NQ * QT, oV = oK + NST * NK * KVT, oB = oV + NST * NK * KVT;
   static constexpr int oInfo = oB + 384, oML = oInfo + 64, oScan = oML + kM * 8;
-  static constexpr int SMEM = oScan + 20 * 8;
-  static constexpr int THREADS = Q8 ? 512 : 384;
+  static constexpr int SMEM = oScan + 24 * 8;
+  static constexpr int THREADS = Q8 ? 640 : 384;
   // TMEM columns: part x of stream t at (2t + x) * 64, outputs behind them
   static constexpr uint32_t O0 = 256, O1 = 384;
   static_assert(SMEM <= 232448, "shared memory");
@@ -210,9 +210,10 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   const uint32_t sQ = smem_u32(smem + C::oQ), sK = smem_u32(smem + C::oK), sV = smem_u32(smem + C::oV);
   const uint32_t ps = a.kv.page_size;
 
-  // registers: 384 threads: 128*72 + 256*216 = 384*168; 512: 128*72 + 256*168 + 128*104 = 512*128
+  // registers: 384 threads: 128*72 + 256*216 = 384*168; 640: 128*64 + 256*128 + 256*80 = 640*96
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
+  if constexpr (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;" ::: "memory");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
   if (warp == 0) {
     // ---------------- TMA producer (f16 pool) ----------------
     if constexpr (!Q8) {
@@ -519,7 +520,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   }
   } else if (warp < 12) {
     // ---------------- softmax (one row per thread) ----------------
-    if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;" ::: "memory");
+    if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;" ::: "memory");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;" ::: "memory");
     const int t = (warp - 4) >> 2;                // stream
     const int row = ((warp & 3) << 5) + lane;     // TMEM lane
@@ -717,31 +718,39 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     }
     if (!ok) *abort_flag = 1;
   } else {
-    // ---------------- dequantising producer (q8 pool) ----------------
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;" ::: "memory");
+    // ---------------- dequantising producers (q8 pool): warps 12-15 for K, 16-19 for V ----------------
     if constexpr (Q8) {
-      const int gt = tid - 384;
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 80;" ::: "memory");
+      const int v = warp >= 16, gt = tid - (v ? 512 : 384);
+      uint64_t *full = v ? v_full : k_full, *empty = v ? v_empty : k_empty;
+      const int8_t *codes = static_cast<const int8_t *>(v ? a.kv.V : a.kv.K);
+      const float *scales = v ? a.kv.Vs : a.kv.Ks;
+      unsigned char *ring = smem + (v ? C::oV : C::oK);
       constexpr int CPR = D / 16;                // 16-code chunks per row
       constexpr int NCH = KT * CPR / 128;        // chunks per thread of one tile
       PieceWalk walk;
       walk.init(span, a.bv, p.u, ps);
       Piece pc;
-      constexpr uint32_t kNone = 0xffffffffu;
-      uint4 w[2][NCH];
-      float sc[2][NCH];
-      uint32_t ahead[NCH];  // pool rows of this thread's chunks, of the tile that K is fetched for (32 bits hold any pool's)
       uint32_t t = 0;
       bool have = walk.next(pc, a.bv, p.u, ps), ok = true;
-      auto locate = [&]() {  // the walk's current tile (kNone: behind the length), and on to the next
+      uint4 w[NCH], wn[NCH];
+      float sc[NCH], sn[NCH];
+      // codes and block scales of the walk's current tile (zeros behind the length), and on to the next
+      auto fetch = [&](uint4 (&x)[NCH], float (&s)[NCH]) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-          const uint32_t pos = (pc.tile0 + t) * KT + (gt + i * 128) / CPR;
-          ahead[i] = kNone;
+          const uint32_t idx = gt + i * 128, c = idx % CPR, pos = (pc.tile0 + t) * KT + idx / CPR;
+          x[i] = make_uint4(0, 0, 0, 0);
+          s[i] = 0.f;
           if (pos < pc.len) {
             const uint32_t pg = (uint32_t)__ldg(pc.pages + (p.page_shift < 32 ? pos >> p.page_shift : pos / ps));
-            const uint32_t at = p.page_shift < 32 ? pos & (ps - 1) : pos % ps;
-            if (pg < a.kv.num_pages) ahead[i] = (pg * ps + at) * a.kv.KV + pc.kvh;
-            else atomicExch(&g_device_error, BG_EINVAL);
+            if (pg < a.kv.num_pages) {
+              const uint64_t row = ((uint64_t)pg * ps + (p.page_shift < 32 ? pos & (ps - 1) : pos % ps)) * a.kv.KV + pc.kvh;
+              x[i] = __ldg(reinterpret_cast<const uint4 *>(codes + row * D + c * 16));
+              s[i] = __ldg(scales + row * (D / 32) + c / 2);
+            } else {
+              atomicExch(&g_device_error, BG_EINVAL);
+            }
           }
         }
         if (++t == pc.ntiles) {
@@ -749,36 +758,27 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
           have = walk.next(pc, a.bv, p.u, ps);
         }
       };
-      auto fetch = [&](int v, const uint32_t (&rows)[NCH]) {  // codes and block scales of K (0) or V (1)
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-          const uint32_t c = (gt + i * 128) % CPR;
-          w[v][i] = make_uint4(0, 0, 0, 0);
-          sc[v][i] = 0.f;
-          if (rows[i] != kNone) {
-            w[v][i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(v ? a.kv.V : a.kv.K) +
-                                                            (uint64_t)rows[i] * D + c * 16));
-            sc[v][i] = __ldg((v ? a.kv.Vs : a.kv.Ks) + (uint64_t)rows[i] * (D / 32) + c / 2);
-          }
-        }
-      };
-      auto convert = [&](int v, int it) {
+      bool more = have;
+      if (more) fetch(w, sc);
+      for (int it = 0; more; ++it) {
+        const bool next = have;
+        if (next) fetch(wn, sn);  // travels while this tile is converted
         const int s = it % C::NST;
-        if (it >= C::NST) ok = mbar_wait_warp(v ? &v_empty[s] : &k_empty[s], ((it / C::NST) - 1) & 1);
-        if (!ok) return;
-        unsigned char *dst = smem + (v ? C::oV : C::oK) + s * 2 * C::KVT;
+        if (it >= C::NST) ok = mbar_wait_warp(&empty[s], ((it / C::NST) - 1) & 1);
+        if (!ok) break;
+        unsigned char *dst = ring + s * 2 * C::KVT;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
           const uint32_t idx = gt + i * 128, r = idx / CPR, c = idx % CPR;
-          const CodeScale cs(sc[v][i]);
+          const CodeScale cs(sc[i]);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             // the lanes of a row's second half take their two chunks in the other order: a quarter warp's
             // stores then fall on all banks
             const uint32_t hh = h ^ (c >> 2);
             uint4 hi, lo;
-            cs.split4(hh ? w[v][i].z : w[v][i].x, hi.x, hi.y, lo.x, lo.y);
-            cs.split4(hh ? w[v][i].w : w[v][i].y, hi.z, hi.w, lo.z, lo.w);
+            cs.split4(hh ? w[i].z : w[i].x, hi.x, hi.y, lo.x, lo.y);
+            cs.split4(hh ? w[i].w : w[i].y, hi.z, hi.w, lo.z, lo.w);
             unsigned char *d = dst + sw_off<KT>(r, 2 * c + hh);
             *reinterpret_cast<uint4 *>(d) = hi;
             *reinterpret_cast<uint4 *>(d + C::KVT) = lo;
@@ -786,37 +786,12 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(v ? &v_full[s] : &k_full[s]);
-      };
-      // K runs one tile ahead of V (K0 K1 V0 K2 V1 ...: S of a tile comes a softmax before its PV), and each
-      // is fetched for its next tile as soon as its registers are free, to travel while the other is converted.
-      if (have) {
-        locate();
-        fetch(0, ahead);
-        fetch(1, ahead);
-        convert(0, 0);
-        bool k_more = have;  // K of tile it + 1 has been (or is to be) fetched
-        if (k_more) {
-          locate();
-          fetch(0, ahead);
-        }
-        for (int it = 0; ok; ++it) {
-          const bool v_more = k_more;
-          uint32_t v_row[NCH];
+        if (lane == 0) mbar_arrive(&full[s]);
+        more = next;
 #pragma unroll
-          for (int i = 0; i < NCH; ++i) v_row[i] = ahead[i];  // of tile it + 1
-          if (k_more) {
-            convert(0, it + 1);
-            if (!ok) break;
-            k_more = have;
-            if (k_more) {
-              locate();
-              fetch(0, ahead);
-            }
-          }
-          convert(1, it);
-          if (!ok || !v_more) break;
-          fetch(1, v_row);
+        for (int i = 0; i < NCH; ++i) {
+          w[i] = wn[i];
+          sc[i] = sn[i];
         }
       }
       if (!ok) *abort_flag = 1;
