@@ -38,15 +38,15 @@ BatchView view(const bg_paged_batch *b) {
 }
 
 constexpr uint32_t kSMs = 148;
-constexpr uint64_t kManyTiles = 8 * 2 * kSMs;
+constexpr uint64_t kManyTiles = 8;
 
 // The kernels of one call and the layout of its workspace: partial rows o [part_rows][D] f32, then ml
 // [part_rows] float2, then the descriptions of what is to be joined.
 //   join        a shared prefix: every row joins its parts
 //   tc_pre      the prefix's units run on tcgen05
 //   tc_own      sequences of more than 16 rows run on tcgen05
-//               Both from kManyTiles tiles of 16 rows on that the decode kernel would walk instead, about 8 a
-//               block: that kernel takes ~0.6 us a tile, a tcgen05 launch ~12 us before its first result (26
+//               Both where the decode kernel would walk more than kManyTiles tiles of 16 rows a block instead:
+//               that kernel takes ~0.6 us a tile, a tcgen05 launch ~12 us before its first result (26
 //               streams of 4 heads a group behind 206 positions: TODO1; 64 behind 8192: TODO2).  What a
 //               sequence holds is bounded by its row of the page table.
 //   decode      the decode kernel has the rest: sequences of at most 16 rows beside tc_own -- not launched
@@ -78,19 +78,20 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
     return p;
   }
   const uint64_t group = (uint64_t)b->max_q * G, all = (uint64_t)b->tokens * G;
-  const bool tc = paged_tc_supported((int)kv->mode, D, kv->page_size);
+  const bool tc = paged_tc_supported((int)kv->mode, D, kv->page_size, lo);
   const uint64_t own_tiles = (all + 15) / 16 * KV * ((cap + 63) / 64);
   const uint64_t pre_tiles = (all + 15) / 16 * KV * ((uint64_t)(b->prefix_len + 63) / 64);
-  p.tc_own = tc && group > 16 && own_tiles > kManyTiles;
-  p.tc_pre = tc && p.join && all > 16 && pre_tiles > kManyTiles;
+  const uint64_t many = kManyTiles * paged_decode_blocks((int)kv->mode, D, 16);
+  p.tc_own = tc && group > 16 && own_tiles > many;
+  p.tc_pre = tc && p.join && all > 16 && pre_tiles > many;
   p.decode = !p.tc_own || (p.join && !p.tc_pre) || b->tokens < (uint64_t)b->batch * b->max_q;
   // rows of a unit: as many as a sequence's rows (or, behind a prefix, all rows) fill; f32 rows have a form for 4
   const uint64_t fill = p.tc_own ? 16 : p.join && !p.tc_pre ? (all > group ? all : group) : group;
   // (16 f32 rows of head_dim 256 do not fit the registers: two units of 8 read the positions twice, but sooner)
   p.ru = fill <= 4 && lo ? 4 : fill <= 8 || (lo && D == 256) ? 8 : 16;
   p.blocks = paged_decode_blocks((int)kv->mode, D, p.ru);
-  p.ru_own = paged_tc_rows(lo, group);
-  p.ru_pre = paged_tc_rows(lo, all);
+  p.ru_own = paged_tc_rows(D, lo, group);
+  p.ru_pre = paged_tc_rows(D, lo, all);
   uint64_t at = p.decode ? 2ull * p.blocks * p.ru : 0;
   p.slot_own = (uint32_t)at;
   if (p.tc_own) at += 2ull * kSMs * p.ru_own;

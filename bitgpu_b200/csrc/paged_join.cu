@@ -82,6 +82,7 @@ int launch_paged_join_cuts(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru,
   if (ru >= 128) {
     const dim3 wide(blocks, ru / kWarps);
     if (a.D == 128) return launch_dependent(join_cuts_wide_kernel<128>, wide, st, a, ru);
+    if (a.D == 256) return launch_dependent(join_cuts_wide_kernel<256>, wide, st, a, ru);
     return BG_EUNSUPPORTED;
   }
   const dim3 grid(blocks, ru);

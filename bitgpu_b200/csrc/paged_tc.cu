@@ -48,8 +48,12 @@ template <int D, bool Q8, bool LO, int NQT>
 struct TcCfg {
   static constexpr int NQ = LO ? 2 : 1, NK = Q8 ? 2 : 1;     // operand halves
   static constexpr int QT = kM * D * 2;                      // bytes of one f16 query tile
-  static constexpr int KT = Q8 ? 64 : 128;                   // positions of a K/V tile
-  static constexpr int PARTS = KT / 64, SLOTS = 3 - PARTS;   // 64-column parts of a score tile; score tiles per stream
+  // positions of a K/V tile, as shared memory allows beside the query halves
+  static constexpr int KT = D == 128 ? (Q8 ? 64 : 128) : (Q8 || LO ? 32 : 64);
+  static constexpr int SW = KT < 64 ? KT : 64;               // columns of a softmax step
+  static constexpr int PARTS = KT / SW, SLOTS = 3 - PARTS;   // steps per score tile; score tiles per stream
+  static constexpr int NS = D == 128 ? 2 : 1;                // streams (TMEM holds one O of 256 columns)
+  static_assert(D == 128 || (NQT == 1 && !(Q8 && LO)), "head_dim 256: one stream, no room for all halves");
   static constexpr int KVT = KT * D * 2;                     // bytes of one f16 K (or V) tile
   static constexpr int LEAD = Q8 ? 2 : 1;                    // a unit's own cost, in tiles
   static constexpr int NST = 2;                              // ring stages of K and of V
@@ -57,7 +61,7 @@ struct TcCfg {
   static constexpr int oInfo = oB + 384, oML = oInfo + 64, oScan = oML + kM * 8;
   static constexpr int SMEM = oScan + 24 * 8;
   static constexpr int THREADS = Q8 ? 640 : 384;
-  // TMEM columns: part x of stream t at (2t + x) * 64, outputs behind them
+  // TMEM columns: part x of stream t at (2t + x) * SW, outputs behind them
   static constexpr uint32_t O0 = 256, O1 = 384;
   static_assert(SMEM <= 232448, "shared memory");
 };
@@ -151,8 +155,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                     const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ TcParams p) {
   using C = TcCfg<D, Q8, LO, NQT>;
-  constexpr int KT = C::KT, NQ = C::NQ, NK = C::NK;
-  static_assert(D == 128, "two streams need two O tiles of 128 columns");
+  constexpr int KT = C::KT, SW = C::SW, NQ = C::NQ, NK = C::NK;
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::oB);
   uint64_t *k_full = bars, *k_empty = bars + 4, *v_full = bars + 8, *v_empty = bars + 12;
@@ -187,7 +190,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     mbar_init(q_full, !LO && p.q_tma ? 1 : 64);
     mbar_init(q_free, 1);
     mbar_init(mma_done, 1);
-    mbar_init(info_free, 8);
+    mbar_init(info_free, 4 * C::NS);
     mbar_init(b_done, 4);
     mbar_init(tail, 1);
     *abort_flag = 0;
@@ -302,7 +305,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     };
     // S = Q K^T into score tile u: small products first, so that they are added up among themselves
     auto issue_s = [&](int t, int u, int s) {
-      const uint32_t slot = tmem + (2 * t + u) * 64, k = k_lo + s * (NK * C::KVT / 16);
+      const uint32_t slot = tmem + (2 * t + u) * SW, k = k_lo + s * (NK * C::KVT / 16);
       const uint32_t q = q_lo + (NQT == 2 ? t : 0) * (NQ * C::QT / 16);
       if constexpr (LO) one_s(slot, q + C::QT / 16, k, std::false_type{});
       if constexpr (Q8) one_s(slot, q, k + C::KVT / 16, std::bool_constant<LO>{});
@@ -312,18 +315,18 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       if (acc) umma_ts_lo<kHi, true>(o, pa, v, idO);
       else umma_ts_lo<kHi, false>(o, pa, v, idO);
 #pragma unroll
-      for (int kk = 1; kk < 4; ++kk) umma_ts_lo<kHi, true>(o, pa + kk * 8, v + kk * (16 * 128 / 16), idO);
+      for (int kk = 1; kk < SW / 16; ++kk) umma_ts_lo<kHi, true>(o, pa + kk * 8, v + kk * (16 * 128 / 16), idO);
     };
-    // O_t += P V for 64 positions, part h of a tile (P from the columns of part x)
+    // O_t += P V for the SW positions of part h of a tile (P from the columns of part x)
     auto issue_pv = [&](int t, int x, int s, int h, bool acc) {
-      const uint32_t slot = tmem + (2 * t + x) * 64, v = v_lo + s * (NK * C::KVT / 16) + h * (64 * 128 / 16);
+      const uint32_t slot = tmem + (2 * t + x) * SW, v = v_lo + s * (NK * C::KVT / 16) + h * (SW * 128 / 16);
       const uint32_t o = tmem + (t ? C::O1 : C::O0);
-      if constexpr (LO) one_pv(o, slot + 32, v, acc);
+      if constexpr (LO) one_pv(o, slot + SW / 2, v, acc);
       if constexpr (Q8) one_pv(o, slot, v + C::KVT / 16, LO || acc);
       one_pv(o, slot, v, LO || Q8 || acc);
     };
     // a stream's tiles are STEP apart; AHEAD tiles' S come before the first PV, as far as the ring holds their K
-    constexpr int STEP = 3 - NQT, AHEAD = C::SLOTS * STEP < C::NST ? C::SLOTS * STEP : C::NST;
+    constexpr int STEP = NQT == 2 ? 1 : C::NS, AHEAD = C::SLOTS * STEP < C::NST ? C::SLOTS * STEP : C::NST;
     static_assert(AHEAD % STEP == 0, "the next S belongs to the same stream");
     bool ok = true;
     int it = 0;         // tiles of all pieces before this one
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
           send_s(0, u, i);
           send_s(1, u, i);
         } else {
-          send_s(i & 1, u, i);
+          send_s(C::NS == 2 ? i & 1 : 0, u, i);
         }
       }
       // the PVs of stream t, tile i, and behind them the S that takes over its columns: in-order execution
@@ -389,7 +392,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         if (NQT == 2) {
           step(0, i, u);
           if (ok) step(1, i, u);
-        } else if (i & 1) {
+        } else if (C::NS == 2 && (i & 1)) {
           step(1, i, u);
         } else {
           step(0, i, u);
@@ -528,6 +531,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     const uint32_t obase = (tmem + (t ? C::O1 : C::O0)) | lane_off;
     const float sl2 = a.sl2;
     bool ok = true;
+    if (t < C::NS) {
     uint32_t sp = 0;           // next phase parity of s_full, one bit per slot of this stream
     uint32_t nv = 0;           // this stream's PVs of the pieces before
     for (uint32_t piece = 0;; ++piece) {
@@ -540,29 +544,29 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       const uint32_t R = in.R0 + min(r, in.rows - 1);
       const int lim = min(in.lim_base + (int)(R / a.G), (int)in.len - 1);
       float m_used = kNegBig, l = 0.f;
-      const int step = NQT == 2 ? 1 : 2;
+      const int step = NQT == 2 ? 1 : C::NS;
       const int first = NQT == 2 ? 0 : t;
       for (int j = first; j < (int)in.ntiles; j += step) {
-       const int jj = NQT == 2 ? j : j >> 1;  // tile of this stream
+       const int jj = NQT == 2 ? j : j / C::NS;  // tile of this stream
 #pragma unroll 1
        for (int h = 0; h < C::PARTS; ++h) {
-        const int g = jj * C::PARTS + h, part = g & 1;  // 64-column step of this stream, and where it lies
+        const int g = jj * C::PARTS + h, part = g & 1;  // step of this stream, and where its scores lie
         if (h == 0) {
           const int u = C::PARTS == 2 ? 0 : part;
           if (!mbar_wait_warp(&s_full[2 * t + u], (sp >> u) & 1)) { ok = false; break; }
           sp ^= 1u << u;
           tc_fence_after();
         }
-        const uint32_t sbase = (tmem + (2 * t + part) * 64) | lane_off;
-        const int key0 = (int)(in.tile0 + j) * KT + h * 64;
-        const int nvalid = min(64, max(0, lim - key0 + 1));
-        uint32_t x[2][32];  // the step's scores of the row: one TMEM wait
+        const uint32_t sbase = (tmem + (2 * t + part) * SW) | lane_off;
+        const int key0 = (int)(in.tile0 + j) * KT + h * SW;
+        const int nvalid = min(SW, max(0, lim - key0 + 1));
+        uint32_t x[SW / 32][32];  // the step's scores of the row: one TMEM wait
 #pragma unroll
-        for (int c = 0; c < 2; ++c) tmem_ld32(sbase + c * 32, x[c]);
+        for (int c = 0; c < SW / 32; ++c) tmem_ld32(sbase + c * 32, x[c]);
         tmem_wait_ld();
-        if (nvalid < 64) {
+        if (nvalid < SW) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+          for (int c = 0; c < SW / 32; ++c)
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (c * 32 + i >= nvalid) x[c][i] = __float_as_uint(-INFINITY);
@@ -571,7 +575,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
 #pragma unroll
         for (int k = 0; k < 8; ++k) mx8[k] = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < SW / 32; ++c)
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             const int k = (c * 16 + i / 2) & 7;
@@ -608,7 +612,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         const uint64_t sl2x2 = pack2(sl2, sl2), mneg2 = pack2(mneg, mneg);
         uint64_t sums[2] = {0, 0};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < SW / 32; ++c) {
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -623,7 +627,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
             }
           }
           tmem_st16(sbase + c * 16, hi);
-          if constexpr (LO) tmem_st16(sbase + 32 + c * 16, lo);
+          if constexpr (LO) tmem_st16(sbase + SW / 2 + c * 16, lo);
         }
         const float2 sum = unpack2(add2(sums[0], sums[1]));
         l += sum.x + sum.y;
@@ -637,12 +641,12 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       }
       if (!ok) break;
       // ---- the piece's rows ----
-      const int mine = NQT == 2 ? (int)in.ntiles : ((int)in.ntiles + 1 - t) >> 1;  // this stream's tiles
+      const int mine = NQT == 2 || C::NS == 1 ? (int)in.ntiles : ((int)in.ntiles + 1 - t) >> 1;  // this stream's tiles
       const bool some = mine > 0;
       if (some && !mbar_wait_warp(&pv_done[t], (nv + mine * C::PARTS - 1) & 1)) { ok = false; break; }
       nv += mine * C::PARTS;
       float f0 = 1.f, f1 = 0.f, M = m_used, L = l;
-      if constexpr (NQT == 1) {
+      if constexpr (NQT == 1 && C::NS == 2) {
         if (t == 1) {
           // stream 0 still reads the last piece's (m, l) until it frees O
           tc_fence_after();
@@ -671,7 +675,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         uint32_t o[32];
         tmem_ld32(obase + c * 32, o);
         tmem_wait_ld();
-        if constexpr (NQT == 1) {
+        if constexpr (NQT == 1 && C::NS == 2) {
           if (in.ntiles > 1) {  // uniform: O_1 holds something
             uint32_t o1[32];
             tmem_ld32(((tmem + C::O1) | lane_off) + c * 32, o1);
@@ -715,6 +719,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_free[NQT == 2 ? t : 0]);
+    }
     }
     if (!ok) *abort_flag = 1;
   } else {
@@ -775,7 +780,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
           for (int h = 0; h < 2; ++h) {
             // the lanes of a row's second half take their two chunks in the other order: a quarter warp's
             // stores then fall on all banks
-            const uint32_t hh = h ^ (c >> 2);
+            const uint32_t hh = h ^ ((c >> 2) & 1);
             uint4 hi, lo;
             cs.split4(hh ? w[i].z : w[i].x, hi.x, hi.y, lo.x, lo.y);
             cs.split4(hh ? w[i].w : w[i].y, hi.z, hi.w, lo.z, lo.w);
@@ -853,20 +858,28 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_lo, bool p
 
 template <bool Q8>
 int launch_q(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_lo, bool prefix, cudaStream_t st) {
-  if (!(a.q_f16 && a.out_f16)) return launch_cfg<128, Q8, true, 1>(a, blocks, rows_lo, prefix, st);
+  const bool lo = !(a.q_f16 && a.out_f16);
+  if (a.D == 256) {
+    if (!lo) return launch_cfg<256, Q8, false, 1>(a, blocks, rows_lo, prefix, st);
+    if constexpr (!Q8) return launch_cfg<256, false, true, 1>(a, blocks, rows_lo, prefix, st);
+    return BG_EUNSUPPORTED;
+  }
+  if (lo) return launch_cfg<128, Q8, true, 1>(a, blocks, rows_lo, prefix, st);
   return ru == 256 ? launch_cfg<128, Q8, false, 2>(a, blocks, rows_lo, prefix, st)
                    : launch_cfg<128, Q8, false, 1>(a, blocks, rows_lo, prefix, st);
 }
 
 }  // namespace
 
-// Page boxes of at least 8 positions keep the 128-byte swizzle's pattern.
-bool paged_tc_supported(int mode, uint32_t D, uint32_t page_size) {
-  return (mode == BG_KV_F16 || mode == BG_KV_Q8) && D == 128 && page_size % 8 == 0;
+// Page boxes of at least 8 positions keep the 128-byte swizzle's pattern.  head_dim 256 with all four halves
+// (f32 rows over a q8 pool) does not fit shared memory.
+bool paged_tc_supported(int mode, uint32_t D, uint32_t page_size, bool lo) {
+  return page_size % 8 == 0 && (D == 128 ? mode == BG_KV_F16 || mode == BG_KV_Q8
+                                         : D == 256 && (mode == BG_KV_F16 || (mode == BG_KV_Q8 && !lo)));
 }
 
-// Rows of a unit: two query tiles where there are rows for them and shared memory for both (f16 rows).
-uint32_t paged_tc_rows(bool lo, uint64_t rows) { return !lo && rows > kM ? 2 * kM : kM; }
+// Rows of a unit: two query tiles where there are rows for them and memory for both (f16 rows of head_dim 128).
+uint32_t paged_tc_rows(uint32_t D, bool lo, uint64_t rows) { return D == 128 && !lo && rows > kM ? 2 * kM : kM; }
 
 int launch_paged_tc(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_lo, bool prefix, cudaStream_t st) {
   return a.mode == BG_KV_Q8 ? launch_q<true>(a, blocks, ru, rows_lo, prefix, st)

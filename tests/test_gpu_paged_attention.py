@@ -123,6 +123,15 @@ def test_prefix_many_tiles(ops, mode, io, B, G):
     run(ops, Ragged(lens, [1] * B, KV=8, G=G, mode=mode, prefix=13001, page=64, seed=B), DT[io], DT[io])
 
 
+@pytest.mark.parametrize("mode,io", [("f16", "f16"), ("f16", "f32"), ("q8", "f16"), ("q8", "f32")])
+def test_many_tiles_d256(ops, mode, io):
+    """head_dim 256, six heads a group: a long prefix and long prompts through the matrix kernels."""
+    lens = [(11 * i) % 70 + 1 for i in range(30)]
+    run(ops, Ragged(lens, [1] * 30, KV=4, G=6, D=256, mode=mode, prefix=9001, page=64, seed=3), DT[io], DT[io], gated=True)
+    run(ops, Ragged([3000, 1001, 150, 9], [130, 300, 150, 1], KV=4, G=6, D=256, mode=mode, page=16, seed=4), DT[io], DT[io],
+        gated=True)
+
+
 @pytest.mark.parametrize("mode", ["f16", "q8"])
 @pytest.mark.parametrize("io", ["f32", "f16"])
 @pytest.mark.parametrize("n", [33, 129, 257])
