@@ -78,7 +78,7 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
     return p;
   }
   const uint64_t group = (uint64_t)b->max_q * G, all = (uint64_t)b->tokens * G;
-  const bool tc = paged_tc_supported((int)kv->mode, D, kv->page_size, lo);
+  const bool tc = paged_tc_supported((int)kv->mode, D, G, kv->page_size, lo);
   const uint64_t own_tiles = (all + 15) / 16 * KV * ((cap + 63) / 64);
   const uint64_t pre_tiles = (all + 15) / 16 * KV * ((uint64_t)(b->prefix_len + 63) / 64);
   const uint64_t many = kManyTiles * paged_decode_blocks((int)kv->mode, D, 16);
@@ -90,8 +90,8 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
   // (16 f32 rows of head_dim 256 do not fit the registers: two units of 8 read the positions twice, but sooner)
   p.ru = fill <= 4 && lo ? 4 : fill <= 8 || (lo && D == 256) ? 8 : 16;
   p.blocks = paged_decode_blocks((int)kv->mode, D, p.ru);
-  p.ru_own = paged_tc_rows(D, lo, group);
-  p.ru_pre = paged_tc_rows(D, lo, all);
+  p.ru_own = paged_tc_rows(D, G, lo, group);
+  p.ru_pre = paged_tc_rows(D, G, lo, all);
   uint64_t at = p.decode ? 2ull * p.blocks * p.ru : 0;
   p.slot_own = (uint32_t)at;
   if (p.tc_own) at += 2ull * kSMs * p.ru_own;

@@ -79,8 +79,8 @@ int launch_dependent(K kern, dim3 grid, cudaStream_t st, A... args) {
 }  // namespace
 
 int launch_paged_join_cuts(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, cudaStream_t st) {
-  if (ru >= 128) {
-    const dim3 wide(blocks, ru / kWarps);
+  if (ru > 16) {  // a tcgen05 kernel's
+    const dim3 wide(blocks, (ru + kWarps - 1) / kWarps);
     if (a.D == 128) return launch_dependent(join_cuts_wide_kernel<128>, wide, st, a, ru);
     if (a.D == 256) return launch_dependent(join_cuts_wide_kernel<256>, wide, st, a, ru);
     return BG_EUNSUPPORTED;

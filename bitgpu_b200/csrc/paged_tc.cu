@@ -17,7 +17,8 @@
 //
 // Precision, by the types of the call:
 //   f16 rows, f16 pool: operands are exact, P is rounded once to f16 (kept 2^6 up, away from subnormals);
-//   f32 rows (LO): q and p are split into two f16 halves (22 bits) -- two products for S, two for O;
+//   f32 rows (LO): q and p are split into two f16 halves (22 bits) -- two products for S, two for O; weights
+//           below 2^-31 of a row's largest fall under f16's smallest step and are lost;
 //   q8 pool: code * scale has more than 11 bits, so K and V are split too when they are dequantised into
 //           the operand tiles: one more product each.  (A single f16 rounding of K and V would double the
 //           error of f16 rows; the extra products cost less than that here, because the softmax warps
@@ -72,7 +73,7 @@ struct TcParams {
   uint32_t box, ppt;  // positions of a page box, boxes per tile
   uint32_t join_rows;
   uint32_t page_shift;  // log2(page_size), or 32
-  uint32_t q_tma;     // f16 rows whose group divides 128: query tiles come by TMA
+  uint32_t rpt;       // rows of a query tile: whole tokens, at most 128
   uint32_t wide;      // out and the partial rows start on 32-byte boundaries
 };
 
@@ -132,6 +133,14 @@ struct CodeScale {
   }
 };
 
+// 1 / (1 + exp(-g)) to about 4 * 2^-24 of its value (a row's thread has head_dim of them in the epilogue, where
+// expf and a division each made a gated prompt three times as long).
+__device__ __forceinline__ float sigmoid(float g) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2_approx(-kLog2e * g)));
+  return r;
+}
+
 // N consecutive words of one row.  A row belongs to one thread, so a store instruction touches 32 rows:
 // 32-byte stores fill whole sectors (16-byte ones write every sector twice: 5.5 -> 2.5 us per 256 rows).
 template <int N>
@@ -187,7 +196,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       mbar_init(&pv_done[i], 1);
       mbar_init(&o_free[i], 4);
     }
-    mbar_init(q_full, !LO && p.q_tma ? 1 : 64);
+    mbar_init(q_full, LO ? 64 : 1);
     mbar_init(q_free, 1);
     mbar_init(mma_done, 1);
     mbar_init(info_free, 4 * C::NS);
@@ -422,7 +431,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       }
       if (!more) {
         if (gt == 0) info->ntiles = 0;
-        if (LO || !p.q_tma || gt == 0) mbar_arrive(q_full);
+        if (LO || gt == 0) mbar_arrive(q_full);
         break;
       }
       const bool whole = pc.npieces == 1;
@@ -447,21 +456,22 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
           rp[r] = RowPieces{whole ? row0 + R / a.G * a.H + pc.kvh * a.G + R % a.G : slot + r, pc.npieces, p.u.RU, 0};
         }
       }
-      if (!LO && p.q_tma) {
-        // rows behind the unit's are other sequences' (or zeros): computed along, never written
+      if constexpr (!LO) {
+        // f16 rows come by TMA as boxes of whole tokens' heads; tokens behind the unit's are other sequences'
+        // (or zeros) and the tile's last rows stay as they were: computed along, never written
         loaded = piece + 1;
         if (gt == 0) {
-          mbar_expect_tx(q_full, NQT * C::QT);
-          const int tok = (int)(pc.R0 / a.G), per = kM / (int)a.G;
+          mbar_expect_tx(q_full, NQT * p.rpt * D * 2);
+          const int tok = (int)(pc.R0 / a.G), per = (int)(p.rpt / a.G);
           for (int q = 0; q < NQT; ++q)
             for (int cb = 0; cb < D / 64; ++cb)
               tma_load_4d(smem + C::oQ + q * C::QT + cb * kM * 128, &tmQ, q_full, cb * 64, 0, (int)pc.kvh, tok + q * per);
         }
         continue;
-      }
+      } else {
       // a thread has one 16-byte column of every fourth row; (token, head) step along without divisions
       constexpr int CPR = D / 8;  // chunks of 8 values per row
-      constexpr int RS = 64 / CPR, NIT = NQT * kM / RS;
+      constexpr int RS = 64 / CPR, NIT = kM / RS;  // (one query tile)
       const uint32_t c = gt % CPR, up_t = RS / a.G, up_g = RS % a.G;
       uint32_t r = gt / CPR, tok = (pc.R0 + r) / a.G, g = (pc.R0 + r) % a.G;
       auto step = [&]() {
@@ -474,18 +484,6 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         }
       };
       const uint32_t head0 = pc.kvh * a.G;
-      if constexpr (!LO) {
-#pragma unroll 4
-        for (int i = 0; i < NIT; ++i) {
-          const bool there = r < pc.rows;
-          const uint64_t off = there ? ((uint64_t)tok * a.H + head0 + g) * CPR + c : 0;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(sQ + (r >> 7) * C::QT + sw_off<kM>(r & 127, c)),
-                       "l"(static_cast<const uint4 *>(a.q) + off), "r"(there ? 16u : 0u)
-                       : "memory");
-          step();
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-      } else {
 #pragma unroll 1
         for (int i0 = 0; i0 < NIT; i0 += 4) {
           float x[4][8];
@@ -506,7 +504,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
             uint4 hi, lo;
             split8(x[u], hi, lo);
             const uint32_t rr = r0 + u * RS;
-            unsigned char *d = smem + C::oQ + (rr >> 7) * NQ * C::QT + sw_off<kM>(rr & 127, c);
+            unsigned char *d = smem + C::oQ + sw_off<kM>(rr, c);
             *reinterpret_cast<uint4 *>(d) = hi;
             *reinterpret_cast<uint4 *>(d + C::QT) = lo;
           }
@@ -518,7 +516,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     if (!ok) {
       *abort_flag = 1;
       // no query tile may still be in flight when the block exits (otherwise q_free is behind it)
-      if (!LO && p.q_tma && gt == 0 && loaded) mbar_wait(q_full, (loaded - 1) & 1);
+      if (!LO && gt == 0 && loaded) mbar_wait(q_full, (loaded - 1) & 1);
     }
   }
   } else if (warp < 12) {
@@ -540,9 +538,15 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       __syncwarp();
       if (in.ntiles == 0) break;
       if (lane == 0) mbar_arrive(info_free);
-      const uint32_t r = (NQT == 2 ? t * kM : 0) + row;
+      const uint32_t r = (NQT == 2 ? t * p.rpt : 0) + row;
       const uint32_t R = in.R0 + min(r, in.rows - 1);
       const int lim = min(in.lim_base + (int)(R / a.G), (int)in.len - 1);
+      if (a.gate && in.dest == kDirect && (NQT == 2 || t == 0)) {
+        // the gates of the row, to L2: the epilogue would wait for HBM
+        const float *g = a.gate + ((uint64_t)(R / a.G) * a.H + in.kvh * a.G + R % a.G) * D;
+#pragma unroll 1
+        for (int i = 0; i < D / 32; ++i) asm volatile("prefetch.global.L2 [%0];" ::"l"(g + 32 * i));
+      }
       float m_used = kNegBig, l = 0.f;
       const int step = NQT == 2 ? 1 : C::NS;
       const int first = NQT == 2 ? 0 : t;
@@ -667,9 +671,16 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       }
       tc_fence_after();
       const float inv = L != 0.f ? 1.0f / L : 0.f;  // a row that attends nothing is zero
-      const bool valid = r < in.rows;
+      const bool valid = (uint32_t)row < p.rpt && r < in.rows;
       const uint64_t orow = (uint64_t)(R / a.G) * a.H + in.kvh * a.G + R % a.G;
       const uint64_t prow = in.dest == kRowBuf ? in.row0 + orow : in.dest + r;
+      const bool gated = a.gate && in.dest == kDirect && valid;
+      const float4 *gate = reinterpret_cast<const float4 *>(a.gate + orow * D);
+      float4 gn[8];  // the next chunk's gate travels while a chunk is written
+      if (gated) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) gn[i] = __ldg(gate + i);
+      }
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -695,15 +706,17 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         }
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
-        if (a.gate) {
-          const float4 *g = reinterpret_cast<const float4 *>(a.gate + orow * D + c * 32);
+        if (gated) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float4 x = __ldg(g + i);
-            o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) / (1.0f + expf(-x.x)));
-            o[4 * i + 1] = __float_as_uint(__uint_as_float(o[4 * i + 1]) / (1.0f + expf(-x.y)));
-            o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) / (1.0f + expf(-x.z)));
-            o[4 * i + 3] = __float_as_uint(__uint_as_float(o[4 * i + 3]) / (1.0f + expf(-x.w)));
+            o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) * sigmoid(gn[i].x));
+            o[4 * i + 1] = __float_as_uint(__uint_as_float(o[4 * i + 1]) * sigmoid(gn[i].y));
+            o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) * sigmoid(gn[i].z));
+            o[4 * i + 3] = __float_as_uint(__uint_as_float(o[4 * i + 3]) * sigmoid(gn[i].w));
+          }
+          if (c + 1 < D / 32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) gn[i] = __ldg(gate + 8 * (c + 1) + i);
           }
         }
         if (a.out_f16) {
@@ -815,7 +828,8 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_lo, bool p
   TcParams p;
   p.a = a;
   // a launch has either the prefix's units or the sequences' own
-  p.u = unit_shape(a.G, a.kv.KV, NQT * kM, C::KT, C::LEAD, prefix ? 0xffffffffu : rows_lo, 0xffffffffu, prefix);
+  p.rpt = kM / a.G * a.G;
+  p.u = unit_shape(a.G, a.kv.KV, NQT * p.rpt, C::KT, C::LEAD, prefix ? 0xffffffffu : rows_lo, 0xffffffffu, prefix);
   p.box = page_box(ps, C::KT);
   p.ppt = C::KT / p.box;
   p.page_shift = 32;
@@ -823,12 +837,11 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_lo, bool p
     if (1u << i == ps) p.page_shift = i;
   p.join_rows = a.own_pieces != nullptr;
   CUtensorMap tk = {}, tv = {}, tq = {};
-  p.q_tma = !LO && kM % a.G == 0;
   p.wide = (((uintptr_t)a.out | (uintptr_t)a.part_o) & 31) == 0;
-  if (p.q_tma) {
+  if (!LO) {
     const uint64_t dims[4] = {D, a.G, a.kv.KV, a.bv.T};
     const uint64_t strides[3] = {D * 2, (uint64_t)a.G * D * 2, (uint64_t)a.H * D * 2};
-    const uint32_t box[4] = {64, a.G, 1, kM / a.G};
+    const uint32_t box[4] = {64, a.G, 1, p.rpt / a.G};
     if (make_tmap_4d(&tq, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return BG_EUNSUPPORTED;
   }
   if (!Q8) {
@@ -865,7 +878,7 @@ int launch_q(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows
     return BG_EUNSUPPORTED;
   }
   if (lo) return launch_cfg<128, Q8, true, 1>(a, blocks, rows_lo, prefix, st);
-  return ru == 256 ? launch_cfg<128, Q8, false, 2>(a, blocks, rows_lo, prefix, st)
+  return ru > kM ? launch_cfg<128, Q8, false, 2>(a, blocks, rows_lo, prefix, st)
                    : launch_cfg<128, Q8, false, 1>(a, blocks, rows_lo, prefix, st);
 }
 
@@ -873,13 +886,18 @@ int launch_q(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows
 
 // Page boxes of at least 8 positions keep the 128-byte swizzle's pattern.  head_dim 256 with all four halves
 // (f32 rows over a q8 pool) does not fit shared memory.
-bool paged_tc_supported(int mode, uint32_t D, uint32_t page_size, bool lo) {
-  return page_size % 8 == 0 && (D == 128 ? mode == BG_KV_F16 || mode == BG_KV_Q8
-                                         : D == 256 && (mode == BG_KV_F16 || (mode == BG_KV_Q8 && !lo)));
+bool paged_tc_supported(int mode, uint32_t D, uint32_t G, uint32_t page_size, bool lo) {
+  return G <= kM && page_size % 8 == 0 &&
+         (D == 128 ? mode == BG_KV_F16 || mode == BG_KV_Q8
+                   : D == 256 && (mode == BG_KV_F16 || (mode == BG_KV_Q8 && !lo)));
 }
 
-// Rows of a unit: two query tiles where there are rows for them and memory for both (f16 rows of head_dim 128).
-uint32_t paged_tc_rows(uint32_t D, bool lo, uint64_t rows) { return D == 128 && !lo && rows > kM ? 2 * kM : kM; }
+// Rows of a unit: whole tokens' heads, two query tiles where there are rows for them and memory for both (f16
+// rows of head_dim 128).
+uint32_t paged_tc_rows(uint32_t D, uint32_t G, bool lo, uint64_t rows) {
+  const uint32_t tile = kM / G * G;
+  return D == 128 && !lo && rows > tile ? 2 * tile : tile;
+}
 
 int launch_paged_tc(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_lo, bool prefix, cudaStream_t st) {
   return a.mode == BG_KV_Q8 ? launch_q<true>(a, blocks, ru, rows_lo, prefix, st)
