@@ -376,7 +376,7 @@ bool paged_decode_supported(int mode, uint32_t D, uint32_t page_size);
 uint32_t paged_decode_blocks(int mode, uint32_t D, uint32_t ru);  // blocks that fill the GPU
 int launch_paged_decode(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_hi, bool prefix, cudaStream_t st);
 // tcgen05 kernel: many rows a sequence (own part), or the rows of the batch against the shared prefix.
-bool paged_tc_supported(int mode, uint32_t D, uint32_t G, uint32_t page_size, bool lo);
+bool paged_tc_supported(int mode, uint32_t D, uint32_t G, uint32_t page_size);
 uint32_t paged_tc_rows(uint32_t D, uint32_t G, bool lo, uint64_t rows);
 int launch_paged_tc(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_lo, bool prefix, cudaStream_t st);
 // Join the cut units of `blocks` blocks of ru rows (no prefix), or every row's pieces (prefix).

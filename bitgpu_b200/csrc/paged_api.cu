@@ -46,9 +46,10 @@ constexpr uint64_t kManyTiles = 8;
 //   tc_pre      the prefix's units run on tcgen05
 //   tc_own      sequences of more than 16 rows run on tcgen05
 //               Both where the decode kernel would walk more than kManyTiles tiles of 16 rows a block instead:
-//               that kernel takes ~0.6 us a tile, a tcgen05 launch ~12 us before its first result (26
-//               streams of 4 heads a group behind 206 positions: TODO1; 64 behind 8192: TODO2).  What a
-//               sequence holds is bounded by its row of the page table.
+//               that kernel takes ~0.6 us a tile, a tcgen05 launch ~12 us before its first result (f16, 8
+//               kv heads of 4; decode kernel and tcgen05: 26 streams behind 206 shared positions 16 and
+//               23 us, 64 behind 8192 103 and 43; 4 prompts of 64 tokens after 236 positions 31 and 23).
+//               What a sequence holds is bounded by its row of the page table.
 //   decode      the decode kernel has the rest: sequences of at most 16 rows beside tc_own -- not launched
 //               where tokens == batch * max_q says that there are none; were it wrong, tc_own has them
 struct Plan {
@@ -78,12 +79,15 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
     return p;
   }
   const uint64_t group = (uint64_t)b->max_q * G, all = (uint64_t)b->tokens * G;
-  const bool tc = paged_tc_supported((int)kv->mode, D, G, kv->page_size, lo);
+  const bool tc = paged_tc_supported((int)kv->mode, D, G, kv->page_size);
   const uint64_t own_tiles = (all + 15) / 16 * KV * ((cap + 63) / 64);
   const uint64_t pre_tiles = (all + 15) / 16 * KV * ((uint64_t)(b->prefix_len + 63) / 64);
   const uint64_t many = kManyTiles * paged_decode_blocks((int)kv->mode, D, 16);
-  p.tc_own = tc && group > 16 && own_tiles > many;
-  p.tc_pre = tc && p.join && all > 16 && pre_tiles > many;
+  // f32 rows over a q8 pool of head_dim 256 have a ring of one stage: 36 rows a sequence behind 953 positions take
+  // 160 us there and 138 with the decode kernel, 60 behind 13388 shared ones 78 and 104
+  const uint64_t few = lo && D == 256 && kv->mode == BG_KV_Q8 ? 48 : 16;
+  p.tc_own = tc && group > few && own_tiles > many;
+  p.tc_pre = tc && p.join && all > few && pre_tiles > many;
   p.decode = !p.tc_own || (p.join && !p.tc_pre) || b->tokens < (uint64_t)b->batch * b->max_q;
   // rows of a unit: as many as a sequence's rows (or, behind a prefix, all rows) fill; f32 rows have a form for 4
   const uint64_t fill = p.tc_own ? 16 : p.join && !p.tc_pre ? (all > group ? all : group) : group;

@@ -54,10 +54,10 @@ struct TcCfg {
   static constexpr int SW = KT < 64 ? KT : 64;               // columns of a softmax step
   static constexpr int PARTS = KT / SW, SLOTS = 3 - PARTS;   // steps per score tile; score tiles per stream
   static constexpr int NS = D == 128 ? 2 : 1;                // streams (TMEM holds one O of 256 columns)
-  static_assert(D == 128 || (NQT == 1 && !(Q8 && LO)), "head_dim 256: one stream, no room for all halves");
+  static_assert(D == 128 || NQT == 1, "head_dim 256: one stream");
   static constexpr int KVT = KT * D * 2;                     // bytes of one f16 K (or V) tile
   static constexpr int LEAD = Q8 ? 2 : 1;                    // a unit's own cost, in tiles
-  static constexpr int NST = 2;                              // ring stages of K and of V
+  static constexpr int NST = D == 256 && Q8 && LO ? 1 : 2;   // ring stages of K and of V
   static constexpr int oQ = 0, oK = NQT * NQ * QT, oV = oK + NST * NK * KVT, oB = oV + NST * NK * KVT;
   static constexpr int oInfo = oB + 384, oML = oInfo + 64, oScan = oML + kM * 8;
   static constexpr int SMEM = oScan + 24 * 8;
@@ -224,301 +224,301 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
 
   // registers: 384 threads: 128*72 + 256*216 = 384*168; 640: 128*64 + 256*128 + 256*80 = 640*96
   if (warp < 4) {
-  if constexpr (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;" ::: "memory");
-  else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
-  if (warp == 0) {
-    // ---------------- TMA producer (f16 pool) ----------------
-    if constexpr (!Q8) {
+    if constexpr (Q8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;" ::: "memory");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;" ::: "memory");
+    if (warp == 0) {
+      // ---------------- TMA producer (f16 pool) ----------------
+      if constexpr (!Q8) {
+        PieceWalk walk;
+        walk.init(span, a.bv, p.u, ps);
+        Piece pc;
+        bool ok = true;
+        int it = 0, tails = 0, kdone = 0, vdone = 0;
+        while (ok && walk.next(pc, a.bv, p.u, ps)) {
+          auto page_of = [&](uint32_t tile) -> uint32_t {
+            const uint32_t pos = (pc.tile0 + tile) * KT + lane * p.box;
+            if ((uint32_t)lane >= p.ppt || tile >= pc.ntiles || pos >= pc.len) return a.kv.num_pages;
+            const uint32_t pg = (uint32_t)__ldg(pc.pages + pos / ps);
+            if (pg < a.kv.num_pages) return pg;
+            atomicExch(&g_device_error, BG_EINVAL);
+            return a.kv.num_pages;
+          };
+          uint32_t pg_next = page_of(0);
+          for (uint32_t t = 0; ok && t < pc.ntiles; ++t, ++it) {
+            const uint32_t pg = pg_next;
+            pg_next = page_of(t + 1);
+            const int s = it % C::NST;
+            const uint32_t pos0 = (pc.tile0 + t) * KT, par = ((it / C::NST) - 1) & 1;
+            const int y = (int)((pos0 + lane * p.box) % ps);
+            if (it >= C::NST) ok = mbar_wait_warp(&k_empty[s], par);
+            if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
+            if (lane == 0) mbar_expect_tx(&k_full[s], C::KVT);
+            __syncwarp();
+            if ((uint32_t)lane < p.ppt)
+              for (int cb = 0; cb < D / 64; ++cb)
+                tma_load_4d(smem + C::oK + s * C::KVT + cb * KT * 128 + lane * p.box * 128, &tmK, &k_full[s], cb * 64,
+                            (int)pc.kvh, y, (int)pg);
+            kdone = it + 1;
+            if (it >= C::NST) ok = mbar_wait_warp(&v_empty[s], par);
+            if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
+            // slots of the last page behind the length may hold NaN, and 0 * NaN is NaN: such a tile
+            // arrives on its own barrier, its rows behind the length are cleared, then it is handed on
+            const bool last = pos0 + KT > pc.len && pc.len > pos0 && pc.len % p.box;
+            uint64_t *bar = last ? tail : &v_full[s];
+            if (lane == 0) mbar_expect_tx(bar, C::KVT);
+            __syncwarp();
+            unsigned char *dst = smem + C::oV + s * C::KVT;
+            if ((uint32_t)lane < p.ppt)
+              for (int cb = 0; cb < D / 64; ++cb)
+                tma_load_4d(dst + cb * KT * 128 + lane * p.box * 128, &tmV, bar, cb * 64, (int)pc.kvh, y, (int)pg);
+            if (last) {
+              ok = mbar_wait_warp(tail, tails++ & 1);
+              if (!ok) break;
+              const uint32_t r0 = pc.len - pos0, r1 = (r0 + p.box - 1) / p.box * p.box, n = (r1 - r0) * 8;
+              for (uint32_t i = lane; i < n * (D / 64); i += 32) {
+                const uint32_t cb = i / n, x = i % n;
+                *reinterpret_cast<uint4 *>(dst + cb * KT * 128 + r0 * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+              }
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&v_full[s]);
+            }
+            vdone = it + 1;
+          }
+        }
+        if (!ok && lane == 0) *abort_flag = 1;
+        // no copy may still be in flight when the block exits
+        if (lane == 0) {
+          for (int i = max(0, kdone - C::NST); i < kdone; ++i) mbar_wait(&k_full[i % C::NST], (i / C::NST) & 1);
+          for (int i = max(0, vdone - C::NST); i < vdone; ++i) mbar_wait(&v_full[i % C::NST], (i / C::NST) & 1);
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------- MMA issuer ----------------
+      // The whole warp runs the loop and one elected lane issues: so the compiler knows every operand to be
+      // uniform (run by one lane under a branch, each MMA first moves its descriptors to uniform registers:
+      // 2900 -> 1720 cycles for a tile's 24 MMAs and their barriers).  One warp for both streams on purpose:
+      // it serves them in turn, which keeps them half a step apart, one on the tensor pipe under the other's
+      // softmax.  (With a warp each they fall into step, wait for the pipe together and then for the exp unit.)
+      const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+      constexpr uint32_t idS = idesc_f16(KT, false), idO = idesc_f16(D, true);
+      constexpr uint32_t kHi = umma_desc_hi(1024);
+      const uint32_t q_lo = umma_desc_lo(sQ, 16), k_lo = umma_desc_lo(sK, 16), v_lo = umma_desc_lo(sV, KT * 128);
+      // one product over D (K steps of 16 values, 32 bytes of a 128-byte swizzle row)
+      auto one_s = [&](uint32_t slot, uint32_t q, uint32_t k, auto acc) {
+        umma_ss_lo<kHi, decltype(acc)::value>(slot, q, k, idS);
+#pragma unroll
+        for (int kk = 1; kk < D / 16; ++kk)
+          umma_ss_lo<kHi, true>(slot, q + ((kk >> 2) * (kM * 128) + (kk & 3) * 32) / 16,
+                                k + ((kk >> 2) * (KT * 128) + (kk & 3) * 32) / 16, idS);
+      };
+      // S = Q K^T into score tile u: small products first, so that they are added up among themselves
+      auto issue_s = [&](int t, int u, int s) {
+        const uint32_t slot = tmem + (2 * t + u) * SW, k = k_lo + s * (NK * C::KVT / 16);
+        const uint32_t q = q_lo + (NQT == 2 ? t : 0) * (NQ * C::QT / 16);
+        if constexpr (LO) one_s(slot, q + C::QT / 16, k, std::false_type{});
+        if constexpr (Q8) one_s(slot, q, k + C::KVT / 16, std::bool_constant<LO>{});
+        one_s(slot, q, k, std::bool_constant<LO || Q8>{});
+      };
+      auto one_pv = [&](uint32_t o, uint32_t pa, uint32_t v, bool acc) {
+        if (acc) umma_ts_lo<kHi, true>(o, pa, v, idO);
+        else umma_ts_lo<kHi, false>(o, pa, v, idO);
+#pragma unroll
+        for (int kk = 1; kk < SW / 16; ++kk) umma_ts_lo<kHi, true>(o, pa + kk * 8, v + kk * (16 * 128 / 16), idO);
+      };
+      // O_t += P V for the SW positions of part h of a tile (P from the columns of part x)
+      auto issue_pv = [&](int t, int x, int s, int h, bool acc) {
+        const uint32_t slot = tmem + (2 * t + x) * SW, v = v_lo + s * (NK * C::KVT / 16) + h * (SW * 128 / 16);
+        const uint32_t o = tmem + (t ? C::O1 : C::O0);
+        if constexpr (LO) one_pv(o, slot + SW / 2, v, acc);
+        if constexpr (Q8) one_pv(o, slot, v + C::KVT / 16, LO || acc);
+        one_pv(o, slot, v, LO || Q8 || acc);
+      };
+      // a stream's tiles are STEP apart; AHEAD tiles' S come before the first PV, as far as the ring holds their K
+      constexpr int STEP = NQT == 2 ? 1 : C::NS, AHEAD = C::SLOTS * STEP < C::NST ? C::SLOTS * STEP : C::NST;
+      static_assert(AHEAD % STEP == 0, "the next S belongs to the same stream");
+      bool ok = true;
+      int it = 0;         // tiles of all pieces before this one
+      uint32_t pp = 0;    // next phase parity of p_full, one bit per part
+      for (uint32_t piece = 0; ok; ++piece) {
+        if (!mbar_wait_warp(q_full, piece & 1)) { ok = false; break; }
+        const int n = (int)__shfl_sync(0xffffffffu, info->ntiles, 0);
+        if (n == 0) break;
+        auto stage = [&](int i) { return (it + i) % C::NST; };
+        auto wait_k = [&](int i) { return mbar_wait_warp(&k_full[stage(i)], ((it + i) / C::NST) & 1); };
+        auto wait_v = [&](int i) { return mbar_wait_warp(&v_full[stage(i)], ((it + i) / C::NST) & 1); };
+        // S of stream t, tile i; the last reader of K_i frees it, the last S of the piece frees Q
+        auto send_s = [&](int t, int u, int i) {
+          tc_fence_after();
+          if (elect_one()) {
+            issue_s(t, u, stage(i));
+            umma_commit(&s_full[2 * t + u]);
+            if (NQT == 1 || t == 1) {
+              umma_commit(&k_empty[stage(i)]);
+              if (i + 1 == n) umma_commit(q_free);
+            }
+          }
+          __syncwarp();
+        };
+        for (int i = 0; ok && i < AHEAD && i < n; ++i) {
+          ok = wait_k(i);
+          if (!ok) break;
+          const int u = (i / STEP) % C::SLOTS;
+          if (NQT == 2) {
+            send_s(0, u, i);
+            send_s(1, u, i);
+          } else {
+            send_s(C::NS == 2 ? i & 1 : 0, u, i);
+          }
+        }
+        // the PVs of stream t, tile i, and behind them the S that takes over its columns: in-order execution
+        // keeps P safe
+        auto step = [&](int t, int i, int u) {
+          if (NQT == 1 || t == 0) ok = wait_v(i);
+          if (ok && i < STEP && piece > 0) ok = mbar_wait_warp(&o_free[NQT == 2 ? t : 0], (piece - 1) & 1);
+#pragma unroll
+          for (int h = 0; h < C::PARTS; ++h) {
+            const int x = C::PARTS == 2 ? h : u, b = 2 * t + x;
+            ok = ok && mbar_wait_warp(&p_full[b], (pp >> b) & 1);
+            if (!ok) return;
+            pp ^= 1u << b;
+            tc_fence_after();
+            if (elect_one()) {
+              issue_pv(t, x, stage(i), h, i >= STEP || h > 0);
+              umma_commit(&pv_done[t]);
+              if (h == C::PARTS - 1 && (NQT == 1 || t == 1)) umma_commit(&v_empty[stage(i)]);
+            }
+            __syncwarp();
+          }
+          if (i + AHEAD < n) {
+            // (only now: the ring may not hold this K before V(i) has been used)
+            if (NQT == 1 || t == 0) ok = wait_k(i + AHEAD);
+            if (ok) send_s(t, ((i + AHEAD) / STEP) % C::SLOTS, i + AHEAD);
+          }
+        };
+        for (int i = 0; ok && i < n; ++i) {
+          const int u = (i / STEP) % C::SLOTS;
+          if (NQT == 2) {
+            step(0, i, u);
+            if (ok) step(1, i, u);
+          } else if (C::NS == 2 && (i & 1)) {
+            step(1, i, u);
+          } else {
+            step(0, i, u);
+          }
+        }
+        it += n;
+      }
+      if (!ok) *abort_flag = 1;
+      // every MMA must complete before the block frees its TMEM
+      if (elect_one()) umma_commit(mma_done);
+      __syncwarp();
+      mbar_wait_warp(mma_done, 0);
+    } else {
+      // ---------------- query rows and descriptions ----------------
+      const int gt = (warp - 2) * 32 + lane;
       PieceWalk walk;
       walk.init(span, a.bv, p.u, ps);
       Piece pc;
       bool ok = true;
-      int it = 0, tails = 0, kdone = 0, vdone = 0;
-      while (ok && walk.next(pc, a.bv, p.u, ps)) {
-        auto page_of = [&](uint32_t tile) -> uint32_t {
-          const uint32_t pos = (pc.tile0 + tile) * KT + lane * p.box;
-          if ((uint32_t)lane >= p.ppt || tile >= pc.ntiles || pos >= pc.len) return a.kv.num_pages;
-          const uint32_t pg = (uint32_t)__ldg(pc.pages + pos / ps);
-          if (pg < a.kv.num_pages) return pg;
-          atomicExch(&g_device_error, BG_EINVAL);
-          return a.kv.num_pages;
-        };
-        uint32_t pg_next = page_of(0);
-        for (uint32_t t = 0; ok && t < pc.ntiles; ++t, ++it) {
-          const uint32_t pg = pg_next;
-          pg_next = page_of(t + 1);
-          const int s = it % C::NST;
-          const uint32_t pos0 = (pc.tile0 + t) * KT, par = ((it / C::NST) - 1) & 1;
-          const int y = (int)((pos0 + lane * p.box) % ps);
-          if (it >= C::NST) ok = mbar_wait_warp(&k_empty[s], par);
-          if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
-          if (lane == 0) mbar_expect_tx(&k_full[s], C::KVT);
-          __syncwarp();
-          if ((uint32_t)lane < p.ppt)
-            for (int cb = 0; cb < D / 64; ++cb)
-              tma_load_4d(smem + C::oK + s * C::KVT + cb * KT * 128 + lane * p.box * 128, &tmK, &k_full[s], cb * 64,
-                          (int)pc.kvh, y, (int)pg);
-          kdone = it + 1;
-          if (it >= C::NST) ok = mbar_wait_warp(&v_empty[s], par);
-          if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
-          // slots of the last page behind the length may hold NaN, and 0 * NaN is NaN: such a tile
-          // arrives on its own barrier, its rows behind the length are cleared, then it is handed on
-          const bool last = pos0 + KT > pc.len && pc.len > pos0 && pc.len % p.box;
-          uint64_t *bar = last ? tail : &v_full[s];
-          if (lane == 0) mbar_expect_tx(bar, C::KVT);
-          __syncwarp();
-          unsigned char *dst = smem + C::oV + s * C::KVT;
-          if ((uint32_t)lane < p.ppt)
-            for (int cb = 0; cb < D / 64; ++cb)
-              tma_load_4d(dst + cb * KT * 128 + lane * p.box * 128, &tmV, bar, cb * 64, (int)pc.kvh, y, (int)pg);
-          if (last) {
-            ok = mbar_wait_warp(tail, tails++ & 1);
-            if (!ok) break;
-            const uint32_t r0 = pc.len - pos0, r1 = (r0 + p.box - 1) / p.box * p.box, n = (r1 - r0) * 8;
-            for (uint32_t i = lane; i < n * (D / 64); i += 32) {
-              const uint32_t cb = i / n, x = i % n;
-              *reinterpret_cast<uint4 *>(dst + cb * KT * 128 + r0 * 128 + x * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&v_full[s]);
-          }
-          vdone = it + 1;
+      uint32_t loaded = 0;  // pieces whose query tile was asked for
+      if (a.cuts && gt == 0) a.cuts[blockIdx.x].npieces = 0;
+      for (uint32_t piece = 0; ok; ++piece) {
+        const bool more = walk.next(pc, a.bv, p.u, ps);
+        if (piece > 0) {
+          ok = mbar_wait_warp(q_free, (piece - 1) & 1) && mbar_wait_warp(info_free, (piece - 1) & 1);
+          if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) break;
         }
-      }
-      if (!ok && lane == 0) *abort_flag = 1;
-      // no copy may still be in flight when the block exits
-      if (lane == 0) {
-        for (int i = max(0, kdone - C::NST); i < kdone; ++i) mbar_wait(&k_full[i % C::NST], (i / C::NST) & 1);
-        for (int i = max(0, vdone - C::NST); i < vdone; ++i) mbar_wait(&v_full[i % C::NST], (i / C::NST) & 1);
-      }
-    }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    // The whole warp runs the loop and one elected lane issues: so the compiler knows every operand to be
-    // uniform (run by one lane under a branch, each MMA first moves its descriptors to uniform registers:
-    // 2900 -> 1720 cycles for a tile's 24 MMAs and their barriers).  One warp for both streams on purpose:
-    // it serves them in turn, which keeps them half a step apart, one on the tensor pipe under the other's
-    // softmax.  (With a warp each they fall into step, wait for the pipe together and then for the exp unit.)
-    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
-    constexpr uint32_t idS = idesc_f16(KT, false), idO = idesc_f16(D, true);
-    constexpr uint32_t kHi = umma_desc_hi(1024);
-    const uint32_t q_lo = umma_desc_lo(sQ, 16), k_lo = umma_desc_lo(sK, 16), v_lo = umma_desc_lo(sV, KT * 128);
-    // one product over D (K steps of 16 values, 32 bytes of a 128-byte swizzle row)
-    auto one_s = [&](uint32_t slot, uint32_t q, uint32_t k, auto acc) {
-      umma_ss_lo<kHi, decltype(acc)::value>(slot, q, k, idS);
-#pragma unroll
-      for (int kk = 1; kk < D / 16; ++kk)
-        umma_ss_lo<kHi, true>(slot, q + ((kk >> 2) * (kM * 128) + (kk & 3) * 32) / 16,
-                              k + ((kk >> 2) * (KT * 128) + (kk & 3) * 32) / 16, idS);
-    };
-    // S = Q K^T into score tile u: small products first, so that they are added up among themselves
-    auto issue_s = [&](int t, int u, int s) {
-      const uint32_t slot = tmem + (2 * t + u) * SW, k = k_lo + s * (NK * C::KVT / 16);
-      const uint32_t q = q_lo + (NQT == 2 ? t : 0) * (NQ * C::QT / 16);
-      if constexpr (LO) one_s(slot, q + C::QT / 16, k, std::false_type{});
-      if constexpr (Q8) one_s(slot, q, k + C::KVT / 16, std::bool_constant<LO>{});
-      one_s(slot, q, k, std::bool_constant<LO || Q8>{});
-    };
-    auto one_pv = [&](uint32_t o, uint32_t pa, uint32_t v, bool acc) {
-      if (acc) umma_ts_lo<kHi, true>(o, pa, v, idO);
-      else umma_ts_lo<kHi, false>(o, pa, v, idO);
-#pragma unroll
-      for (int kk = 1; kk < SW / 16; ++kk) umma_ts_lo<kHi, true>(o, pa + kk * 8, v + kk * (16 * 128 / 16), idO);
-    };
-    // O_t += P V for the SW positions of part h of a tile (P from the columns of part x)
-    auto issue_pv = [&](int t, int x, int s, int h, bool acc) {
-      const uint32_t slot = tmem + (2 * t + x) * SW, v = v_lo + s * (NK * C::KVT / 16) + h * (SW * 128 / 16);
-      const uint32_t o = tmem + (t ? C::O1 : C::O0);
-      if constexpr (LO) one_pv(o, slot + SW / 2, v, acc);
-      if constexpr (Q8) one_pv(o, slot, v + C::KVT / 16, LO || acc);
-      one_pv(o, slot, v, LO || Q8 || acc);
-    };
-    // a stream's tiles are STEP apart; AHEAD tiles' S come before the first PV, as far as the ring holds their K
-    constexpr int STEP = NQT == 2 ? 1 : C::NS, AHEAD = C::SLOTS * STEP < C::NST ? C::SLOTS * STEP : C::NST;
-    static_assert(AHEAD % STEP == 0, "the next S belongs to the same stream");
-    bool ok = true;
-    int it = 0;         // tiles of all pieces before this one
-    uint32_t pp = 0;    // next phase parity of p_full, one bit per part
-    for (uint32_t piece = 0; ok; ++piece) {
-      if (!mbar_wait_warp(q_full, piece & 1)) { ok = false; break; }
-      const int n = (int)__shfl_sync(0xffffffffu, info->ntiles, 0);
-      if (n == 0) break;
-      auto stage = [&](int i) { return (it + i) % C::NST; };
-      auto wait_k = [&](int i) { return mbar_wait_warp(&k_full[stage(i)], ((it + i) / C::NST) & 1); };
-      auto wait_v = [&](int i) { return mbar_wait_warp(&v_full[stage(i)], ((it + i) / C::NST) & 1); };
-      // S of stream t, tile i; the last reader of K_i frees it, the last S of the piece frees Q
-      auto send_s = [&](int t, int u, int i) {
-        tc_fence_after();
-        if (elect_one()) {
-          issue_s(t, u, stage(i));
-          umma_commit(&s_full[2 * t + u]);
-          if (NQT == 1 || t == 1) {
-            umma_commit(&k_empty[stage(i)]);
-            if (i + 1 == n) umma_commit(q_free);
-          }
+        if (!more) {
+          if (gt == 0) info->ntiles = 0;
+          if (LO || gt == 0) mbar_arrive(q_full);
+          break;
         }
-        __syncwarp();
-      };
-      for (int i = 0; ok && i < AHEAD && i < n; ++i) {
-        ok = wait_k(i);
-        if (!ok) break;
-        const int u = (i / STEP) % C::SLOTS;
-        if (NQT == 2) {
-          send_s(0, u, i);
-          send_s(1, u, i);
-        } else {
-          send_s(C::NS == 2 ? i & 1 : 0, u, i);
-        }
-      }
-      // the PVs of stream t, tile i, and behind them the S that takes over its columns: in-order execution
-      // keeps P safe
-      auto step = [&](int t, int i, int u) {
-        if (NQT == 1 || t == 0) ok = wait_v(i);
-        if (ok && i < STEP && piece > 0) ok = mbar_wait_warp(&o_free[NQT == 2 ? t : 0], (piece - 1) & 1);
-#pragma unroll
-        for (int h = 0; h < C::PARTS; ++h) {
-          const int x = C::PARTS == 2 ? h : u, b = 2 * t + x;
-          ok = ok && mbar_wait_warp(&p_full[b], (pp >> b) & 1);
-          if (!ok) return;
-          pp ^= 1u << b;
-          tc_fence_after();
-          if (elect_one()) {
-            issue_pv(t, x, stage(i), h, i >= STEP || h > 0);
-            umma_commit(&pv_done[t]);
-            if (h == C::PARTS - 1 && (NQT == 1 || t == 1)) umma_commit(&v_empty[stage(i)]);
-          }
-          __syncwarp();
-        }
-        if (i + AHEAD < n) {
-          // (only now: the ring may not hold this K before V(i) has been used)
-          if (NQT == 1 || t == 0) ok = wait_k(i + AHEAD);
-          if (ok) send_s(t, ((i + AHEAD) / STEP) % C::SLOTS, i + AHEAD);
-        }
-      };
-      for (int i = 0; ok && i < n; ++i) {
-        const int u = (i / STEP) % C::SLOTS;
-        if (NQT == 2) {
-          step(0, i, u);
-          if (ok) step(1, i, u);
-        } else if (C::NS == 2 && (i & 1)) {
-          step(1, i, u);
-        } else {
-          step(0, i, u);
-        }
-      }
-      it += n;
-    }
-    if (!ok) *abort_flag = 1;
-    // every MMA must complete before the block frees its TMEM
-    if (elect_one()) umma_commit(mma_done);
-    __syncwarp();
-    mbar_wait_warp(mma_done, 0);
-  } else {
-    // ---------------- query rows and descriptions ----------------
-    const int gt = (warp - 2) * 32 + lane;
-    PieceWalk walk;
-    walk.init(span, a.bv, p.u, ps);
-    Piece pc;
-    bool ok = true;
-    uint32_t loaded = 0;  // pieces whose query tile was asked for
-    if (a.cuts && gt == 0) a.cuts[blockIdx.x].npieces = 0;
-    for (uint32_t piece = 0; ok; ++piece) {
-      const bool more = walk.next(pc, a.bv, p.u, ps);
-      if (piece > 0) {
-        ok = mbar_wait_warp(q_free, (piece - 1) & 1) && mbar_wait_warp(info_free, (piece - 1) & 1);
-        if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) break;
-      }
-      if (!more) {
-        if (gt == 0) info->ntiles = 0;
-        if (LO || gt == 0) mbar_arrive(q_full);
-        break;
-      }
-      const bool whole = pc.npieces == 1;
-      const uint32_t slot = a.slot0 + (2 * blockIdx.x + (pc.starts ? 1 : 0)) * p.u.RU;
-      const uint32_t row0 = pc.own ? a.own_row0 : a.pre_row0;
-      if (gt == 0) {
-        info->R0 = pc.R0;
-        info->rows = pc.rows;
-        info->kvh = pc.kvh;
-        info->tile0 = pc.tile0;
-        info->ntiles = pc.ntiles;
-        info->len = pc.len;
-        info->lim_base = pc.lim_base;
-        info->dest = !whole ? slot : p.join_rows ? kRowBuf : kDirect;
-        info->row0 = row0;
-        if (!p.join_rows && !whole && pc.starts) a.cuts[blockIdx.x] = CutUnit{pc.R0, pc.rows, pc.kvh, pc.npieces};
-      }
-      if (p.join_rows && pc.starts) {
-        RowPieces *rp = (pc.own ? a.own_pieces : a.pre_pieces) + (uint64_t)pc.kvh * a.bv.T * a.G + pc.R0;
-        for (uint32_t r = gt; r < pc.rows; r += 64) {
-          const uint32_t R = pc.R0 + r;
-          rp[r] = RowPieces{whole ? row0 + R / a.G * a.H + pc.kvh * a.G + R % a.G : slot + r, pc.npieces, p.u.RU, 0};
-        }
-      }
-      if constexpr (!LO) {
-        // f16 rows come by TMA as boxes of whole tokens' heads; tokens behind the unit's are other sequences'
-        // (or zeros) and the tile's last rows stay as they were: computed along, never written
-        loaded = piece + 1;
+        const bool whole = pc.npieces == 1;
+        const uint32_t slot = a.slot0 + (2 * blockIdx.x + (pc.starts ? 1 : 0)) * p.u.RU;
+        const uint32_t row0 = pc.own ? a.own_row0 : a.pre_row0;
         if (gt == 0) {
-          mbar_expect_tx(q_full, NQT * p.rpt * D * 2);
-          const int tok = (int)(pc.R0 / a.G), per = (int)(p.rpt / a.G);
-          for (int q = 0; q < NQT; ++q)
-            for (int cb = 0; cb < D / 64; ++cb)
-              tma_load_4d(smem + C::oQ + q * C::QT + cb * kM * 128, &tmQ, q_full, cb * 64, 0, (int)pc.kvh, tok + q * per);
+          info->R0 = pc.R0;
+          info->rows = pc.rows;
+          info->kvh = pc.kvh;
+          info->tile0 = pc.tile0;
+          info->ntiles = pc.ntiles;
+          info->len = pc.len;
+          info->lim_base = pc.lim_base;
+          info->dest = !whole ? slot : p.join_rows ? kRowBuf : kDirect;
+          info->row0 = row0;
+          if (!p.join_rows && !whole && pc.starts) a.cuts[blockIdx.x] = CutUnit{pc.R0, pc.rows, pc.kvh, pc.npieces};
         }
-        continue;
-      } else {
-      // a thread has one 16-byte column of every fourth row; (token, head) step along without divisions
-      constexpr int CPR = D / 8;  // chunks of 8 values per row
-      constexpr int RS = 64 / CPR, NIT = kM / RS;  // (one query tile)
-      const uint32_t c = gt % CPR, up_t = RS / a.G, up_g = RS % a.G;
-      uint32_t r = gt / CPR, tok = (pc.R0 + r) / a.G, g = (pc.R0 + r) % a.G;
-      auto step = [&]() {
-        r += RS;
-        tok += up_t;
-        g += up_g;
-        if (g >= a.G) {
-          g -= a.G;
-          ++tok;
+        if (p.join_rows && pc.starts) {
+          RowPieces *rp = (pc.own ? a.own_pieces : a.pre_pieces) + (uint64_t)pc.kvh * a.bv.T * a.G + pc.R0;
+          for (uint32_t r = gt; r < pc.rows; r += 64) {
+            const uint32_t R = pc.R0 + r;
+            rp[r] = RowPieces{whole ? row0 + R / a.G * a.H + pc.kvh * a.G + R % a.G : slot + r, pc.npieces, p.u.RU, 0};
+          }
         }
-      };
-      const uint32_t head0 = pc.kvh * a.G;
-#pragma unroll 1
-        for (int i0 = 0; i0 < NIT; i0 += 4) {
-          float x[4][8];
-          const uint32_t r0 = r;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[u][j] = 0.f;
-            if (r < pc.rows) {
-              const uint64_t off = ((uint64_t)tok * a.H + head0 + g) * D + c * 8;
-              if (a.q_f16) load_f16<8>(static_cast<const __half *>(a.q) + off, x[u]);
-              else load_f32<8>(static_cast<const float *>(a.q) + off, x[u]);
+        if constexpr (!LO) {
+          // f16 rows come by TMA as boxes of whole tokens' heads; tokens behind the unit's are other sequences'
+          // (or zeros) and the tile's last rows stay as they were: computed along, never written
+          loaded = piece + 1;
+          if (gt == 0) {
+            mbar_expect_tx(q_full, NQT * p.rpt * D * 2);
+            const int tok = (int)(pc.R0 / a.G), per = (int)(p.rpt / a.G);
+            for (int q = 0; q < NQT; ++q)
+              for (int cb = 0; cb < D / 64; ++cb)
+                tma_load_4d(smem + C::oQ + q * C::QT + cb * kM * 128, &tmQ, q_full, cb * 64, 0, (int)pc.kvh, tok + q * per);
+          }
+          continue;
+        } else {
+          // a thread has one 16-byte column of every fourth row; (token, head) step along without divisions
+          constexpr int CPR = D / 8;  // chunks of 8 values per row
+          constexpr int RS = 64 / CPR, NIT = kM / RS;  // (one query tile)
+          const uint32_t c = gt % CPR, up_t = RS / a.G, up_g = RS % a.G;
+          uint32_t r = gt / CPR, tok = (pc.R0 + r) / a.G, g = (pc.R0 + r) % a.G;
+          auto step = [&]() {
+            r += RS;
+            tok += up_t;
+            g += up_g;
+            if (g >= a.G) {
+              g -= a.G;
+              ++tok;
             }
-            step();
-          }
+          };
+          const uint32_t head0 = pc.kvh * a.G;
+#pragma unroll 1
+          for (int i0 = 0; i0 < NIT; i0 += 4) {
+            float x[4][8];
+            const uint32_t r0 = r;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint4 hi, lo;
-            split8(x[u], hi, lo);
-            const uint32_t rr = r0 + u * RS;
-            unsigned char *d = smem + C::oQ + sw_off<kM>(rr, c);
-            *reinterpret_cast<uint4 *>(d) = hi;
-            *reinterpret_cast<uint4 *>(d + C::QT) = lo;
+            for (int u = 0; u < 4; ++u) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) x[u][j] = 0.f;
+              if (r < pc.rows) {
+                const uint64_t off = ((uint64_t)tok * a.H + head0 + g) * D + c * 8;
+                if (a.q_f16) load_f16<8>(static_cast<const __half *>(a.q) + off, x[u]);
+                else load_f32<8>(static_cast<const float *>(a.q) + off, x[u]);
+              }
+              step();
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              uint4 hi, lo;
+              split8(x[u], hi, lo);
+              const uint32_t rr = r0 + u * RS;
+              unsigned char *d = smem + C::oQ + sw_off<kM>(rr, c);
+              *reinterpret_cast<uint4 *>(d) = hi;
+              *reinterpret_cast<uint4 *>(d + C::QT) = lo;
+            }
           }
         }
+        fence_async_smem();
+        mbar_arrive(q_full);
       }
-      fence_async_smem();
-      mbar_arrive(q_full);
+      if (!ok) {
+        *abort_flag = 1;
+        // no query tile may still be in flight when the block exits (otherwise q_free is behind it)
+        if (!LO && gt == 0 && loaded) mbar_wait(q_full, (loaded - 1) & 1);
+      }
     }
-    if (!ok) {
-      *abort_flag = 1;
-      // no query tile may still be in flight when the block exits (otherwise q_free is behind it)
-      if (!LO && gt == 0 && loaded) mbar_wait(q_full, (loaded - 1) & 1);
-    }
-  }
   } else if (warp < 12) {
     // ---------------- softmax (one row per thread) ----------------
     if constexpr (Q8) asm volatile("setmaxnreg.inc.sync.aligned.u32 128;" ::: "memory");
@@ -530,209 +530,213 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     const float sl2 = a.sl2;
     bool ok = true;
     if (t < C::NS) {
-    uint32_t sp = 0;           // next phase parity of s_full, one bit per slot of this stream
-    uint32_t nv = 0;           // this stream's PVs of the pieces before
-    for (uint32_t piece = 0;; ++piece) {
-      if (!mbar_wait_warp(q_full, piece & 1)) { ok = false; break; }
-      const TcInfo in = *info;
-      __syncwarp();
-      if (in.ntiles == 0) break;
-      if (lane == 0) mbar_arrive(info_free);
-      const uint32_t r = (NQT == 2 ? t * p.rpt : 0) + row;
-      const uint32_t R = in.R0 + min(r, in.rows - 1);
-      const int lim = min(in.lim_base + (int)(R / a.G), (int)in.len - 1);
-      if (a.gate && in.dest == kDirect && (NQT == 2 || t == 0)) {
-        // the gates of the row, to L2: the epilogue would wait for HBM
-        const float *g = a.gate + ((uint64_t)(R / a.G) * a.H + in.kvh * a.G + R % a.G) * D;
-#pragma unroll 1
-        for (int i = 0; i < D / 32; ++i) asm volatile("prefetch.global.L2 [%0];" ::"l"(g + 32 * i));
-      }
-      float m_used = kNegBig, l = 0.f;
-      const int step = NQT == 2 ? 1 : C::NS;
-      const int first = NQT == 2 ? 0 : t;
-      for (int j = first; j < (int)in.ntiles; j += step) {
-       const int jj = NQT == 2 ? j : j / C::NS;  // tile of this stream
-#pragma unroll 1
-       for (int h = 0; h < C::PARTS; ++h) {
-        const int g = jj * C::PARTS + h, part = g & 1;  // step of this stream, and where its scores lie
-        if (h == 0) {
-          const int u = C::PARTS == 2 ? 0 : part;
-          if (!mbar_wait_warp(&s_full[2 * t + u], (sp >> u) & 1)) { ok = false; break; }
-          sp ^= 1u << u;
-          tc_fence_after();
-        }
-        const uint32_t sbase = (tmem + (2 * t + part) * SW) | lane_off;
-        const int key0 = (int)(in.tile0 + j) * KT + h * SW;
-        const int nvalid = min(SW, max(0, lim - key0 + 1));
-        uint32_t x[SW / 32][32];  // the step's scores of the row: one TMEM wait
-#pragma unroll
-        for (int c = 0; c < SW / 32; ++c) tmem_ld32(sbase + c * 32, x[c]);
-        tmem_wait_ld();
-        if (nvalid < SW) {
-#pragma unroll
-          for (int c = 0; c < SW / 32; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c * 32 + i >= nvalid) x[c][i] = __float_as_uint(-INFINITY);
-        }
-        float mx8[8];  // eight independent chains
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mx8[k] = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < SW / 32; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const int k = (c * 16 + i / 2) & 7;
-            mx8[k] = fmax3(mx8[k], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
-          }
-        const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], fmaxf(mx8[5], fmaxf(mx8[6], mx8[7]))));
-        const float mt = mx * sl2;
-        // lazy rescale: the whole warp takes the TMEM round trip when any of its rows moved far; rows
-        // that did not use the factor 1.  The PV before must have completed.
-        // Phases of pv_done are only ever waited for before this tile's P is handed over (or, after the
-        // last one, by the wait below): the barrier cannot have moved on by two.
-        bool waited = g == 0;
-        const bool need = mt > m_used + kRescale;
-        if (__any_sync(0xffffffffu, need)) {
-          if (g > 0) {
-            if (!mbar_wait_warp(&pv_done[t], (nv + g - 1) & 1)) { ok = false; break; }
-            waited = true;
-            tc_fence_after();
-            const float f = need ? ex2_approx(m_used - mt) : 1.0f;
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(obase + c * 32, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st32(obase + c * 32, o);
-            }
-            l *= f;
-          }
-          if (need) m_used = mt;
-        }
-        const float mneg = kUp - m_used;
-        const uint64_t sl2x2 = pack2(sl2, sl2), mneg2 = pack2(mneg, mneg);
-        uint64_t sums[2] = {0, 0};
-#pragma unroll
-        for (int c = 0; c < SW / 32; ++c) {
-          uint32_t hi[16], lo[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 e = unpack2(fma2(pack2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1])), sl2x2, mneg2));
-            const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
-            const uint64_t pp = pack2(p0, p1);
-            sums[i & 1] = add2(sums[i & 1], pp);
-            hi[i] = pack_half2(p0, p1);
-            if constexpr (LO) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
-              lo[i] = pack_half2(p0 - f.x, p1 - f.y);
-            }
-          }
-          tmem_st16(sbase + c * 16, hi);
-          if constexpr (LO) tmem_st16(sbase + SW / 2 + c * 16, lo);
-        }
-        const float2 sum = unpack2(add2(sums[0], sums[1]));
-        l += sum.x + sum.y;
-        tmem_wait_st();
-        if (j + step >= (int)in.ntiles && h == C::PARTS - 1 && !waited && !mbar_wait_warp(&pv_done[t], (nv + g - 1) & 1)) { ok = false; break; }
-        tc_fence_before();
+      uint32_t sp = 0;           // next phase parity of s_full, one bit per slot of this stream
+      uint32_t nv = 0;           // this stream's PVs of the pieces before
+      for (uint32_t piece = 0;; ++piece) {
+        if (!mbar_wait_warp(q_full, piece & 1)) { ok = false; break; }
+        const TcInfo in = *info;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * t + part]);
-       }
-       if (!ok) break;
-      }
-      if (!ok) break;
-      // ---- the piece's rows ----
-      const int mine = NQT == 2 || C::NS == 1 ? (int)in.ntiles : ((int)in.ntiles + 1 - t) >> 1;  // this stream's tiles
-      const bool some = mine > 0;
-      if (some && !mbar_wait_warp(&pv_done[t], (nv + mine * C::PARTS - 1) & 1)) { ok = false; break; }
-      nv += mine * C::PARTS;
-      float f0 = 1.f, f1 = 0.f, M = m_used, L = l;
-      if constexpr (NQT == 1 && C::NS == 2) {
-        if (t == 1) {
-          // stream 0 still reads the last piece's (m, l) until it frees O
-          tc_fence_after();
-          if (piece > 0 && !mbar_wait_warp(&o_free[0], (piece - 1) & 1)) { ok = false; break; }
-          ml_s[row] = make_float2(m_used, some ? l : 0.f);
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(b_done);
-          continue;
-        }
-        if (!mbar_wait_warp(b_done, piece & 1)) { ok = false; break; }
-        // (stream 1 has seen its last PV done before it counted in)
-        const float2 ml = ml_s[row];
-        M = fmaxf(m_used, ml.x);
-        f0 = ex2_approx(m_used - M);
-        f1 = in.ntiles > 1 ? ex2_approx(ml.x - M) : 0.f;
-        L = l * f0 + ml.y * f1;
-      }
-      tc_fence_after();
-      const float inv = L != 0.f ? 1.0f / L : 0.f;  // a row that attends nothing is zero
-      const bool valid = (uint32_t)row < p.rpt && r < in.rows;
-      const uint64_t orow = (uint64_t)(R / a.G) * a.H + in.kvh * a.G + R % a.G;
-      const uint64_t prow = in.dest == kRowBuf ? in.row0 + orow : in.dest + r;
-      const bool gated = a.gate && in.dest == kDirect && valid;
-      const float4 *gate = reinterpret_cast<const float4 *>(a.gate + orow * D);
-      float4 gn[8];  // the next chunk's gate travels while a chunk is written
-      if (gated) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) gn[i] = __ldg(gate + i);
-      }
+        if (in.ntiles == 0) break;
+        if (lane == 0) mbar_arrive(info_free);
+        const uint32_t r = (NQT == 2 ? t * p.rpt : 0) + row;
+        const uint32_t R = in.R0 + min(r, in.rows - 1);
+        const int lim = min(in.lim_base + (int)(R / a.G), (int)in.len - 1);
+        if (a.gate && in.dest == kDirect && (NQT == 2 || t == 0)) {
+          // the gates of the row, to L2: the epilogue would wait for HBM
+          const float *g = a.gate + ((uint64_t)(R / a.G) * a.H + in.kvh * a.G + R % a.G) * D;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(obase + c * 32, o);
-        tmem_wait_ld();
-        if constexpr (NQT == 1 && C::NS == 2) {
-          if (in.ntiles > 1) {  // uniform: O_1 holds something
-            uint32_t o1[32];
-            tmem_ld32(((tmem + C::O1) | lane_off) + c * 32, o1);
+          for (int i = 0; i < D / 32; ++i) asm volatile("prefetch.global.L2 [%0];" ::"l"(g + 32 * i));
+        }
+        float m_used = kNegBig, l = 0.f;
+        const int step = NQT == 2 ? 1 : C::NS;
+        const int first = NQT == 2 ? 0 : t;
+        for (int j = first; j < (int)in.ntiles; j += step) {
+          const int jj = NQT == 2 ? j : j / C::NS;  // tile of this stream
+#pragma unroll 1
+          for (int h = 0; h < C::PARTS; ++h) {
+            const int g = jj * C::PARTS + h, part = g & 1;  // step of this stream, and where its scores lie
+            if (h == 0) {
+              const int u = C::PARTS == 2 ? 0 : part;
+              if (!mbar_wait_warp(&s_full[2 * t + u], (sp >> u) & 1)) { ok = false; break; }
+              sp ^= 1u << u;
+              tc_fence_after();
+            }
+            const uint32_t sbase = (tmem + (2 * t + part) * SW) | lane_off;
+            const int key0 = (int)(in.tile0 + j) * KT + h * SW;
+            const int nvalid = min(SW, max(0, lim - key0 + 1));
+            uint32_t x[SW / 32][32];  // the step's scores of the row: one TMEM wait
+#pragma unroll
+            for (int c = 0; c < SW / 32; ++c) tmem_ld32(sbase + c * 32, x[c]);
             tmem_wait_ld();
+            if (nvalid < SW) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(o1[i]) * f1);
-          } else {
+              for (int c = 0; c < SW / 32; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f0);
+                for (int i = 0; i < 32; ++i)
+                  if (c * 32 + i >= nvalid) x[c][i] = __float_as_uint(-INFINITY);
+            }
+            float mx8[8];  // eight independent chains
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mx8[k] = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < SW / 32; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const int k = (c * 16 + i / 2) & 7;
+                mx8[k] = fmax3(mx8[k], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+              }
+            const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]),
+                                   fmax3(mx8[3], mx8[4], fmaxf(mx8[5], fmaxf(mx8[6], mx8[7]))));
+            const float mt = mx * sl2;
+            // lazy rescale: the whole warp takes the TMEM round trip when any of its rows moved far; rows
+            // that did not use the factor 1.  The PV before must have completed.
+            // Phases of pv_done are only ever waited for before this tile's P is handed over (or, after the
+            // last one, by the wait below): the barrier cannot have moved on by two.
+            bool waited = g == 0;
+            const bool need = mt > m_used + kRescale;
+            if (__any_sync(0xffffffffu, need)) {
+              if (g > 0) {
+                if (!mbar_wait_warp(&pv_done[t], (nv + g - 1) & 1)) { ok = false; break; }
+                waited = true;
+                tc_fence_after();
+                const float f = need ? ex2_approx(m_used - mt) : 1.0f;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                  uint32_t o[32];
+                  tmem_ld32(obase + c * 32, o);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                  tmem_st32(obase + c * 32, o);
+                }
+                l *= f;
+              }
+              if (need) m_used = mt;
+            }
+            const float mneg = kUp - m_used;
+            const uint64_t sl2x2 = pack2(sl2, sl2), mneg2 = pack2(mneg, mneg);
+            uint64_t sums[2] = {0, 0};
+#pragma unroll
+            for (int c = 0; c < SW / 32; ++c) {
+              uint32_t hi[16], lo[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const uint64_t s2 = pack2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1]));
+                const float2 e = unpack2(fma2(s2, sl2x2, mneg2));
+                const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
+                const uint64_t pp = pack2(p0, p1);
+                sums[i & 1] = add2(sums[i & 1], pp);
+                hi[i] = pack_half2(p0, p1);
+                if constexpr (LO) {
+                  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
+                  lo[i] = pack_half2(p0 - f.x, p1 - f.y);
+                }
+              }
+              tmem_st16(sbase + c * 16, hi);
+              if constexpr (LO) tmem_st16(sbase + SW / 2 + c * 16, lo);
+            }
+            const float2 sum = unpack2(add2(sums[0], sums[1]));
+            l += sum.x + sum.y;
+            tmem_wait_st();
+            const bool last = j + step >= (int)in.ntiles && h == C::PARTS - 1;
+            if (last && !waited && !mbar_wait_warp(&pv_done[t], (nv + g - 1) & 1)) { ok = false; break; }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * t + part]);
           }
+          if (!ok) break;
         }
-        if (!valid) continue;
-        if (in.dest != kDirect) {
-          store_words<32>(a.part_o + prow * D + c * 32, o, p.wide);
-          continue;
+        if (!ok) break;
+        // ---- the piece's rows ----
+        const int mine = NQT == 2 || C::NS == 1 ? (int)in.ntiles : ((int)in.ntiles + 1 - t) >> 1;  // this stream's tiles
+        const bool some = mine > 0;
+        if (some && !mbar_wait_warp(&pv_done[t], (nv + mine * C::PARTS - 1) & 1)) { ok = false; break; }
+        nv += mine * C::PARTS;
+        float f0 = 1.f, f1 = 0.f, M = m_used, L = l;
+        if constexpr (NQT == 1 && C::NS == 2) {
+          if (t == 1) {
+            // stream 0 still reads the last piece's (m, l) until it frees O
+            tc_fence_after();
+            if (piece > 0 && !mbar_wait_warp(&o_free[0], (piece - 1) & 1)) { ok = false; break; }
+            ml_s[row] = make_float2(m_used, some ? l : 0.f);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_done);
+            continue;
+          }
+          if (!mbar_wait_warp(b_done, piece & 1)) { ok = false; break; }
+          // (stream 1 has seen its last PV done before it counted in)
+          const float2 ml = ml_s[row];
+          M = fmaxf(m_used, ml.x);
+          f0 = ex2_approx(m_used - M);
+          f1 = in.ntiles > 1 ? ex2_approx(ml.x - M) : 0.f;
+          L = l * f0 + ml.y * f1;
         }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+        tc_fence_after();
+        const float inv = L != 0.f ? 1.0f / L : 0.f;  // a row that attends nothing is zero
+        const bool valid = (uint32_t)row < p.rpt && r < in.rows;
+        const uint64_t orow = (uint64_t)(R / a.G) * a.H + in.kvh * a.G + R % a.G;
+        const uint64_t prow = in.dest == kRowBuf ? in.row0 + orow : in.dest + r;
+        const bool gated = a.gate && in.dest == kDirect && valid;
+        const float4 *gate = reinterpret_cast<const float4 *>(a.gate + orow * D);
+        float4 gn[8];  // the next chunk's gate travels while a chunk is written
         if (gated) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) * sigmoid(gn[i].x));
-            o[4 * i + 1] = __float_as_uint(__uint_as_float(o[4 * i + 1]) * sigmoid(gn[i].y));
-            o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) * sigmoid(gn[i].z));
-            o[4 * i + 3] = __float_as_uint(__uint_as_float(o[4 * i + 3]) * sigmoid(gn[i].w));
-          }
-          if (c + 1 < D / 32) {
+          for (int i = 0; i < 8; ++i) gn[i] = __ldg(gate + i);
+        }
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld32(obase + c * 32, o);
+          tmem_wait_ld();
+          if constexpr (NQT == 1 && C::NS == 2) {
+            if (in.ntiles > 1) {  // uniform: O_1 holds something
+              uint32_t o1[32];
+              tmem_ld32(((tmem + C::O1) | lane_off) + c * 32, o1);
+              tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) gn[i] = __ldg(gate + 8 * (c + 1) + i);
+              for (int i = 0; i < 32; ++i)
+                o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + __uint_as_float(o1[i]) * f1);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f0);
+            }
+          }
+          if (!valid) continue;
+          if (in.dest != kDirect) {
+            store_words<32>(a.part_o + prow * D + c * 32, o, p.wide);
+            continue;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+          if (gated) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) * sigmoid(gn[i].x));
+              o[4 * i + 1] = __float_as_uint(__uint_as_float(o[4 * i + 1]) * sigmoid(gn[i].y));
+              o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) * sigmoid(gn[i].z));
+              o[4 * i + 3] = __float_as_uint(__uint_as_float(o[4 * i + 3]) * sigmoid(gn[i].w));
+            }
+            if (c + 1 < D / 32) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) gn[i] = __ldg(gate + 8 * (c + 1) + i);
+            }
+          }
+          if (a.out_f16) {
+            uint32_t h[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) h[i] = pack_half2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+            store_words<16>(static_cast<__half *>(a.out) + orow * D + c * 32, h, p.wide);
+          } else {
+            store_words<32>(static_cast<float *>(a.out) + orow * D + c * 32, o, p.wide);
           }
         }
-        if (a.out_f16) {
-          uint32_t h[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) h[i] = pack_half2(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
-          store_words<16>(static_cast<__half *>(a.out) + orow * D + c * 32, h, p.wide);
-        } else {
-          store_words<32>(static_cast<float *>(a.out) + orow * D + c * 32, o, p.wide);
-        }
+        if (valid && in.dest != kDirect) a.part_ml[prow] = make_float2(M - kUp, L);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&o_free[NQT == 2 ? t : 0]);
       }
-      if (valid && in.dest != kDirect) a.part_ml[prow] = make_float2(M - kUp, L);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&o_free[NQT == 2 ? t : 0]);
-    }
     }
     if (!ok) *abort_flag = 1;
   } else {
@@ -842,7 +846,8 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_lo, bool p
     const uint64_t dims[4] = {D, a.G, a.kv.KV, a.bv.T};
     const uint64_t strides[3] = {D * 2, (uint64_t)a.G * D * 2, (uint64_t)a.H * D * 2};
     const uint32_t box[4] = {64, a.G, 1, p.rpt / a.G};
-    if (make_tmap_4d(&tq, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return BG_EUNSUPPORTED;
+    if (make_tmap_4d(&tq, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
+      return BG_EUNSUPPORTED;
   }
   if (!Q8) {
     const uint64_t rb = (uint64_t)D * 2;
@@ -874,8 +879,7 @@ int launch_q(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows
   const bool lo = !(a.q_f16 && a.out_f16);
   if (a.D == 256) {
     if (!lo) return launch_cfg<256, Q8, false, 1>(a, blocks, rows_lo, prefix, st);
-    if constexpr (!Q8) return launch_cfg<256, false, true, 1>(a, blocks, rows_lo, prefix, st);
-    return BG_EUNSUPPORTED;
+    return launch_cfg<256, Q8, true, 1>(a, blocks, rows_lo, prefix, st);
   }
   if (lo) return launch_cfg<128, Q8, true, 1>(a, blocks, rows_lo, prefix, st);
   return ru > kM ? launch_cfg<128, Q8, false, 2>(a, blocks, rows_lo, prefix, st)
@@ -884,12 +888,9 @@ int launch_q(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows
 
 }  // namespace
 
-// Page boxes of at least 8 positions keep the 128-byte swizzle's pattern.  head_dim 256 with all four halves
-// (f32 rows over a q8 pool) does not fit shared memory.
-bool paged_tc_supported(int mode, uint32_t D, uint32_t G, uint32_t page_size, bool lo) {
-  return G <= kM && page_size % 8 == 0 &&
-         (D == 128 ? mode == BG_KV_F16 || mode == BG_KV_Q8
-                   : D == 256 && (mode == BG_KV_F16 || (mode == BG_KV_Q8 && !lo)));
+// Page boxes of at least 8 positions keep the 128-byte swizzle's pattern.
+bool paged_tc_supported(int mode, uint32_t D, uint32_t G, uint32_t page_size) {
+  return G <= kM && page_size % 8 == 0 && (D == 128 || D == 256) && (mode == BG_KV_F16 || mode == BG_KV_Q8);
 }
 
 // Rows of a unit: whole tokens' heads, two query tiles where there are rows for them and memory for both (f16
