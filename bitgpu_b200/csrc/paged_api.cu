@@ -184,6 +184,7 @@ int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, ui
                        void *workspace, size_t workspace_bytes, bg_stream_t stream) {
   if (int rc = check_paged(kv, batch, KV, D)) return rc;
   if (H == 0 || H % KV || q_dtype > BG_DT_F16 || out_dtype > BG_DT_F16) return BG_EINVAL;
+  if (!(scale >= 0.f && scale < INFINITY)) return BG_EINVAL;
   if (batch->batch == 0 || batch->tokens == 0) return BG_OK;
   if (!q || !out || !aligned16(q) || !aligned16(out) || !aligned16(gate) || !aligned16(workspace)) return BG_EINVAL;
   const Plan plan = make_plan(kv, batch, H, KV, D, !generic_forced(), !(q_dtype == BG_DT_F16 && out_dtype == BG_DT_F16));

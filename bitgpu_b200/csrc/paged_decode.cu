@@ -16,9 +16,10 @@
 //     B operand in registers through movmatrix;
 //   * f32 rows (LO): q and p are split into two f16 operands (22 bits).  Up to four rows a unit (PK; one
 //     token of a group of four heads) the halves share one product, hi in columns 0-3 and lo in 4-7 of the
-//     MMA's eight; otherwise both products run twice.  f16 rows: q is exact and p is rounded once to f16, which costs about as much as the rounding of
-//     the result.  p carries a factor 2^14 (q8: 2^6, since V's block scale is folded into p), which
-//     cancels in the quotient and keeps small weights out of f16's subnormals;
+//     MMA's eight; otherwise both products run twice.  f16 rows: q is exact and p is rounded once to f16,
+//     which costs about as much as the rounding of the result.  p carries a factor 2^14 (q8: 2^6, since
+//     V's block scale is folded into p), which cancels in the quotient and keeps small weights out of
+//     f16's subnormals;
 //   * q8 codes enter the products as exact f16 integers: byte + 128 under the f16 pattern 0x64xx is
 //     1152 + code, and one packed subtraction leaves the code.  (Cancelling the 1152 inside the MMA
 //     instead costs accuracy: the f32 accumulator then holds sums 1152 / |code| times as large.)
@@ -37,7 +38,8 @@ constexpr int kTile = 64;    // positions per tile
 constexpr int kConsumers = 4;
 constexpr int kThreads = 32 * (kConsumers + 1);
 constexpr int kUnits = 2;    // staged units
-constexpr int kLead = 1;     // tiles' time that a unit costs beside its tiles (64 short own parts: 0 55.8 us a call, 1 52.1, 2 52.1)
+// tiles' time that a unit costs beside its tiles (64 short own parts: 0 55.8 us a call, 1 52.1, 2 52.1)
+constexpr int kLead = 1;
 
 struct DecodeParams {
   PagedAttnArgs a;

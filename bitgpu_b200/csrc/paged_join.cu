@@ -23,8 +23,8 @@ __global__ void __launch_bounds__(128) join_cuts_kernel(PagedAttnArgs a, uint32_
   const uint64_t off = ((uint64_t)t * a.H + c.kvh * a.G + R % a.G) * D;
   const uint32_t idx0 = a.slot0 + (2 * blockIdx.x + 1) * ru + r;
   join_row_block<D, kWarps>(
-      a.part_o, a.part_ml, min(c.npieces, gridDim.x - blockIdx.x), [&](uint32_t k) { return (uint64_t)piece_index(idx0, ru, k); }, sm, a.out, a.out_f16,
-      a.gate, off);
+      a.part_o, a.part_ml, min(c.npieces, gridDim.x - blockIdx.x),
+      [&](uint32_t k) { return (uint64_t)piece_index(idx0, ru, k); }, sm, a.out, a.out_f16, a.gate, off);
 }
 
 // The same for units of many rows and few pieces (tcgen05 kernel): one warp per row.

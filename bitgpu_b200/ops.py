@@ -528,7 +528,8 @@ def paged_attention(q, cache, batch, scale=0.0, gate=None, out_dtype=torch.float
     """Causal GQA attention of ``q[tokens, H, D]`` (f32 or f16) over a paged cache: the token at own
     position ``o`` of its sequence attends the batch's shared prefix and own positions ``0 .. o``.
     ``scale`` 0 means ``1/sqrt(D)``; ``gate[tokens, H, D]`` (f32) applies the sigmoid output gate.
-    Returns ``out[tokens, H, D]``; rows behind the last sequence are not written."""
+    Returns ``out[tokens, H, D]`` (which may be ``q`` itself); rows behind the last sequence are not
+    written."""
     _need(q, name="q")
     if q.dtype not in _DT:
         raise ValueError(f"q must be float32 or float16, got {q.dtype}")

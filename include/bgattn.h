@@ -258,9 +258,10 @@ int bg_paged_append(const bg_paged_cache *kv, const bg_paged_batch *batch, uint3
                     uint32_t table_rows, void *q_out, uint32_t q_out_dtype, bg_stream_t stream);
 
 /* bg_paged_attention: causal GQA attention of q [tokens][H][D] over the paged cache; the token at own
- * position o attends the whole prefix and own positions 0 .. o.  scale == 0 selects 1/sqrt(D); gate
- * [tokens][H][D] f32 or NULL as in bg_attention; out [tokens][H][D].  The shared prefix is read once
- * for all rows of the batch and joined with each sequence's own part by their log-sum-exp.
+ * position o attends the whole prefix and own positions 0 .. o.  scale == 0 selects 1/sqrt(D), a negative one
+ * is refused; gate [tokens][H][D] f32 or NULL as in bg_attention; out [tokens][H][D], which may be q
+ * itself (q_dtype == out_dtype).  The shared prefix is read once for all rows of the batch and joined with
+ * each sequence's own part by their log-sum-exp.
  * workspace: bg_paged_attention_workspace_size bytes, 16-byte aligned, of any content; calls that may
  * overlap on the GPU need one each. */
 size_t bg_paged_attention_workspace_size(const bg_paged_cache *kv, const bg_paged_batch *batch, uint32_t H, uint32_t KV,

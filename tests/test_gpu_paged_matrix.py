@@ -172,3 +172,80 @@ def test_same_bits_twice(ops, mode, io):  # noqa: F811
     a = ops.paged_attention(q, cache, b, out_dtype=DT[io])
     for _ in range(5):
         assert torch.equal(a, ops.paged_attention(q, cache, b, out_dtype=DT[io]))
+
+
+@pytest.mark.parametrize("mode,io", KINDS)
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("room", [64, 1 << 18])
+def test_output_in_place(ops, mode, io, D, room):  # noqa: F811
+    """out may be q, whichever kernels run."""
+    for prefix in (0, 1500):
+        r = wide(Ragged([300, 20, 90], [60, 1, 30], KV=4, G=6, D=D, mode=mode, prefix=prefix, page=64, seed=9),
+                 max(room, 384))
+        q = r.queries(DT[io]).cuda()
+        cache, b = r.cache(ops), r.batch(ops)
+        want = ops.paged_attention(q, cache, b, out_dtype=DT[io])
+        assert torch.equal(ops.paged_attention(q, cache, b, out=q), want)
+
+
+@pytest.mark.parametrize("mode,io", KINDS)
+@pytest.mark.parametrize("room", [320, 1 << 18])
+@pytest.mark.parametrize("news", [[1, 1], [60, 30]])
+def test_shut_and_open_gates(ops, mode, io, room, news):  # noqa: F811
+    r = wide(Ragged([300, 90], news, mode=mode, seed=9), room)
+    q = r.queries(DT[io]).cuda()
+    cache, b = r.cache(ops), r.batch(ops)
+    want = ops.paged_attention(q, cache, b, out_dtype=DT[io])
+    inf = torch.full(q.shape, float("inf"), device="cuda")
+    assert torch.equal(ops.paged_attention(q, cache, b, gate=inf, out_dtype=DT[io]), want)
+    assert not ops.paged_attention(q, cache, b, gate=-inf, out_dtype=DT[io]).any()
+
+
+@pytest.mark.parametrize("mode", ["f32", "f16", "q8"])
+def test_many_sequences(ops, mode):  # noqa: F811
+    """Thousands of short sequences, a few of them without a token."""
+    B = 5000
+    lens = [i * 7 % 19 + 1 for i in range(B)]
+    news = [0 if i % 97 == 5 else min(lens[i], i % 2 + 1) for i in range(B)]
+    run(ops, Ragged(lens, news, KV=1, G=2, D=128, page=8, mode=mode, seed=5))
+
+
+@pytest.mark.parametrize("mode,D,pages", [("f16", 128, 66000), ("q8", 128, 66000), ("q8", 256, 33000), ("f32", 64, 40000)])
+@pytest.mark.parametrize("room", [640, 1 << 18])
+def test_far_pages(ops, mode, D, pages, room):  # noqa: F811
+    """Pages behind the first 2^32 values (f32: bytes) of a pool: the bits of a small pool, appended and read."""
+    KV, G, page, n = 8, 4, 64, 20
+    far = ops.PagedKVCache.from_tensors(*[
+        torch.empty((pages, page, KV, w), dtype=dt, device="cuda")
+        for dt, w in [({"f16": torch.float16, "q8": torch.int8, "f32": torch.float32}[mode], D)] * 2
+        + [(torch.float32, D // 32)] * 2 * (mode == "q8")])
+    near = ops.PagedKVCache(n, page, KV, D, mode)
+    torch.manual_seed(1)
+    lens, news = [500, 70, 129], [100, 1, 129]
+    T = sum(news)
+    table = torch.zeros(3, room // page, dtype=torch.int32, device="cuda")
+    table[:, :6] = torch.randperm(18)[:18].view(3, 6).int().cuda()
+    table[0, 6:8] = torch.tensor([18, 19], dtype=torch.int32)
+    qkv = torch.randn(T, (G + 2) * KV, D, device="cuda")
+    H = G * KV
+    out = []
+    for cache, first in ((near, 0), (far, pages - n)):
+        args = (table + first, torch.tensor(lens).int().cuda())
+        cu = torch.tensor([0, 100, 101, T]).int().cuda()
+        if first:  # the positions before the new tokens
+            for x in ("K", "V") + ("Ks", "Vs") * (mode == "q8"):
+                getattr(far, x)[first:] = before[x]
+        else:
+            near.K.copy_(torch.randn(near.K.shape, device="cuda") * 20)
+            near.V.copy_(torch.randn(near.V.shape, device="cuda") * 20)
+            if mode == "q8":
+                near.Ks.uniform_(0.5, 1.5)
+                near.Vs.uniform_(0.5, 1.5)
+            before = {x: getattr(near, x).clone() for x in ("K", "V") + ("Ks", "Vs") * (mode == "q8")}
+        b = ops.PagedBatch(*args, cu, T, max(news))
+        ops.paged_append(cache, b, qkv[:, H:H + KV], qkv[:, H + KV:])
+        out.append(ops.paged_attention(qkv[:, :H].contiguous(), cache, b))
+    for x in ("K", "V") + ("Ks", "Vs") * (mode == "q8"):
+        assert torch.equal(getattr(far, x)[pages - n:], getattr(near, x)), x
+        assert not torch.equal(getattr(near, x), before[x])
+    assert torch.isfinite(out[0]).all() and torch.equal(out[0], out[1])

@@ -122,3 +122,9 @@ def test_find_seq_search():
         for t in list(range(0, cu[-1] + 2, max(1, cu[-1] // 50))) + [cu[-1] - 1, cu[-1]]:
             want = max((b for b in range(B) if cu[b] <= t), default=-1) if t < cu[-1] else -1
             assert find(cu, t) == want or t < 0, (B, t)
+
+
+@pytest.mark.parametrize("scale", [-0.1, float("nan"), float("inf"), -float("inf")])
+def test_scale_refusals(scale):
+    assert lib().bg_paged_attention(C.byref(cache()), C.byref(batch()), 8, 2, 128, A, 0, scale, None, A, 0, A, 1 << 30,
+                                    None) == BG_EINVAL
