@@ -679,8 +679,11 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         const uint64_t prow = in.dest == kRowBuf ? in.row0 + orow : in.dest + r;
         const bool gated = a.gate && in.dest == kDirect && valid;
         const float4 *gate = reinterpret_cast<const float4 *>(a.gate + orow * D);
-        float4 gn[8];  // the next chunk's gate travels while a chunk is written
-        if (gated) {
+        // the next chunk's gate travels while a chunk is written, where there are registers for it (otherwise
+        // 128 streams behind 32768 shared q8 positions, without any gate, take 211 us for 208)
+        constexpr bool AHEAD_GATE = !Q8 || (D == 256 && !LO);
+        float4 gn[8];
+        if (AHEAD_GATE && gated) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) gn[i] = __ldg(gate + i);
         }
@@ -711,6 +714,10 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
           if (gated) {
+            if (!AHEAD_GATE) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) gn[i] = __ldg(gate + 8 * c + i);
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               o[4 * i] = __float_as_uint(__uint_as_float(o[4 * i]) * sigmoid(gn[i].x));
@@ -718,7 +725,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
               o[4 * i + 2] = __float_as_uint(__uint_as_float(o[4 * i + 2]) * sigmoid(gn[i].z));
               o[4 * i + 3] = __float_as_uint(__uint_as_float(o[4 * i + 3]) * sigmoid(gn[i].w));
             }
-            if (c + 1 < D / 32) {
+            if (AHEAD_GATE && c + 1 < D / 32) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) gn[i] = __ldg(gate + 8 * (c + 1) + i);
             }
