@@ -347,34 +347,32 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         auto stage = [&](int i) { return (it + i) % C::NST; };
         auto wait_k = [&](int i) { return mbar_wait_warp(&k_full[stage(i)], ((it + i) / C::NST) & 1); };
         auto wait_v = [&](int i) { return mbar_wait_warp(&v_full[stage(i)], ((it + i) / C::NST) & 1); };
-        // S of stream t, tile i; the last reader of K_i frees it, the last S of the piece frees Q
+        // (one lane) S of stream t, tile i; the last reader of K_i frees it, the last S of the piece frees Q
         auto send_s = [&](int t, int u, int i) {
-          tc_fence_after();
-          if (elect_one()) {
-            issue_s(t, u, stage(i));
-            umma_commit(&s_full[2 * t + u]);
-            if (NQT == 1 || t == 1) {
-              umma_commit(&k_empty[stage(i)]);
-              if (i + 1 == n) umma_commit(q_free);
-            }
+          issue_s(t, u, stage(i));
+          umma_commit(&s_full[2 * t + u]);
+          if (NQT == 1 || t == 1) {
+            umma_commit(&k_empty[stage(i)]);
+            if (i + 1 == n) umma_commit(q_free);
           }
-          __syncwarp();
         };
         for (int i = 0; ok && i < AHEAD && i < n; ++i) {
           ok = wait_k(i);
           if (!ok) break;
           const int u = (i / STEP) % C::SLOTS;
-          if (NQT == 2) {
-            send_s(0, u, i);
-            send_s(1, u, i);
-          } else {
-            send_s(C::NS == 2 ? i & 1 : 0, u, i);
+          tc_fence_after();
+          if (elect_one()) {
+            send_s(NQT == 1 && C::NS == 2 ? i & 1 : 0, u, i);
+            if (NQT == 2) send_s(1, u, i);
           }
+          __syncwarp();
         }
         // the PVs of stream t, tile i, and behind them the S that takes over its columns: in-order execution
-        // keeps P safe
+        // keeps P safe.  The ring's waits come before P's, under the softmax: K(i + AHEAD) and V(i) only need what
+        // earlier steps issued.
         auto step = [&](int t, int i, int u) {
-          if (NQT == 1 || t == 0) ok = wait_v(i);
+          const bool more = i + AHEAD < n;
+          if (NQT == 1 || t == 0) ok = wait_v(i) && (!more || wait_k(i + AHEAD));
           if (ok && i < STEP && piece > 0) ok = mbar_wait_warp(&o_free[NQT == 2 ? t : 0], (piece - 1) & 1);
 #pragma unroll
           for (int h = 0; h < C::PARTS; ++h) {
@@ -386,14 +384,12 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
             if (elect_one()) {
               issue_pv(t, x, stage(i), h, i >= STEP || h > 0);
               umma_commit(&pv_done[t]);
-              if (h == C::PARTS - 1 && (NQT == 1 || t == 1)) umma_commit(&v_empty[stage(i)]);
+              if (h == C::PARTS - 1) {
+                if (NQT == 1 || t == 1) umma_commit(&v_empty[stage(i)]);
+                if (more) send_s(t, ((i + AHEAD) / STEP) % C::SLOTS, i + AHEAD);
+              }
             }
             __syncwarp();
-          }
-          if (i + AHEAD < n) {
-            // (only now: the ring may not hold this K before V(i) has been used)
-            if (NQT == 1 || t == 0) ok = wait_k(i + AHEAD);
-            if (ok) send_s(t, ((i + AHEAD) / STEP) % C::SLOTS, i + AHEAD);
           }
         };
         for (int i = 0; ok && i < n; ++i) {
