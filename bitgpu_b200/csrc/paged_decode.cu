@@ -672,8 +672,9 @@ int launch_md(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t row
   if (ru == 8)
     return lo ? launch_cfg<MODE, D, 1, true>(a, blocks, rows_hi, prefix, st)
               : launch_cfg<MODE, D, 1, false>(a, blocks, rows_hi, prefix, st);
-  return lo ? launch_cfg<MODE, D, 2, true>(a, blocks, rows_hi, prefix, st)
-            : launch_cfg<MODE, D, 2, false>(a, blocks, rows_hi, prefix, st);
+  if constexpr (D == 128)  // f32 rows of head_dim 256 come in units of 8
+    if (lo) return launch_cfg<MODE, D, 2, true>(a, blocks, rows_hi, prefix, st);
+  return launch_cfg<MODE, D, 2, false>(a, blocks, rows_hi, prefix, st);
 }
 
 }  // namespace
