@@ -351,6 +351,7 @@ struct PagedAttnArgs {
   uint32_t H, G, D, max_q;
   float sl2;  // softmax scale * log2(e)
   const void *q;
+  void *q_halves;  // tcgen05 kernels, rows that are not f16 in and out: q as two f16 halves [2][T][H][D]
   const float *gate;
   void *out;
   // partial rows: o [n][D] unnormalised, ml [n] (running max in log2 units, sum); n = part_rows
@@ -378,6 +379,7 @@ int launch_paged_decode(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, ui
 // tcgen05 kernel: many rows a sequence (own part), or the rows of the batch against the shared prefix.
 bool paged_tc_supported(int mode, uint32_t D, uint32_t G, uint32_t page_size);
 uint32_t paged_tc_rows(uint32_t D, uint32_t G, bool lo, uint64_t rows);
+int launch_paged_split_rows(const PagedAttnArgs &a, cudaStream_t st);
 int launch_paged_tc(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_lo, bool prefix, cudaStream_t st);
 // Join the cut units of `blocks` blocks of ru rows (no prefix), or every row's pieces (prefix).
 int launch_paged_join_cuts(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, cudaStream_t st);

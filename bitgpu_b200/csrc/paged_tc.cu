@@ -25,7 +25,7 @@
 //           and not the tensor pipe set the pace of the single-product form.)
 //
 // Warp roles: warp 0 TMA producer of K and V (f16 pool; page boxes, 128-byte swizzle), warp 1 MMA issuer,
-// warps 2-3 bring the next unit's query rows as soon as the last S of the current one is done, warps 4-11
+// warps 2-3 ask for the next unit's query rows as soon as the last S of the current one is done, warps 4-11
 // softmax (one row per thread), warps 12-15 and 16-19 (q8 pool) dequantise K and V, a tile ahead in registers.
 // All waits are bounded; on expiry the block records BG_ETIMEOUT, stops issuing, waits for what it issued,
 // frees its TMEM and exits.
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       mbar_init(&pv_done[i], 1);
       mbar_init(&o_free[i], 4);
     }
-    mbar_init(q_full, LO ? 64 : 1);
+    mbar_init(q_full, 1);
     mbar_init(q_free, 1);
     mbar_init(mma_done, 1);
     mbar_init(info_free, 4 * C::NS);
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         }
         if (!more) {
           if (gt == 0) info->ntiles = 0;
-          if (LO || gt == 0) mbar_arrive(q_full);
+          if (gt == 0) mbar_arrive(q_full);
           break;
         }
         const bool whole = pc.npieces == 1;
@@ -452,67 +452,22 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
             rp[r] = RowPieces{whole ? row0 + R / a.G * a.H + pc.kvh * a.G + R % a.G : slot + r, pc.npieces, p.u.RU, 0};
           }
         }
-        if constexpr (!LO) {
-          // f16 rows come by TMA as boxes of whole tokens' heads; tokens behind the unit's are other sequences'
-          // (or zeros) and the tile's last rows stay as they were: computed along, never written
-          loaded = piece + 1;
-          if (gt == 0) {
-            mbar_expect_tx(q_full, NQT * p.rpt * D * 2);
-            const int tok = (int)(pc.R0 / a.G), per = (int)(p.rpt / a.G);
-            for (int q = 0; q < NQT; ++q)
-              for (int cb = 0; cb < D / 64; ++cb)
-                tma_load_4d(smem + C::oQ + q * C::QT + cb * kM * 128, &tmQ, q_full, cb * 64, 0, (int)pc.kvh, tok + q * per);
-          }
-          continue;
-        } else {
-          // a thread has one 16-byte column of every fourth row; (token, head) step along without divisions
-          constexpr int CPR = D / 8;  // chunks of 8 values per row
-          constexpr int RS = 64 / CPR, NIT = kM / RS;  // (one query tile)
-          const uint32_t c = gt % CPR, up_t = RS / a.G, up_g = RS % a.G;
-          uint32_t r = gt / CPR, tok = (pc.R0 + r) / a.G, g = (pc.R0 + r) % a.G;
-          auto step = [&]() {
-            r += RS;
-            tok += up_t;
-            g += up_g;
-            if (g >= a.G) {
-              g -= a.G;
-              ++tok;
-            }
-          };
-          const uint32_t head0 = pc.kvh * a.G;
-#pragma unroll 1
-          for (int i0 = 0; i0 < NIT; i0 += 4) {
-            float x[4][8];
-            const uint32_t r0 = r;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) x[u][j] = 0.f;
-              if (r < pc.rows) {
-                const uint64_t off = ((uint64_t)tok * a.H + head0 + g) * D + c * 8;
-                if (a.q_f16) load_f16<8>(static_cast<const __half *>(a.q) + off, x[u]);
-                else load_f32<8>(static_cast<const float *>(a.q) + off, x[u]);
-              }
-              step();
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              uint4 hi, lo;
-              split8(x[u], hi, lo);
-              const uint32_t rr = r0 + u * RS;
-              unsigned char *d = smem + C::oQ + sw_off<kM>(rr, c);
-              *reinterpret_cast<uint4 *>(d) = hi;
-              *reinterpret_cast<uint4 *>(d + C::QT) = lo;
-            }
-          }
+        // rows come by TMA as boxes of whole tokens' heads; tokens behind the unit's are other sequences' (or
+        // zeros) and the tile's last rows stay as they were: computed along, never written
+        loaded = piece + 1;
+        if (gt == 0) {
+          mbar_expect_tx(q_full, NQT * C::NQ * p.rpt * D * 2);
+          const int tok = (int)(pc.R0 / a.G), per = (int)(p.rpt / a.G);
+          for (int q = 0; q < NQT * C::NQ; ++q)
+            for (int cb = 0; cb < D / 64; ++cb)
+              tma_load_4d(smem + C::oQ + q * C::QT + cb * kM * 128, &tmQ, q_full, cb * 64, 0, (int)pc.kvh,
+                          LO ? tok + q * (int)a.bv.T : tok + q * per);
         }
-        fence_async_smem();
-        mbar_arrive(q_full);
       }
       if (!ok) {
         *abort_flag = 1;
         // no query tile may still be in flight when the block exits (otherwise q_free is behind it)
-        if (!LO && gt == 0 && loaded) mbar_wait(q_full, (loaded - 1) & 1);
+        if (gt == 0 && loaded) mbar_wait(q_full, (loaded - 1) & 1);
       }
     }
   } else if (warp < 12) {
@@ -828,6 +783,23 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
+// Rows of f32 (or, beside an f32 result, f16) as two f16 halves, high ones first.  n: values / 8.
+// One pass for all kv heads' units, which then fetch their tiles by TMA: loaded and split by two warps of
+// the attention kernel, a unit's rows took 8 us at head_dim 128.
+__global__ void __launch_bounds__(256) split_rows_kernel(const void *q, int q_f16, uint4 *halves, uint64_t n) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const uint64_t step = (uint64_t)gridDim.x * 256;
+  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += step) {
+    float x[8];
+    if (q_f16) load_f16<8>(static_cast<const __half *>(q) + i * 8, x);
+    else load_f32<8>(static_cast<const float *>(q) + i * 8, x);
+    uint4 hi, lo;
+    split8(x, hi, lo);
+    halves[i] = hi;
+    halves[n + i] = lo;
+  }
+}
+
 template <int D, bool Q8, bool LO, int NQT>
 int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_lo, bool prefix, cudaStream_t st) {
   using C = TcCfg<D, Q8, LO, NQT>;
@@ -845,13 +817,13 @@ int launch_cfg(const PagedAttnArgs &a, uint32_t blocks, uint32_t rows_lo, bool p
   p.join_rows = a.own_pieces != nullptr;
   CUtensorMap tk = {}, tv = {}, tq = {};
   p.wide = (((uintptr_t)a.out | (uintptr_t)a.part_o) & 31) == 0;
-  if (!LO) {
-    const uint64_t dims[4] = {D, a.G, a.kv.KV, a.bv.T};
-    const uint64_t strides[3] = {D * 2, (uint64_t)a.G * D * 2, (uint64_t)a.H * D * 2};
-    const uint32_t box[4] = {64, a.G, 1, p.rpt / a.G};
-    if (make_tmap_4d(&tq, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B))
-      return BG_EUNSUPPORTED;
-  }
+  // f32 rows: the halves that split_rows_kernel left, the low ones T tokens behind the high ones
+  const uint64_t qdims[4] = {D, a.G, a.kv.KV, (uint64_t)C::NQ * a.bv.T};
+  const uint64_t qstrides[3] = {D * 2, (uint64_t)a.G * D * 2, (uint64_t)a.H * D * 2};
+  const uint32_t qbox[4] = {64, a.G, 1, p.rpt / a.G};
+  if (make_tmap_4d(&tq, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, LO ? a.q_halves : a.q, qdims, qstrides, qbox,
+                   CU_TENSOR_MAP_SWIZZLE_128B))
+    return BG_EUNSUPPORTED;
   if (!Q8) {
     const uint64_t rb = (uint64_t)D * 2;
     const uint64_t dims[4] = {D, a.kv.KV, ps, a.kv.num_pages};
@@ -901,6 +873,22 @@ bool paged_tc_supported(int mode, uint32_t D, uint32_t G, uint32_t page_size) {
 uint32_t paged_tc_rows(uint32_t D, uint32_t G, bool lo, uint64_t rows) {
   const uint32_t tile = kM / G * G;
   return D == 128 && !lo && rows > tile ? 2 * tile : tile;
+}
+
+int launch_paged_split_rows(const PagedAttnArgs &a, cudaStream_t st) {
+  const uint64_t n = (uint64_t)a.bv.T * a.H * a.D / 8, blocks = (n + 255) / 256;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((uint32_t)(blocks < 148 * 8 ? blocks : 148 * 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, split_rows_kernel, a.q, a.q_f16, static_cast<uint4 *>(a.q_halves), n) == cudaSuccess
+             ? BG_OK
+             : BG_ELAUNCH;
 }
 
 int launch_paged_tc(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_lo, bool prefix, cudaStream_t st) {
