@@ -85,7 +85,7 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
   const uint64_t pre_tiles = (all + 15) / 16 * KV * ((uint64_t)(b->prefix_len + 63) / 64);
   const uint64_t many = kManyTiles * paged_decode_blocks((int)kv->mode, D, 16);
   // f32 rows over a q8 pool of head_dim 256 have a ring of one stage: 36 rows a sequence behind 953 positions take
-  // 160 us there and 138 with the decode kernel, 60 behind 13388 shared ones 78 and 104
+  // 154 us there and 137 with the decode kernel, 60 behind 13388 shared ones 74 and 104
   const uint64_t few = lo && D == 256 && kv->mode == BG_KV_Q8 ? 48 : 16;
   p.tc_own = tc && group > few && own_tiles > many;
   p.tc_pre = tc && p.join && all > few && pre_tiles > many;
