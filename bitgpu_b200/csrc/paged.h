@@ -344,6 +344,8 @@ struct PagedAppendArgs {
   void *q_out;  // [T][H][D]
 };
 
+constexpr size_t kRunSums = 2 * 128 * 128;  // two streams of 128 columns, or one of 256, for 128 rows
+
 struct PagedAttnArgs {
   PagedView kv;
   BatchView bv;
@@ -358,6 +360,7 @@ struct PagedAttnArgs {
   float *part_o;
   float2 *part_ml;
   uint64_t part_rows;
+  float4 *run_sums;  // tcgen05 kernels: kRunSums values of each block
   // pieces to join: of the own parts (RowPieces or, without a prefix, CutUnit) and of the prefix
   CutUnit *cuts;
   RowPieces *own_pieces, *pre_pieces;

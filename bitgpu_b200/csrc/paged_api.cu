@@ -41,8 +41,8 @@ constexpr uint32_t kSMs = 148;
 constexpr uint64_t kManyTiles = 8;
 
 // The kernels of one call and the layout of its workspace: partial rows o [part_rows][D] f32, then ml
-// [part_rows] float2, then the descriptions of what is to be joined, then (tcgen05) the halves
-// of f32 rows.
+// [part_rows] float2, then the descriptions of what is to be joined, then (tcgen05) the blocks' run sums and the
+// halves of f32 rows.
 //   join        a shared prefix: every row joins its parts
 //   tc_pre      the prefix's units run on tcgen05
 //   tc_own      sequences of more than 16 rows run on tcgen05
@@ -61,7 +61,7 @@ struct Plan {
   uint32_t slot_own, slot_pre;      // first partial row of each kernel's slots (the decode kernel's: 0)
   uint32_t row_own, row_pre;        // ... of the whole units behind a prefix
   uint64_t rows, part_rows;         // tokens * H; all partial rows
-  size_t desc, halves, bytes;       // offsets of the descriptions and of q's halves (0: none), size of all
+  size_t desc, sums, halves, bytes;  // offsets of the descriptions, of the run sums and q's halves (0: none), size of all
 };
 
 Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, uint32_t KV, uint32_t D, bool fast, bool lo) {
@@ -108,9 +108,13 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
   p.part_rows = at;
   p.desc = (size_t)p.part_rows * (D * 4 + 8);
   p.bytes = p.desc + (p.join ? 2 * p.rows * sizeof(RowPieces) : (p.blocks + kSMs) * sizeof(CutUnit));
-  if (lo && (p.tc_own || p.tc_pre)) {
-    p.halves = (p.bytes + 127) / 128 * 128;
-    p.bytes = p.halves + p.rows * D * 4;
+  if (p.tc_own || p.tc_pre) {
+    p.sums = (p.bytes + 127) / 128 * 128;  // of one launch at a time: they follow one another
+    p.bytes = p.sums + kSMs * kRunSums * sizeof(float);
+    if (lo) {
+      p.halves = p.bytes;
+      p.bytes += p.rows * D * 4;
+    }
   }
   return p;
 }
@@ -217,6 +221,7 @@ int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, ui
   if (!plan.fast) return launch_paged_generic(a, plan.nsplit, st);
   unsigned char *desc = static_cast<unsigned char *>(workspace) + plan.desc;
   CutUnit *cuts = reinterpret_cast<CutUnit *>(desc);
+  if (plan.sums) a.run_sums = reinterpret_cast<float4 *>(static_cast<unsigned char *>(workspace) + plan.sums);
   if (plan.halves) a.q_halves = static_cast<unsigned char *>(workspace) + plan.halves;
   if (plan.join) {
     a.own_pieces = reinterpret_cast<RowPieces *>(desc);

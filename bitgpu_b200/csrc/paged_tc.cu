@@ -24,6 +24,13 @@
 //           error of f16 rows; the extra products cost less than that here, because the softmax warps
 //           and not the tensor pipe set the pace of the single-product form.)
 //
+// The MMA drops the low bits of what it accumulates (a rounding towards zero a step, measured 0.8 * 2^-24 of the
+// sum), so an accumulator that runs over a whole unit of many tiles errs in proportion to their number: 4e-4 after
+// 120000 positions.  So a run is bounded (TcCfg::RUN): the softmax warps then add O to a sum in global memory, one
+// rounded addition a run, and the next PV starts from zero.  It costs f32 rows 5 to 15 % (512 tokens behind 32768
+// positions 660 -> 735 us, q8 1025 -> 1180) and f16 rows of head_dim 128 up to 4 % (mixed prompts 195 -> 202), where
+// the code alone, which such short units never reach, does.
+//
 // Warp roles: warp 0 TMA producer of K and V (f16 pool; page boxes, 128-byte swizzle), warp 1 MMA issuer,
 // warps 2-3 ask for the next unit's query rows as soon as the last S of the current one is done, warps 4-11
 // softmax (one row per thread), warps 12-15 and 16-19 (q8 pool) dequantise K and V, a tile ahead in registers.
@@ -61,6 +68,9 @@ struct TcCfg {
   static constexpr int oQ = 0, oK = NQT * NQ * QT, oV = oK + NST * NK * KVT, oB = oV + NST * NK * KVT;
   static constexpr int oInfo = oB + 384, oML = oInfo + 64, oScan = oML + kM * 8;
   static constexpr int SMEM = oScan + 24 * 8;
+  // a stream's tiles in one accumulator run: at most 64 MMAs for f32 rows (3e-6), 512 for f16 rows (2.5e-5, a
+  // twentieth of the result's rounding)
+  static constexpr int RUN = (LO ? 64 : 512) / (KT / 16 * (NQ + NK - 1)) & (LO ? ~3 : ~0);
   static constexpr int THREADS = Q8 ? 640 : 384;
   // TMEM columns: part x of stream t at (2t + x) * SW, outputs behind them
   static constexpr uint32_t O0 = 256, O1 = 384;
@@ -157,6 +167,57 @@ __device__ __forceinline__ void store_words(void *dst, const uint32_t (&w)[N], u
     for (int i = 0; i < N; i += 4)
       *reinterpret_cast<uint4 *>(static_cast<uint32_t *>(dst) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
   }
+}
+
+// A row's O in TMEM joins its run sum, whose weights are f times those of O now.  Only this thread adds to the row,
+// so reductions (which it need not wait for) happen in its order.
+template <int D>
+__device__ __forceinline__ void add_run(uint32_t obase, float4 *sum, float f, bool summed) {
+  if (summed && __any_sync(0xffffffffu, f != 1.0f)) {  // rare: the reference moved since the last run
+#pragma unroll 4
+    for (int i = 0; i < D / 4; ++i) {
+      const float4 v = __ldcg(sum + i * kM);
+      __stcg(sum + i * kM, make_float4(v.x * f, v.y * f, v.z * f, v.w * f));
+    }
+  }
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32(obase + c * 32, o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float4 *at = sum + (c * 8 + i) * kM;
+      const float4 x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                                   __uint_as_float(o[4 * i + 3]));
+      if (summed)
+        asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(x.x), "f"(x.y), "f"(x.z),
+                     "f"(x.w)
+                     : "memory");
+      else __stcg(at, x);
+    }
+  }
+}
+
+// The whole sum, f times, to O.
+template <int D>
+__device__ __forceinline__ void add_sum(uint32_t obase, const float4 *sum, float f) {
+#pragma unroll 1
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32(obase + c * 32, o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 v = __ldcg(sum + (c * 8 + i) * kM);
+      o[4 * i] = __float_as_uint(fmaf(v.x, f, __uint_as_float(o[4 * i])));
+      o[4 * i + 1] = __float_as_uint(fmaf(v.y, f, __uint_as_float(o[4 * i + 1])));
+      o[4 * i + 2] = __float_as_uint(fmaf(v.z, f, __uint_as_float(o[4 * i + 2])));
+      o[4 * i + 3] = __float_as_uint(fmaf(v.w, f, __uint_as_float(o[4 * i + 3])));
+    }
+    tmem_st32(obase + c * 32, o);
+  }
+  tmem_wait_st();
 }
 
 template <int D, bool Q8, bool LO, int NQT>
@@ -382,7 +443,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
             pp ^= 1u << b;
             tc_fence_after();
             if (elect_one()) {
-              issue_pv(t, x, stage(i), h, i >= STEP || h > 0);
+              issue_pv(t, x, stage(i), h, i / STEP % C::RUN != 0 || h > 0);
               umma_commit(&pv_done[t]);
               if (h == C::PARTS - 1) {
                 if (NQT == 1 || t == 1) umma_commit(&v_empty[stage(i)]);
@@ -483,6 +544,9 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     if (t < C::NS) {
       uint32_t sp = 0;           // next phase parity of s_full, one bit per slot of this stream
       uint32_t nv = 0;           // this stream's PVs of the pieces before
+      // sums of this stream's runs: four columns of the 128 rows after one another
+      constexpr int SUM = D / 4 * kM;
+      float4 *const my_sums = a.run_sums + ((uint64_t)blockIdx.x * C::NS + t) * SUM + row;
       for (uint32_t piece = 0;; ++piece) {
         if (!mbar_wait_warp(q_full, piece & 1)) { ok = false; break; }
         const TcInfo in = *info;
@@ -499,103 +563,117 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
           for (int i = 0; i < D / 32; ++i) asm volatile("prefetch.global.L2 [%0];" ::"l"(g + 32 * i));
         }
         float m_used = kNegBig, l = 0.f;
+        float m_sum = kNegBig;     // what the run sum's weights refer to
+        bool summed = false;       // whether there is one (the same for the whole stream)
         const int step = NQT == 2 ? 1 : C::NS;
         const int first = NQT == 2 ? 0 : t;
-        for (int j = first; j < (int)in.ntiles; j += step) {
-          const int jj = NQT == 2 ? j : j / C::NS;  // tile of this stream
+        for (int j0 = first; ok && j0 < (int)in.ntiles; j0 += C::RUN * step) {
+          if (j0 != first) {
+            // the run's end: O joins the sum before the next PV overwrites it
+            if (!mbar_wait_warp(&pv_done[t], (nv + j0 / step * C::PARTS - 1) & 1)) { ok = false; break; }
+            tc_fence_after();
+            add_run<D>(obase, my_sums, ex2_approx(m_sum - m_used), summed);
+            tc_fence_before();
+            m_sum = m_used;
+            summed = true;
+          }
+          const int j1 = min((int)in.ntiles, j0 + C::RUN * step);
+          for (int j = j0; j < j1; j += step) {
+            const int jj = NQT == 2 ? j : j / C::NS;  // tile of this stream
 #pragma unroll 1
-          for (int h = 0; h < C::PARTS; ++h) {
-            const int g = jj * C::PARTS + h, part = g & 1;  // step of this stream, and where its scores lie
-            if (h == 0) {
-              const int u = C::PARTS == 2 ? 0 : part;
-              if (!mbar_wait_warp(&s_full[2 * t + u], (sp >> u) & 1)) { ok = false; break; }
-              sp ^= 1u << u;
-              tc_fence_after();
-            }
-            const uint32_t sbase = (tmem + (2 * t + part) * SW) | lane_off;
-            const int key0 = (int)(in.tile0 + j) * KT + h * SW;
-            const int nvalid = min(SW, max(0, lim - key0 + 1));
-            uint32_t x[SW / 32][32];  // the step's scores of the row: one TMEM wait
+            for (int h = 0; h < C::PARTS; ++h) {
+              const int g = jj * C::PARTS + h, part = g & 1;  // step of this stream, and where its scores lie
+              if (h == 0) {
+                const int u = C::PARTS == 2 ? 0 : part;
+                if (!mbar_wait_warp(&s_full[2 * t + u], (sp >> u) & 1)) { ok = false; break; }
+                sp ^= 1u << u;
+                tc_fence_after();
+              }
+              const uint32_t sbase = (tmem + (2 * t + part) * SW) | lane_off;
+              const int key0 = (int)(in.tile0 + j) * KT + h * SW;
+              const int nvalid = min(SW, max(0, lim - key0 + 1));
+              uint32_t x[SW / 32][32];  // the step's scores of the row: one TMEM wait
 #pragma unroll
-            for (int c = 0; c < SW / 32; ++c) tmem_ld32(sbase + c * 32, x[c]);
-            tmem_wait_ld();
-            if (nvalid < SW) {
+              for (int c = 0; c < SW / 32; ++c) tmem_ld32(sbase + c * 32, x[c]);
+              tmem_wait_ld();
+              if (nvalid < SW) {
+#pragma unroll
+                for (int c = 0; c < SW / 32; ++c)
+#pragma unroll
+                  for (int i = 0; i < 32; ++i)
+                    if (c * 32 + i >= nvalid) x[c][i] = __float_as_uint(-INFINITY);
+              }
+              float mx8[8];  // eight independent chains
+#pragma unroll
+              for (int k = 0; k < 8; ++k) mx8[k] = -INFINITY;
 #pragma unroll
               for (int c = 0; c < SW / 32; ++c)
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (c * 32 + i >= nvalid) x[c][i] = __float_as_uint(-INFINITY);
-            }
-            float mx8[8];  // eight independent chains
-#pragma unroll
-            for (int k = 0; k < 8; ++k) mx8[k] = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < SW / 32; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                const int k = (c * 16 + i / 2) & 7;
-                mx8[k] = fmax3(mx8[k], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
-              }
-            const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]),
-                                   fmax3(mx8[3], mx8[4], fmaxf(mx8[5], fmaxf(mx8[6], mx8[7]))));
-            const float mt = mx * sl2;
-            // lazy rescale: the whole warp takes the TMEM round trip when any of its rows moved far; rows
-            // that did not use the factor 1.  The PV before must have completed.
-            // Phases of pv_done are only ever waited for before this tile's P is handed over (or, after the
-            // last one, by the wait below): the barrier cannot have moved on by two.
-            bool waited = g == 0;
-            const bool need = mt > m_used + kRescale;
-            if (__any_sync(0xffffffffu, need)) {
-              if (g > 0) {
-                if (!mbar_wait_warp(&pv_done[t], (nv + g - 1) & 1)) { ok = false; break; }
-                waited = true;
-                tc_fence_after();
-                const float f = need ? ex2_approx(m_used - mt) : 1.0f;
+                for (int i = 0; i < 32; i += 2) {
+                  const int k = (c * 16 + i / 2) & 7;
+                  mx8[k] = fmax3(mx8[k], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+                }
+              const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]),
+                                     fmax3(mx8[3], mx8[4], fmaxf(mx8[5], fmaxf(mx8[6], mx8[7]))));
+              const float mt = mx * sl2;
+              // lazy rescale: the whole warp takes the TMEM round trip when any of its rows moved far; rows
+              // that did not use the factor 1.  The PV before must have completed.
+              // Phases of pv_done are only ever waited for before this tile's P is handed over (or, after a run's
+              // last one, by the waits at its end): the barrier cannot have moved on by two.
+              bool waited = g == 0;
+              const bool need = mt > m_used + kRescale;
+              if (__any_sync(0xffffffffu, need)) {
+                if (g > 0) {
+                  if (!mbar_wait_warp(&pv_done[t], (nv + g - 1) & 1)) { ok = false; break; }
+                  waited = true;
+                  tc_fence_after();
+                  const float f = need ? ex2_approx(m_used - mt) : 1.0f;
 #pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                  uint32_t o[32];
-                  tmem_ld32(obase + c * 32, o);
-                  tmem_wait_ld();
+                  for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(obase + c * 32, o);
+                    tmem_wait_ld();
 #pragma unroll
-                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                  tmem_st32(obase + c * 32, o);
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tmem_st32(obase + c * 32, o);
+                  }
+                  l *= f;
                 }
-                l *= f;
+                if (need) m_used = mt;
               }
-              if (need) m_used = mt;
-            }
-            const float mneg = kUp - m_used;
-            const uint64_t sl2x2 = pack2(sl2, sl2), mneg2 = pack2(mneg, mneg);
-            uint64_t sums[2] = {0, 0};
+              const float mneg = kUp - m_used;
+              const uint64_t sl2x2 = pack2(sl2, sl2), mneg2 = pack2(mneg, mneg);
+              uint64_t sums[2] = {0, 0};
 #pragma unroll
-            for (int c = 0; c < SW / 32; ++c) {
-              uint32_t hi[16], lo[16];
+              for (int c = 0; c < SW / 32; ++c) {
+                uint32_t hi[16], lo[16];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const uint64_t s2 = pack2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1]));
-                const float2 e = unpack2(fma2(s2, sl2x2, mneg2));
-                const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
-                const uint64_t pp = pack2(p0, p1);
-                sums[i & 1] = add2(sums[i & 1], pp);
-                hi[i] = pack_half2(p0, p1);
-                if constexpr (LO) {
-                  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
-                  lo[i] = pack_half2(p0 - f.x, p1 - f.y);
+                for (int i = 0; i < 16; ++i) {
+                  const uint64_t s2 = pack2(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1]));
+                  const float2 e = unpack2(fma2(s2, sl2x2, mneg2));
+                  const float p0 = ex2_approx(e.x), p1 = ex2_approx(e.y);
+                  const uint64_t pp = pack2(p0, p1);
+                  sums[i & 1] = add2(sums[i & 1], pp);
+                  hi[i] = pack_half2(p0, p1);
+                  if constexpr (LO) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&hi[i]));
+                    lo[i] = pack_half2(p0 - f.x, p1 - f.y);
+                  }
                 }
+                tmem_st16(sbase + c * 16, hi);
+                if constexpr (LO) tmem_st16(sbase + SW / 2 + c * 16, lo);
               }
-              tmem_st16(sbase + c * 16, hi);
-              if constexpr (LO) tmem_st16(sbase + SW / 2 + c * 16, lo);
+              const float2 sum = unpack2(add2(sums[0], sums[1]));
+              l += sum.x + sum.y;
+              tmem_wait_st();
+              const bool last = j + step >= j1 && h == C::PARTS - 1;
+              if (last && !waited && !mbar_wait_warp(&pv_done[t], (nv + g - 1) & 1)) { ok = false; break; }
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_full[2 * t + part]);
             }
-            const float2 sum = unpack2(add2(sums[0], sums[1]));
-            l += sum.x + sum.y;
-            tmem_wait_st();
-            const bool last = j + step >= (int)in.ntiles && h == C::PARTS - 1;
-            if (last && !waited && !mbar_wait_warp(&pv_done[t], (nv + g - 1) & 1)) { ok = false; break; }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[2 * t + part]);
+            if (!ok) break;
           }
-          if (!ok) break;
         }
         if (!ok) break;
         // ---- the piece's rows ----
@@ -603,6 +681,10 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         const bool some = mine > 0;
         if (some && !mbar_wait_warp(&pv_done[t], (nv + mine * C::PARTS - 1) & 1)) { ok = false; break; }
         nv += mine * C::PARTS;
+        if (summed) {
+          tc_fence_after();
+          add_sum<D>(obase, my_sums, ex2_approx(m_sum - m_used));
+        }
         float f0 = 1.f, f1 = 0.f, M = m_used, L = l;
         if constexpr (NQT == 1 && C::NS == 2) {
           if (t == 1) {

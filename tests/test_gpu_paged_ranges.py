@@ -1,0 +1,110 @@
+"""Paged attention over the whole range of its values, through each of its kernels: small, large and mixed
+q8 block scales, every q8 code, small and large f32 queries, gates, lengths beyond the page table, long runs
+of one accumulator.  Definitions in 64 bits and tolerances: tests/paged_util.py."""
+import math
+
+import pytest
+import torch
+
+from paged_util import Ragged, tolerance
+from test_gpu_paged_attention import DT, ops  # noqa: F401  (a fixture)
+from test_gpu_paged_matrix import wide
+
+pytestmark = pytest.mark.gpu
+
+# rows of a unit decide the kernel's form: 4, 8 or 16 rows of the decode kernel, a tile of the tcgen05 kernel; "cuda"
+# is the CUDA-core kernel
+KERNELS = {"cuda": (4, [1, 3, 1]), "decode4": (4, [1, 1, 1]), "decode8": (6, [1, 1, 1]), "decode16": (4, [3, 2, 4]),
+           "tc": (4, [40, 1, 70])}
+each_kernel = pytest.mark.parametrize("kernel", list(KERNELS))
+
+
+def make(kernel, mode="q8", D=128, lens=(700, 64, 130), seed=1, **kw):
+    G, news = KERNELS[kernel]
+    r = Ragged(list(lens), news, KV=2, G=G, D=D, mode=mode, seed=seed, **kw)
+    return wide(r) if kernel == "tc" else r
+
+
+def rescale(r, which, factor):
+    """Multiply the block scales of K (0) or V (1) by ``factor`` (broadcast to [slots, KV, D / 32])."""
+    sc = r.scales[which]
+    sc.copy_((sc.double().view(-1, r.KV, r.D // 32) * factor).float().view(sc.shape))
+    revalue(r)
+
+
+def revalue(r):
+    """What codes and scales stand for, in 64 bits."""
+    for i in range(2):
+        v = (r.data[i].double() / 127).clamp(min=-1).view(-1, r.KV, r.D // 32, 32)
+        r.values[i] = (v * r.scales[i].double().view(-1, r.KV, r.D // 32, 1)).view(-1, r.KV, r.D)
+
+
+def attend(ops, kernel, r, q, out_dtype, **kw):  # noqa: F811
+    from bitgpu_b200._lib import lib
+    lib().bg_force_generic(int(kernel == "cuda"))
+    try:
+        out = ops.paged_attention(q.cuda(), r.cache(ops), r.batch(ops), out_dtype=out_dtype, **kw)
+    finally:
+        lib().bg_force_generic(0)
+    assert lib().bg_device_status(None) == 0
+    return out.cpu()
+
+
+def check(r, got, want, q_dtype, extra=0.0):
+    """Beside ``tolerance``: weights enter the products as f16 halves at least 2^6 times as large as
+    exp(score - largest score), so a weight may be off by 2^-31 of the largest (the smallest f16 step is 2^-24):
+    2^-31 * sum |v| of a result."""
+    out, A, S = want
+    lost = torch.zeros_like(out)
+    for b, n in enumerate(r.news):
+        v = r.kv(b)[1].abs().nan_to_num(0).sum(0).repeat_interleave(r.G, 0)
+        lost[r.cu[b]:r.cu[b] + n] = 2.0 ** -31 * v
+    tol = tolerance(out, A, S, q_dtype == torch.float16, got.dtype == torch.float16) + lost + extra
+    err = (got.double() - out).abs()
+    assert torch.isfinite(got).all(), "not finite"
+    assert (err <= tol).all(), f"error {float((err / (out.abs() + 1e-300)).max()):.3g} relative, {float((err / tol).max()):.3g} of what is allowed"
+
+
+# ---- long runs of one accumulator ----------------------------------------------------------------
+@pytest.mark.parametrize("mode", ["f16", "q8"])
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("length", [2000, 9000, 40000, 120000])
+def test_long_units(ops, mode, D, length):  # noqa: F811
+    """Units that stay whole over many tiles, values of one sign: the error of f32 rows does not grow with the
+    length.  A run of matrix products into one accumulator has at most 64 steps, each of which may drop less than
+    2^-23 of what has been added up; the parts of equal steps add up to 33 / 64 of that: 64 * 2^-24 in all, beside
+    the tolerance's other terms."""
+    KV, G, n, B = 8, 4, 20, 40
+    H, page = KV * G, 64
+    pages = -(-length // page)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    shape = (pages, page, KV, D)
+    if mode == "f16":
+        kv = [torch.randn(shape, generator=g, device="cuda").half(),
+              (1 + 0.2 * torch.rand(shape, generator=g, device="cuda")).half(), None, None]
+        K, V = kv[0].view(-1, KV, D)[:length].double(), kv[1].view(-1, KV, D)[:length].double()
+    else:
+        sc = [torch.rand(shape[:3] + (D // 32,), generator=g, device="cuda") + s for s in (0.5, 1.0)]
+        kv = [torch.randint(-127, 128, shape, generator=g, device="cuda", dtype=torch.int8),
+              torch.randint(100, 128, shape, generator=g, device="cuda", dtype=torch.int8), *sc]
+        K, V = ((kv[i].double() / 127 * sc[i].double().repeat_interleave(32, -1)).view(-1, KV, D)[:length] for i in (0, 1))
+    cache = ops.PagedKVCache.from_tensors(*kv)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(B, pages).contiguous()
+    lens = torch.full((B,), length, dtype=torch.int32, device="cuda")
+    cu = torch.arange(0, n * B + 1, n, dtype=torch.int32, device="cuda")
+    q = (torch.randn((n * B, H, D), generator=g, device="cuda") * 0.05)
+    got = ops.paged_attention(q, cache, ops.PagedBatch(table, lens, cu, n * B, n))
+    from bitgpu_b200._lib import lib
+    assert lib().bg_device_status(None) == 0
+    worst = 0.0
+    for b, i in ((0, 0), (17, 19), (39, 7)):
+        m = length - n + i + 1
+        t = b * n + i
+        for k in range(KV):
+            qq = q[t].view(KV, G, D)[k].double()
+            s = qq @ K[:m, k].T * D ** -0.5
+            S = float((qq.abs() @ K[:m, k].abs().T).max()) * D ** -0.5
+            w = torch.softmax(s, -1) @ V[:m, k]
+            err = (got[t].view(KV, G, D)[k].double() - w).abs() / ((28 * S + 16 + 64) * 2.0 ** -24 * w)
+            worst = max(worst, float(err.max()))
+    assert worst <= 1, f"{worst:.3g} of what is allowed"
