@@ -192,6 +192,7 @@ struct Piece {
   uint32_t R0, rows, kvh;   // rows [R0, R0 + rows) of kv head kvh
   uint32_t tile0, ntiles;   // tiles of the unit
   uint32_t len;             // positions of the list (the prefix's or the sequence's)
+  uint32_t list;            // the sequence, or B for the prefix
   int32_t lim_base;         // token t attends positions <= lim_base + t
   const int32_t *pages;
   uint32_t npieces;         // pieces of the unit
@@ -245,6 +246,7 @@ struct PieceWalk {
         p.len = bv.prefix_len;
         p.lim_base = 0x40000000;
         p.pages = bv.prefix_pages;
+        p.list = bv.B;
         p.own = false;
         if (cur < at) cur = min(at, t1);
         if (cur >= t1) return false;  // only (some of) the lead is this block's
@@ -267,6 +269,7 @@ struct PieceWalk {
         p.len = (uint32_t)sr.len;
         p.lim_base = sr.len - (int32_t)sr.n - (int32_t)sr.begin;
         p.pages = bv.table + (uint64_t)b * bv.table_stride;
+        p.list = b;
         p.own = true;
         p.ntiles = min(n - done, t1 - cur);
         in += p.ntiles;
@@ -344,6 +347,7 @@ struct PagedAppendArgs {
   void *q_out;  // [T][H][D]
 };
 
+constexpr uint32_t kTopRow = 16;  // a row of largest scales: V's blocks, K's
 constexpr size_t kRunSums = 2 * 128 * 128;  // two streams of 128 columns, or one of 256, for 128 rows
 
 struct PagedAttnArgs {
@@ -360,6 +364,7 @@ struct PagedAttnArgs {
   float *part_o;
   float2 *part_ml;
   uint64_t part_rows;
+  uint32_t *tops;    // tcgen05 kernels, q8 pool: [list: sequences, prefix][kv head][kTopRow]
   float4 *run_sums;  // tcgen05 kernels: kRunSums values of each block
   // pieces to join: of the own parts (RowPieces or, without a prefix, CutUnit) and of the prefix
   CutUnit *cuts;
@@ -380,7 +385,8 @@ bool paged_decode_supported(int mode, uint32_t D, uint32_t page_size);
 uint32_t paged_decode_blocks(int mode, uint32_t D, uint32_t ru);  // blocks that fill the GPU
 int launch_paged_decode(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_hi, bool prefix, cudaStream_t st);
 // tcgen05 kernel: many rows a sequence (own part), or the rows of the batch against the shared prefix.
-bool paged_tc_supported(int mode, uint32_t D, uint32_t G, uint32_t page_size);
+bool paged_tc_supported(int mode, uint32_t D, uint32_t G, uint32_t KV, uint32_t page_size);
+int launch_paged_top_scales(const PagedAttnArgs &a, uint32_t rows_lo, bool own, bool prefix, cudaStream_t st);
 uint32_t paged_tc_rows(uint32_t D, uint32_t G, bool lo, uint64_t rows);
 int launch_paged_split_rows(const PagedAttnArgs &a, cudaStream_t st);
 int launch_paged_tc(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_lo, bool prefix, cudaStream_t st);

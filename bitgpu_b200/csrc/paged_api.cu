@@ -41,8 +41,8 @@ constexpr uint32_t kSMs = 148;
 constexpr uint64_t kManyTiles = 8;
 
 // The kernels of one call and the layout of its workspace: partial rows o [part_rows][D] f32, then ml
-// [part_rows] float2, then the descriptions of what is to be joined, then (tcgen05) the blocks' run sums and the
-// halves of f32 rows.
+// [part_rows] float2, then the descriptions of what is to be joined, then (tcgen05) the blocks' run sums, the
+// largest block scales of a q8 pool and the halves of f32 rows.
 //   join        a shared prefix: every row joins its parts
 //   tc_pre      the prefix's units run on tcgen05
 //   tc_own      sequences of more than 16 rows run on tcgen05
@@ -61,7 +61,7 @@ struct Plan {
   uint32_t slot_own, slot_pre;      // first partial row of each kernel's slots (the decode kernel's: 0)
   uint32_t row_own, row_pre;        // ... of the whole units behind a prefix
   uint64_t rows, part_rows;         // tokens * H; all partial rows
-  size_t desc, sums, halves, bytes;  // offsets of the descriptions, of the run sums and q's halves (0: none), size of all
+  size_t desc, sums, tops, halves, bytes;  // offsets of the descriptions, run sums, scales and q's halves (0: none), size
 };
 
 Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, uint32_t KV, uint32_t D, bool fast, bool lo) {
@@ -80,7 +80,7 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
     return p;
   }
   const uint64_t group = (uint64_t)b->max_q * G, all = (uint64_t)b->tokens * G;
-  const bool tc = paged_tc_supported((int)kv->mode, D, G, kv->page_size);
+  const bool tc = paged_tc_supported((int)kv->mode, D, G, KV, kv->page_size);
   const uint64_t own_tiles = (all + 15) / 16 * KV * ((cap + 63) / 64);
   const uint64_t pre_tiles = (all + 15) / 16 * KV * ((uint64_t)(b->prefix_len + 63) / 64);
   const uint64_t many = kManyTiles * paged_decode_blocks((int)kv->mode, D, 16);
@@ -111,6 +111,11 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
   if (p.tc_own || p.tc_pre) {
     p.sums = (p.bytes + 127) / 128 * 128;  // of one launch at a time: they follow one another
     p.bytes = p.sums + kSMs * kRunSums * sizeof(float);
+    if (kv->mode == BG_KV_Q8) {
+      p.tops = p.bytes;
+      p.bytes += ((uint64_t)b->batch + 1) * KV * kTopRow * 4;
+      p.bytes = (p.bytes + 127) / 128 * 128;
+    }
     if (lo) {
       p.halves = p.bytes;
       p.bytes += p.rows * D * 4;
@@ -222,6 +227,7 @@ int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, ui
   unsigned char *desc = static_cast<unsigned char *>(workspace) + plan.desc;
   CutUnit *cuts = reinterpret_cast<CutUnit *>(desc);
   if (plan.sums) a.run_sums = reinterpret_cast<float4 *>(static_cast<unsigned char *>(workspace) + plan.sums);
+  if (plan.tops) a.tops = reinterpret_cast<uint32_t *>(static_cast<unsigned char *>(workspace) + plan.tops);
   if (plan.halves) a.q_halves = static_cast<unsigned char *>(workspace) + plan.halves;
   if (plan.join) {
     a.own_pieces = reinterpret_cast<RowPieces *>(desc);
@@ -238,10 +244,13 @@ int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, ui
   const PagedAttnArgs dec = with(0, cuts), own = with(plan.slot_own, cuts + plan.blocks), pre = with(plan.slot_pre, nullptr);
   if (plan.halves)
     if (int rc = launch_paged_split_rows(a, st)) return rc;
+  const uint32_t rows_lo = plan.decode ? 16 : 0;  // sequences of more rows are the tcgen05 kernel's
+  if (plan.tops)
+    if (int rc = launch_paged_top_scales(a, rows_lo, plan.tc_own, plan.tc_pre, st)) return rc;
   if (plan.tc_pre)
     if (int rc = launch_paged_tc(pre, kSMs, plan.ru_pre, 0, true, st)) return rc;
   if (plan.tc_own)
-    if (int rc = launch_paged_tc(own, kSMs, plan.ru_own, plan.decode ? 16 : 0, false, st)) return rc;
+    if (int rc = launch_paged_tc(own, kSMs, plan.ru_own, rows_lo, false, st)) return rc;
   if (plan.decode)
     if (int rc = launch_paged_decode(dec, plan.blocks, plan.ru, plan.tc_own ? 16 : 0xffffffffu, plan.join && !plan.tc_pre, st))
       return rc;

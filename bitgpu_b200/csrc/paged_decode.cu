@@ -17,9 +17,11 @@
 //   * f32 rows (LO): q and p are split into two f16 operands (22 bits).  Up to four rows a unit (PK; one
 //     token of a group of four heads) the halves share one product, hi in columns 0-3 and lo in 4-7 of the
 //     MMA's eight; otherwise both products run twice.  f16 rows: q is exact and p is rounded once to f16,
-//     which costs about as much as the rounding of the result.  p carries a factor 2^14 (q8: 2^6, since
-//     V's block scale is folded into p), which cancels in the quotient and keeps small weights out of
-//     f16's subnormals;
+//     which costs about as much as the rounding of the result.  p carries a factor 2^14, which cancels in the
+//     quotient and keeps small weights out of f16's subnormals;
+//   * q8: the weights of V's codes are p * block scale / 127, of any magnitude.  Each warp's 16 positions and each
+//     block of 32 channels have a power of two that brings the largest to [2^14, 2^15); their products start from
+//     zero and join the output by one fused multiply-add that puts the power back;
 //   * q8 codes enter the products as exact f16 integers: byte + 128 under the f16 pattern 0x64xx is
 //     1152 + code, and one packed subtraction leaves the code.  (Cancelling the 1152 inside the MMA
 //     instead costs accuracy: the f32 accumulator then holds sums 1152 / |code| times as large.)
@@ -89,7 +91,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
   constexpr int NST = C::NST, NB = C::NB, KS = D / 16, NN = C::NN;
   static_assert(!PK || (LO && NT == 1), "packed halves");
   constexpr bool TWO = LO && !PK;  // the low halves have products of their own
-  constexpr float kShift = MODE == BG_KV_F16 ? 14.f : 6.f;  // log2 of the factor that p carries
+  constexpr float kShift = MODE == BG_KV_F16 ? 14.f : 0.f;  // log2 of the factor that p carries
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::oB);
   uint64_t *empty = full + NST, *ufull = empty + NST, *uempty = ufull + kUnits;
@@ -430,11 +432,11 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           moved |= corr != 1.0f;
         }
       }
-      // f16 rows: rescale the output only when a running max of this warp moved.  f32 rows: every tile's
+      // f16 rows, q8 pool: rescale the output only when a running max of this warp moved.  f32 rows: every tile's
       // products start from zero and are added to the rescaled output by one fused multiply-add per
       // value -- the MMA truncates what it accumulates, and over the ~100 tiles of a long split that bias
       // alone (3e-6 at 131072 positions) is more than all other errors together.
-      if (!LO && __any_sync(0xffffffffu, moved)) {
+      if ((!LO || MODE == BG_KV_Q8) && __any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -504,11 +506,24 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
         for (int bk = 0; bk < NB; ++bk) {
           const float va = vsc[(row0 + (lane >> 2)) * NB + bk] * (1.0f / 127.0f);
           const float vbb = vsc[(row0 + (lane >> 2) + 8) * NB + bk] * (1.0f / 127.0f);
+          float w[NT][4], top = 0.f;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            w[nt][0] = pr[nt][0] * va;
+            w[nt][1] = pr[nt][1] * va;
+            w[nt][2] = pr[nt][2] * vbb;
+            w[nt][3] = pr[nt][3] * vbb;
+            top = fmaxf(fmaxf(top, fmaxf(fabsf(w[nt][0]), fabsf(w[nt][1]))), fmaxf(fabsf(w[nt][2]), fabsf(w[nt][3])));
+          }
+          // `back`: the power of two of the largest weight, over 2^14 (at least 2^-126); `fore`: its inverse
+          const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+          const uint32_t e = (uint32_t)max((int)(bits & 0x7f800000u) - (14 << 23), 1 << 23);
+          const float back = __uint_as_float(e), fore = __uint_as_float(0x7f000000u - e);
           uint32_t pb0[NT], pb1[NT], pl0[NT], pl1[NT];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            split(pr[nt][0] * va, pr[nt][1] * va, pb0[nt], pl0[nt]);
-            split(pr[nt][2] * vbb, pr[nt][3] * vbb, pb1[nt], pl1[nt]);
+            split(w[nt][0] * fore, w[nt][1] * fore, pb0[nt], pl0[nt]);
+            split(w[nt][2] * fore, w[nt][3] * fore, pb1[nt], pl1[nt]);
           }
           uint32_t r[4];
           ldsm_x4_t(r, swz<kTile>(vb, row0 + lrow, 2 * bk + lhi));
@@ -518,22 +533,17 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           const uint32_t a1[4] = {code(r[2], kSelEven), code(r[2], kSelOdd), code(r[3], kSelEven), code(r[3], kSelOdd)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            if constexpr (LO) {
-              float x0[4] = {0.f, 0.f, 0.f, 0.f}, x1[4] = {0.f, 0.f, 0.f, 0.f};
-              if constexpr (TWO) {
-                mma16816(x0, a0, pl0[nt], pl1[nt]);
-                mma16816(x1, a1, pl0[nt], pl1[nt]);
-              }
-              mma16816(x0, a0, pb0[nt], pb1[nt]);
-              mma16816(x1, a1, pb0[nt], pb1[nt]);
+            float x0[4] = {0.f, 0.f, 0.f, 0.f}, x1[4] = {0.f, 0.f, 0.f, 0.f};
+            if constexpr (TWO) {
+              mma16816(x0, a0, pl0[nt], pl1[nt]);
+              mma16816(x1, a1, pl0[nt], pl1[nt]);
+            }
+            mma16816(x0, a0, pb0[nt], pb1[nt]);
+            mma16816(x1, a1, pb0[nt], pb1[nt]);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                oacc[nt][2 * bk][i] = fmaf(oacc[nt][2 * bk][i], cr[nt][i & 1], x0[i]);
-                oacc[nt][2 * bk + 1][i] = fmaf(oacc[nt][2 * bk + 1][i], cr[nt][i & 1], x1[i]);
-              }
-            } else {
-              mma16816(oacc[nt][2 * bk], a0, pb0[nt], pb1[nt]);
-              mma16816(oacc[nt][2 * bk + 1], a1, pb0[nt], pb1[nt]);
+            for (int i = 0; i < 4; ++i) {
+              oacc[nt][2 * bk][i] = fmaf(x0[i], back, oacc[nt][2 * bk][i]);
+              oacc[nt][2 * bk + 1][i] = fmaf(x1[i], back, oacc[nt][2 * bk + 1][i]);
             }
           }
         }

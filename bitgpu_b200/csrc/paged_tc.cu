@@ -22,7 +22,12 @@
 //   q8 pool: code * scale has more than 11 bits, so K and V are split too when they are dequantised into
 //           the operand tiles: one more product each.  (A single f16 rounding of K and V would double the
 //           error of f16 rows; the extra products cost less than that here, because the softmax warps
-//           and not the tensor pipe set the pace of the single-product form.)
+//           and not the tensor pipe set the pace of the single-product form.)  The halves hold code * scale
+//           without the scales' magnitude: K without the power of two of the largest scale of its page list, which
+//           the scores get back with the softmax scale, V without one per 32 channels, which the output gets back.
+//           top_scales_kernel finds them beforehand: prefix of 32768 q8 positions 211 -> 224 us, 512 f32 tokens
+//           behind as many 1180 -> 1220, 977 alone 77 -> 81.  (Found in this kernel, by the dequantising warps or by an
+//           idle one, per tile or per run of tiles, they cost the first two 230 to 250 and 1430 to 1600.)
 //
 // The MMA drops the low bits of what it accumulates (a rounding towards zero a step, measured 0.8 * 2^-24 of the
 // sum), so an accumulator that runs over a whole unit of many tiles errs in proportion to their number: 4e-4 after
@@ -37,6 +42,7 @@
 // All waits are bounded; on expiry the block records BG_ETIMEOUT, stops issuing, waits for what it issued,
 // frees its TMEM and exits.
 #include <cuda.h>
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -66,7 +72,7 @@ struct TcCfg {
   static constexpr int LEAD = Q8 ? 2 : 1;                    // a unit's own cost, in tiles
   static constexpr int NST = D == 256 && Q8 && LO ? 1 : 2;   // ring stages of K and of V
   static constexpr int oQ = 0, oK = NQT * NQ * QT, oV = oK + NST * NK * KVT, oB = oV + NST * NK * KVT;
-  static constexpr int oInfo = oB + 384, oML = oInfo + 64, oScan = oML + kM * 8;
+  static constexpr int oInfo = oB + 384, oVP = oInfo + 64, oML = oVP + 64, oScan = oML + kM * 8;
   static constexpr int SMEM = oScan + 24 * 8;
   // a stream's tiles in one accumulator run: at most 64 MMAs for f32 rows (3e-6), 512 for f16 rows (2.5e-5, a
   // twentieth of the result's rounding)
@@ -91,6 +97,7 @@ struct alignas(16) TcInfo {
   uint32_t R0, rows, kvh, tile0, ntiles, len;
   int32_t lim_base;
   uint32_t dest, row0;
+  float k_pow2;  // of K's scales (q8 pool)
 };
 constexpr uint32_t kDirect = 0xffffffffu, kRowBuf = 0xfffffffeu;
 
@@ -114,14 +121,28 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// Codes of one block scale s as two f16 halves of code * s / 127, in packed f16 arithmetic.  With
-// s / 127 = m 2^e and m = mh + ml in f16:  c' = code 2^e is exact (byte + 128 under the pattern 0x64xx is
+// The power of two that values below 2^(x + 1) are freed of to stay below 2^14 (x: the exponent in `bits`; at least
+// 2^-126), and its inverse.
+__device__ __forceinline__ float pow2_of(uint32_t bits) {
+  return __uint_as_float((uint32_t)max((int)(bits & 0x7f800000u) - (13 << 23), 1 << 23));
+}
+__device__ __forceinline__ float pow2_inv(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
+
+// Largest block scales (as bits, which order like the magnitudes) of each page list and kv head: V's blocks, K's at
+// kTopK.
+constexpr uint32_t kTopK = 8;
+__device__ __forceinline__ uint32_t top_scale(const PagedAttnArgs &a, const Piece &pc, uint32_t which) {
+  return __ldcg(a.tops + ((uint64_t)pc.list * a.kv.KV + pc.kvh) * kTopRow + which);
+}
+
+// Codes of one block as two f16 halves of code * x, x below 2^14 / 127, in packed f16 arithmetic.  With
+// x = m 2^e and m = mh + ml in f16:  c' = code 2^e is exact (byte + 128 under the pattern 0x64xx is
 // 1152 + code, and one fused multiply-add removes the 1152 and applies 2^e);  hi = c' mh rounded;
-// c' mh - hi is exact in f16, so  lo = c' ml + (c' mh - hi)  carries the rest to 2^-22 of the value.
+// c' mh - hi is exact in f16, so  lo = c' ml + (c' mh - hi)  carries the rest, to 2^-22 of the value or half of f16's
+// smallest step: 2^-25.
 struct CodeScale {
   __half2 p2, bias, mh, ml;
-  __device__ __forceinline__ explicit CodeScale(float s) {
-    const float x = s * (1.0f / 127.0f);
+  __device__ __forceinline__ explicit CodeScale(float x) {
     const int e = min(4, max(-20, (int)((__float_as_uint(x) >> 23) & 255) - 127));
     const float m = x * __uint_as_float((uint32_t)(127 - e) << 23), f = __uint_as_float((uint32_t)(127 + e) << 23);
     p2 = __float2half2_rn(f);
@@ -236,6 +257,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   uint32_t *tmem_at = reinterpret_cast<uint32_t *>(bars + 35);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 36);
   TcInfo *info = reinterpret_cast<TcInfo *>(smem + C::oInfo);
+  volatile float *v_pow2 = reinterpret_cast<float *>(smem + C::oVP);  // [2][8], by piece (q8 pool)
   float2 *ml_s = reinterpret_cast<float2 *>(smem + C::oML);
   const PagedAttnArgs &a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -274,10 +296,13 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // (a q8 pool's kernel follows top_scales_kernel, which lets it begin when all before is done: only what that one
+  // writes has to be waited for)
+  if (!Q8) asm volatile("griddepcontrol.wait;" ::: "memory");
   tc_fence_before();
   const TileSpan span = block_span<C::THREADS>(a.bv, p.u, a.kv.page_size, a.min_tiles,
                                                reinterpret_cast<uint32_t *>(smem + C::oScan));
+  if (Q8) asm volatile("griddepcontrol.wait;" ::: "memory");
   tc_fence_after();
   const uint32_t tmem = *tmem_at;
   const uint32_t sQ = smem_u32(smem + C::oQ), sK = smem_u32(smem + C::oK), sV = smem_u32(smem + C::oV);
@@ -482,6 +507,8 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       if (a.cuts && gt == 0) a.cuts[blockIdx.x].npieces = 0;
       for (uint32_t piece = 0; ok; ++piece) {
         const bool more = walk.next(pc, a.bv, p.u, ps);
+        uint32_t top = 0;
+        if (Q8 && more && gt <= kTopK) top = top_scale(a, pc, gt);
         if (piece > 0) {
           ok = mbar_wait_warp(q_free, (piece - 1) & 1) && mbar_wait_warp(info_free, (piece - 1) & 1);
           if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) break;
@@ -513,6 +540,11 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
             rp[r] = RowPieces{whole ? row0 + R / a.G * a.H + pc.kvh * a.G + R % a.G : slot + r, pc.npieces, p.u.RU, 0};
           }
         }
+        if constexpr (Q8) {
+          if (gt < kTopK) v_pow2[(piece & 1) * 8 + gt] = pow2_of(top);
+          if (gt == kTopK) info->k_pow2 = pow2_of(top);
+          __syncwarp();
+        }
         // rows come by TMA as boxes of whole tokens' heads; tokens behind the unit's are other sequences' (or
         // zeros) and the tile's last rows stay as they were: computed along, never written
         loaded = piece + 1;
@@ -539,7 +571,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
     const int row = ((warp & 3) << 5) + lane;     // TMEM lane
     const uint32_t lane_off = (uint32_t)((warp & 3) << 5) << 16;
     const uint32_t obase = (tmem + (t ? C::O1 : C::O0)) | lane_off;
-    const float sl2 = a.sl2;
+    float sl2 = a.sl2;
     bool ok = true;
     if (t < C::NS) {
       uint32_t sp = 0;           // next phase parity of s_full, one bit per slot of this stream
@@ -562,6 +594,8 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
 #pragma unroll 1
           for (int i = 0; i < D / 32; ++i) asm volatile("prefetch.global.L2 [%0];" ::"l"(g + 32 * i));
         }
+        // (never so small that a masked score times it is not -infinity)
+        if constexpr (Q8) sl2 = fmaxf(a.sl2 * in.k_pow2, 0x1p-126f);
         float m_used = kNegBig, l = 0.f;
         float m_sum = kNegBig;     // what the run sum's weights refer to
         bool summed = false;       // whether there is one (the same for the whole stream)
@@ -740,6 +774,11 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
             }
           }
           if (!valid) continue;
+          if constexpr (Q8) {
+            const float v2 = v_pow2[(piece & 1) * 8 + c];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * v2);
+          }
           if (in.dest != kDirect) {
             store_words<32>(a.part_o + prow * D + c * 32, o, p.wide);
             continue;
@@ -798,7 +837,11 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       uint4 w[NCH], wn[NCH];
       float sc[NCH], sn[NCH];
       // codes and block scales of the walk's current tile (zeros behind the length), and on to the next
-      auto fetch = [&](uint4 (&x)[NCH], float (&s)[NCH]) {
+      static_assert(128 % CPR == 0, "a thread's chunks lie in one block of 32 channels");
+      float pow2 = 1.f;  // of the walk's current piece
+      if (have) pow2 = pow2_of(top_scale(a, pc, v ? gt % CPR / 2 : kTopK));
+      auto fetch = [&](uint4 (&x)[NCH], float (&s)[NCH], float &inv) {
+        inv = pow2_inv(pow2) * (1.0f / 127.0f);
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
           const uint32_t idx = gt + i * 128, c = idx % CPR, pos = (pc.tile0 + t) * KT + idx / CPR;
@@ -818,13 +861,15 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         if (++t == pc.ntiles) {
           t = 0;
           have = walk.next(pc, a.bv, p.u, ps);
+          if (have) pow2 = pow2_of(top_scale(a, pc, v ? gt % CPR / 2 : kTopK));
         }
       };
       bool more = have;
-      if (more) fetch(w, sc);
+      float inv = 0.f, inv_next = 0.f;
+      if (more) fetch(w, sc, inv);
       for (int it = 0; more; ++it) {
         const bool next = have;
-        if (next) fetch(wn, sn);  // travels while this tile is converted
+        if (next) fetch(wn, sn, inv_next);  // travels while this tile is converted
         const int s = it % C::NST;
         if (it >= C::NST) ok = mbar_wait_warp(&empty[s], ((it / C::NST) - 1) & 1);
         if (!ok) break;
@@ -832,7 +877,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
           const uint32_t idx = gt + i * 128, r = idx / CPR, c = idx % CPR;
-          const CodeScale cs(sc[i]);
+          const CodeScale cs(sc[i] * inv);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             // the lanes of a row's second half take their two chunks in the other order: a quarter warp's
@@ -850,6 +895,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&full[s]);
         more = next;
+        inv = inv_next;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
           w[i] = wn[i];
@@ -863,6 +909,65 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// The largest block scales of the page lists that the tcgen05 kernels read (q8 pool): list blockIdx.z (the sequences
+// of more than rows_lo rows, then the prefix), kv head blockIdx.y, by a cluster of kParts blocks.  Reads 1/9 of what
+// the lists' K and V have.
+constexpr uint32_t kParts = 8;
+template <int NB>
+__global__ void __cluster_dims__(kParts, 1, 1) __launch_bounds__(512)
+    top_scales_kernel(PagedAttnArgs a, uint32_t rows_lo, uint32_t first) {
+  __shared__ uint32_t top[kTopRow];
+  const uint32_t list = first + blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 31, ps = a.kv.page_size;
+  if (threadIdx.x < kTopRow) top[threadIdx.x] = 0;
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int32_t *pages = a.bv.prefix_pages;
+  uint32_t len = a.bv.prefix_len;
+  if (list < a.bv.B) {
+    const SeqRange sr = seq_range(a.bv, list, ps);
+    pages = a.bv.table + (uint64_t)list * a.bv.table_stride;
+    len = sr.n * a.G > rows_lo ? (uint32_t)sr.len : 0;
+  }
+  constexpr uint32_t abs = 0x7fffffffu;
+  uint32_t k = 0, v[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) v[b] = 0;
+#pragma unroll 4
+  for (uint32_t pos = blockIdx.x * 512 + threadIdx.x; pos < len; pos += kParts * 512) {
+    const uint32_t pg = (uint32_t)__ldg(pages + pos / ps);
+    if (pg >= a.kv.num_pages) continue;
+    const uint64_t row = ((uint64_t)pg * ps + pos % ps) * a.kv.KV + kvh;
+    const uint4 *ks = reinterpret_cast<const uint4 *>(a.kv.Ks + row * NB), *vs = reinterpret_cast<const uint4 *>(a.kv.Vs + row * NB);
+#pragma unroll
+    for (int q = 0; q < NB / 4; ++q) {
+      const uint4 x = __ldg(ks + q), y = __ldg(vs + q);
+      k = max(k, max(max(x.x & abs, x.y & abs), max(x.z & abs, x.w & abs)));
+      v[4 * q] = max(v[4 * q], y.x & abs);
+      v[4 * q + 1] = max(v[4 * q + 1], y.y & abs);
+      v[4 * q + 2] = max(v[4 * q + 2], y.z & abs);
+      v[4 * q + 3] = max(v[4 * q + 3], y.w & abs);
+    }
+  }
+  __syncwarp();
+  k = __reduce_max_sync(0xffffffffu, k);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const uint32_t x = __reduce_max_sync(0xffffffffu, v[b]);
+    if (lane == 0) atomicMax(top + b, x);
+  }
+  if (lane == 0) atomicMax(top + kTopK, k);
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  cluster.sync();
+  if (blockIdx.x == 0 && threadIdx.x <= kTopK) {
+    uint32_t mx = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kParts; ++i) mx = max(mx, cluster.map_shared_rank(top, i)[threadIdx.x]);
+    a.tops[((uint64_t)list * a.kv.KV + kvh) * kTopRow + threadIdx.x] = mx;
+  }
+  cluster.sync();  // nobody's shared memory goes before it is read
 }
 
 // Rows of f32 (or, beside an f32 result, f16) as two f16 halves, high ones first.  n: values / 8.
@@ -946,8 +1051,8 @@ int launch_q(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows
 }  // namespace
 
 // Page boxes of at least 8 positions keep the 128-byte swizzle's pattern.
-bool paged_tc_supported(int mode, uint32_t D, uint32_t G, uint32_t page_size) {
-  return G <= kM && page_size % 8 == 0 && (D == 128 || D == 256) && (mode == BG_KV_F16 || mode == BG_KV_Q8);
+bool paged_tc_supported(int mode, uint32_t D, uint32_t G, uint32_t KV, uint32_t page_size) {
+  return G <= kM && KV <= 65535 && page_size % 8 == 0 && (D == 128 || D == 256) && (mode == BG_KV_F16 || mode == BG_KV_Q8);
 }
 
 // Rows of a unit: whole tokens' heads, two query tiles where there are rows for them and memory for both (f16
@@ -971,6 +1076,25 @@ int launch_paged_split_rows(const PagedAttnArgs &a, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, split_rows_kernel, a.q, a.q_f16, static_cast<uint4 *>(a.q_halves), n) == cudaSuccess
              ? BG_OK
              : BG_ELAUNCH;
+}
+
+int launch_paged_top_scales(const PagedAttnArgs &a, uint32_t rows_lo, bool own, bool prefix, cudaStream_t st) {
+  const uint32_t first = own ? 0 : a.bv.B, end = a.bv.B + (prefix ? 1 : 0);
+  for (uint32_t l = first; l < end; l += 65535) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kParts, a.kv.KV, end - l < 65535 ? end - l : 65535);
+    cfg.blockDim = dim3(512);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = a.D == 128 ? cudaLaunchKernelEx(&cfg, top_scales_kernel<4>, a, rows_lo, l)
+                                     : cudaLaunchKernelEx(&cfg, top_scales_kernel<8>, a, rows_lo, l);
+    if (e != cudaSuccess) return BG_ELAUNCH;
+  }
+  return BG_OK;
 }
 
 int launch_paged_tc(const PagedAttnArgs &a, uint32_t blocks, uint32_t ru, uint32_t rows_lo, bool prefix, cudaStream_t st) {

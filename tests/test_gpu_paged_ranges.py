@@ -65,15 +65,9 @@ def check(r, got, want, q_dtype, extra=0.0):
     assert (err <= tol).all(), f"error {float((err / (out.abs() + 1e-300)).max()):.3g} relative, {float((err / tol).max()):.3g} of what is allowed"
 
 
-# ---- long runs of one accumulator ----------------------------------------------------------------
-@pytest.mark.parametrize("mode", ["f16", "q8"])
-@pytest.mark.parametrize("D", [128, 256])
-@pytest.mark.parametrize("length", [2000, 9000, 40000, 120000])
-def test_long_units(ops, mode, D, length):  # noqa: F811
-    """Units that stay whole over many tiles, values of one sign: the error of f32 rows does not grow with the
-    length.  A run of matrix products into one accumulator has at most 64 steps, each of which may drop less than
-    2^-23 of what has been added up; the parts of equal steps add up to 33 / 64 of that: 64 * 2^-24 in all, beside
-    the tolerance's other terms."""
+def long_batch(ops, mode, D, length, io, drift=False):  # noqa: F811
+    """40 sequences of 20 tokens over the same ``length`` positions, V of one sign: (got, check(tolerance factor))."""
+    from bitgpu_b200._lib import lib
     KV, G, n, B = 8, 4, 20, 40
     H, page = KV * G, 64
     pages = -(-length // page)
@@ -85,6 +79,10 @@ def test_long_units(ops, mode, D, length):  # noqa: F811
         K, V = kv[0].view(-1, KV, D)[:length].double(), kv[1].view(-1, KV, D)[:length].double()
     else:
         sc = [torch.rand(shape[:3] + (D // 32,), generator=g, device="cuda") + s for s in (0.5, 1.0)]
+        if drift:
+            pos = torch.arange(pages * page, device="cuda").view(pages, page, 1, 1)
+            sc[0] *= torch.exp2(torch.round(3 * torch.sin(pos / 900.0)) - 2)
+            sc[1] *= torch.exp2(torch.round(10 * torch.cos(pos / 700.0 + torch.arange(D // 32, device="cuda"))))
         kv = [torch.randint(-127, 128, shape, generator=g, device="cuda", dtype=torch.int8),
               torch.randint(100, 128, shape, generator=g, device="cuda", dtype=torch.int8), *sc]
         K, V = ((kv[i].double() / 127 * sc[i].double().repeat_interleave(32, -1)).view(-1, KV, D)[:length] for i in (0, 1))
@@ -92,9 +90,8 @@ def test_long_units(ops, mode, D, length):  # noqa: F811
     table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(B, pages).contiguous()
     lens = torch.full((B,), length, dtype=torch.int32, device="cuda")
     cu = torch.arange(0, n * B + 1, n, dtype=torch.int32, device="cuda")
-    q = (torch.randn((n * B, H, D), generator=g, device="cuda") * 0.05)
-    got = ops.paged_attention(q, cache, ops.PagedBatch(table, lens, cu, n * B, n))
-    from bitgpu_b200._lib import lib
+    q = (torch.randn((n * B, H, D), generator=g, device="cuda") * 0.05).to(DT[io])
+    got = ops.paged_attention(q, cache, ops.PagedBatch(table, lens, cu, n * B, n), out_dtype=DT[io])
     assert lib().bg_device_status(None) == 0
     worst = 0.0
     for b, i in ((0, 0), (17, 19), (39, 7)):
@@ -105,6 +102,115 @@ def test_long_units(ops, mode, D, length):  # noqa: F811
             s = qq @ K[:m, k].T * D ** -0.5
             S = float((qq.abs() @ K[:m, k].abs().T).max()) * D ** -0.5
             w = torch.softmax(s, -1) @ V[:m, k]
-            err = (got[t].view(KV, G, D)[k].double() - w).abs() / ((28 * S + 16 + 64) * 2.0 ** -24 * w)
-            worst = max(worst, float(err.max()))
+            # f32 rows: 64 steps of a run; f16 rows: 512, beside two roundings to f16
+            tol = (28 * S + 16 + 64) * 2.0 ** -24 * w if io == "f32" else (28 * S + 16 + 512) * 2.0 ** -24 * w + 2.0 ** -10 * w
+            worst = max(worst, float(((got[t].view(KV, G, D)[k].double() - w).abs() / tol).max()))
     assert worst <= 1, f"{worst:.3g} of what is allowed"
+
+
+# ---- q8 block scales -----------------------------------------------------------------------------
+@each_kernel
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("vs", [1e-20, 1e-6, 1e-4, 1e-2, 1e3, 1e6, 1e20])
+def test_value_scales(ops, kernel, D, vs):  # noqa: F811
+    """V of any magnitude is read to the same relative error, f32 rows."""
+    r = make(kernel, D=D)
+    rescale(r, 1, vs)
+    q = r.queries(torch.float32)
+    check(r, attend(ops, kernel, r, q, torch.float32), r.attention(q), torch.float32)
+
+
+@each_kernel
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("vs", [1e-3, 1e-1, 1e1, 1e3])
+def test_value_scales_f16(ops, kernel, D, vs):  # noqa: F811
+    r = make(kernel, D=D)
+    rescale(r, 1, vs)
+    q = r.queries(torch.float16)
+    check(r, attend(ops, kernel, r, q, torch.float16), r.attention(q), torch.float16)
+
+
+@each_kernel
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("by", ["block", "position", "both"])
+def test_mixed_value_scales(ops, kernel, D, by):  # noqa: F811
+    """Block scales that differ by up to ten decimal orders between channels, and by three between positions.
+    The largest of a channel's scales sets the step of the others: f16 halves of at most 2^15 end at 2^-24, so
+    that a value (or a weight times a scale) is off by at most 2^-25 / 2^13 = 2^-38 of the largest scale."""
+    r = make(kernel, D=D)
+    g = torch.Generator().manual_seed(5)
+    n, nb = r.values[1].shape[0], D // 32
+    f = torch.ones(n, r.KV, nb, dtype=torch.float64)
+    if by != "position":
+        f = f * 10.0 ** torch.linspace(-8, 2, nb, dtype=torch.float64)
+    if by != "block":
+        f = f * 10.0 ** (3 * torch.rand((n, r.KV, nb), generator=g, dtype=torch.float64) - 1.5)
+    rescale(r, 1, f)
+    q = r.queries(torch.float32)
+    top = torch.stack([r.kv(b)[1].abs().amax(0) for b in range(3)]).amax(0).view(r.KV, nb, 32).amax(-1, keepdim=True)
+    top = top.expand(r.KV, nb, 32).reshape(r.KV, 1, D).expand(r.KV, r.G, D).reshape(r.H, D)
+    check(r, attend(ops, kernel, r, q, torch.float32), r.attention(q), torch.float32, extra=max(r.lens) * 2.0 ** -38 * top)
+
+
+@each_kernel
+@pytest.mark.parametrize("mode_order", ["rising", "falling"])
+def test_value_scales_along_a_sequence(ops, kernel, mode_order):  # noqa: F811
+    """Scales that grow (or shrink) by a factor of two every 64 positions, over 2^31 in all."""
+    r = make(kernel, lens=(2000, 64, 130))
+    f = torch.ones(r.values[1].shape[0], dtype=torch.float64)
+    for b, n in enumerate(r.lens):
+        e = torch.arange(n) // 64 - 16.0
+        f[r.rows(b, n)] = 2.0 ** (e if mode_order == "rising" else -e).double()
+    rescale(r, 1, f[:, None, None])
+    q = r.queries(torch.float32)
+    top = torch.stack([r.kv(b)[1].abs().amax() for b in range(3)]).amax()
+    check(r, attend(ops, kernel, r, q, torch.float32), r.attention(q), torch.float32, extra=float(2000 * 2.0 ** -38 * top))
+
+
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("io", ["f32", "f16"])
+@pytest.mark.parametrize("length", [700, 5000, 40001])
+def test_drifting_scales_of_long_units(ops, D, io, length):  # noqa: F811
+    """Units of many tiles whose K scales rise and fall by 2^6 and V scales by 2^20, each block in its own time."""
+    long_batch(ops, "q8", D, length, io, drift=True)
+
+
+@each_kernel
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("ks", [1e-20, 1e-6, 1e-4, 1e3, 1e6, 1e20])
+@pytest.mark.parametrize("io", ["f32", "f16"])
+def test_key_scales(ops, kernel, D, ks, io):  # noqa: F811
+    """K of any magnitude, with the softmax scale that such keys need."""
+    r = make(kernel, D=D)
+    rescale(r, 0, ks)
+    q = r.queries(DT[io])
+    sc = 1 / (ks * math.sqrt(D))
+    check(r, attend(ops, kernel, r, q, DT[io], scale=sc), r.attention(q, None, sc), DT[io])
+
+
+@each_kernel
+@pytest.mark.parametrize("D", [128, 256])
+def test_mixed_key_scales(ops, kernel, D):  # noqa: F811
+    r = make(kernel, D=D)
+    g = torch.Generator().manual_seed(6)
+    rescale(r, 0, 10.0 ** (5 * torch.rand((r.values[0].shape[0], r.KV, D // 32), generator=g, dtype=torch.float64) - 4.5))
+    q = r.queries(torch.float32)
+    check(r, attend(ops, kernel, r, q, torch.float32), r.attention(q), torch.float32)
+
+
+# ---- long runs of one accumulator ----------------------------------------------------------------
+@pytest.mark.parametrize("mode", ["f16", "q8"])
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("length", [2000, 9000, 40000, 120000])
+def test_long_units(ops, mode, D, length):  # noqa: F811
+    """Units that stay whole over many tiles, values of one sign: the error of f32 rows does not grow with the
+    length.  A run of matrix products into one accumulator has at most 64 steps, each of which may drop less than
+    2^-23 of what has been added up; the parts of equal steps add up to 33 / 64 of that: 64 * 2^-24 in all, beside
+    the tolerance's other terms."""
+    long_batch(ops, mode, D, length, "f32")
+
+
+@pytest.mark.parametrize("mode", ["f16", "q8"])
+@pytest.mark.parametrize("D", [128, 256])
+def test_long_units_f16(ops, mode, D):  # noqa: F811
+    long_batch(ops, mode, D, 60000, "f16")
