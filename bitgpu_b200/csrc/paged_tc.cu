@@ -141,12 +141,13 @@ __device__ __forceinline__ uint32_t top_scale(const PagedAttnArgs &a, const Piec
 // c' mh - hi is exact in f16, so  lo = c' ml + (c' mh - hi)  carries the rest, to 2^-22 of the value or half of f16's
 // smallest step: 2^-25.
 struct CodeScale {
-  __half2 p2, bias, mh, ml;
+  __half2 p2, bias, least, mh, ml;
   __device__ __forceinline__ explicit CodeScale(float x) {
     const int e = min(4, max(-20, (int)((__float_as_uint(x) >> 23) & 255) - 127));
     const float m = x * __uint_as_float((uint32_t)(127 - e) << 23), f = __uint_as_float((uint32_t)(127 + e) << 23);
     p2 = __float2half2_rn(f);
     bias = __float2half2_rn(-1152.0f * f);
+    least = __float2half2_rn(-127.0f * f);  // code -128 stands for -1 too
     mh = __float2half2_rn(m);
     ml = __float2half2_rn(m - __low2float(mh));
   }
@@ -156,7 +157,7 @@ struct CodeScale {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint32_t x = __byte_perm(b, 0x64646464u, i ? 0x4342 : 0x4140);
-      const __half2 c = __hfma2(*reinterpret_cast<const __half2 *>(&x), p2, bias);
+      const __half2 c = __hmax2(__hfma2(*reinterpret_cast<const __half2 *>(&x), p2, bias), least);
       const __half2 h = __hmul2(c, mh), r = __hfma2(c, mh, __hneg2(h)), l = __hfma2(c, ml, r);
       (i ? h1 : h0) = *reinterpret_cast<const uint32_t *>(&h);
       (i ? l1 : l0) = *reinterpret_cast<const uint32_t *>(&l);

@@ -198,6 +198,21 @@ def test_mixed_key_scales(ops, kernel, D):  # noqa: F811
     check(r, attend(ops, kernel, r, q, torch.float32), r.attention(q), torch.float32)
 
 
+# ---- q8 codes ------------------------------------------------------------------------------------
+@each_kernel
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("io", ["f32", "f16"])
+def test_every_code(ops, kernel, D, io):  # noqa: F811
+    """Codes from -128 on: code -128 stands for -1, as -127 does."""
+    r = make(kernel, D=D)
+    for d in r.data:
+        d.copy_(torch.randint(-128, 128, d.shape, generator=r.g))
+        d[torch.rand(d.shape, generator=r.g) < 0.3] = -128
+    revalue(r)
+    q = r.queries(DT[io], 0.5)
+    check(r, attend(ops, kernel, r, q, DT[io]), r.attention(q), DT[io])
+
+
 # ---- long runs of one accumulator ----------------------------------------------------------------
 @pytest.mark.parametrize("mode", ["f16", "q8"])
 @pytest.mark.parametrize("D", [128, 256])
