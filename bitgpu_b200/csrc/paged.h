@@ -298,6 +298,13 @@ struct PieceWalk {
   }
 };
 
+// The power of two that values below 2^(x + 1) are freed of to stay below 2^14 (x: the exponent in `bits`; at least
+// 2^-126), and its inverse.
+__device__ __forceinline__ float pow2_of(uint32_t bits) {
+  return __uint_as_float((uint32_t)max((int)(bits & 0x7f800000u) - (13 << 23), 1 << 23));
+}
+__device__ __forceinline__ float pow2_inv(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
+
 // Where a unit's rows wait to be joined.  Without a prefix only cut units leave any: one CutUnit per
 // block (npieces 0: none).  With a prefix every row joins two lists of pieces: one RowPieces per (kv
 // head, R) and part; piece 0 is partial row idx0, piece k row idx0 + (2k - 1) * step.
@@ -357,7 +364,9 @@ struct PagedAttnArgs {
   uint32_t H, G, D, max_q;
   float sl2;  // softmax scale * log2(e)
   const void *q;
-  void *q_halves;  // tcgen05 kernels, rows that are not f16 in and out: q as two f16 halves [2][T][H][D]
+  // tcgen05 kernels, rows that are not f16 in and out: q as two f16 halves [2][T][H][D] and each row's power of two
+  void *q_halves;
+  float *q_pow2;  // [T][H]
   const float *gate;
   void *out;
   // partial rows: o [n][D] unnormalised, ml [n] (running max in log2 units, sum); n = part_rows

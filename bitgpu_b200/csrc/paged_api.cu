@@ -42,7 +42,7 @@ constexpr uint64_t kManyTiles = 8;
 
 // The kernels of one call and the layout of its workspace: partial rows o [part_rows][D] f32, then ml
 // [part_rows] float2, then the descriptions of what is to be joined, then (tcgen05) the blocks' run sums, the
-// largest block scales of a q8 pool and the halves of f32 rows.
+// largest block scales of a q8 pool, the halves of f32 rows and their powers of two.
 //   join        a shared prefix: every row joins its parts
 //   tc_pre      the prefix's units run on tcgen05
 //   tc_own      sequences of more than 16 rows run on tcgen05
@@ -118,7 +118,7 @@ Plan make_plan(const bg_paged_cache *kv, const bg_paged_batch *b, uint32_t H, ui
     }
     if (lo) {
       p.halves = p.bytes;
-      p.bytes += p.rows * D * 4;
+      p.bytes += p.rows * (D * 4 + 4);
     }
   }
   return p;
@@ -228,7 +228,10 @@ int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, ui
   CutUnit *cuts = reinterpret_cast<CutUnit *>(desc);
   if (plan.sums) a.run_sums = reinterpret_cast<float4 *>(static_cast<unsigned char *>(workspace) + plan.sums);
   if (plan.tops) a.tops = reinterpret_cast<uint32_t *>(static_cast<unsigned char *>(workspace) + plan.tops);
-  if (plan.halves) a.q_halves = static_cast<unsigned char *>(workspace) + plan.halves;
+  if (plan.halves) {
+    a.q_halves = static_cast<unsigned char *>(workspace) + plan.halves;
+    a.q_pow2 = reinterpret_cast<float *>(static_cast<unsigned char *>(workspace) + plan.halves + plan.rows * D * 4);
+  }
   if (plan.join) {
     a.own_pieces = reinterpret_cast<RowPieces *>(desc);
     a.pre_pieces = a.own_pieces + plan.rows;

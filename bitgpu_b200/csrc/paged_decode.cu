@@ -14,7 +14,8 @@
 //   * four consumer warps take 16 positions of a tile each.  Scores are computed transposed (m16n8k16
 //     with positions on M, up to 8 query rows on N), and so is the output, O^T = V^T P^T; P reaches the
 //     B operand in registers through movmatrix;
-//   * f32 rows (LO): q and p are split into two f16 operands (22 bits).  Up to four rows a unit (PK; one
+//   * f32 rows (LO): q, without the power of two of its row's largest value (which the softmax scale puts back), and p
+//     are split into two f16 operands (22 bits).  Up to four rows a unit (PK; one
 //     token of a group of four heads) the halves share one product, hi in columns 0-3 and lo in 4-7 of the
 //     MMA's eight; otherwise both products run twice.  f16 rows: q is exact and p is rounded once to f16,
 //     which costs about as much as the rounding of the result.  p carries a factor 2^14, which cancels in the
@@ -283,10 +284,25 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
     // Q^T operand fragments (B of m16n8k16): column n = lane / 4, k pairs
     uint32_t qh[NT][KS][2], ql[TWO ? NT : 1][TWO ? KS : 1][2];
     int32_t lim[NT][2];  // last attended position of the lane's score columns
+    float sl[NT][2];     // and their softmax scale, times their row's power of two
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const uint32_t r = PK ? (lane >> 2) & 3 : nt * 8 + (lane >> 2);
       const unsigned char *qr = smem + C::oQ + us * C::QSLOT + r * (a.q_f16 ? D * 2 + 16 : C::QROW);
+      float pow2 = 1.f, inv = 1.f;  // of the row's values
+      if (LO && !a.q_f16) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {  // four lanes have a quarter each
+          const uint4 v = *reinterpret_cast<const uint4 *>(qr + (4 * i + (lane & 3)) * 16);
+          constexpr uint32_t abs = 0x7fffffffu;
+          top = max(top, max(max(v.x & abs, v.y & abs), max(v.z & abs, v.w & abs)));
+        }
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        pow2 = pow2_of(top);
+        inv = pow2_inv(pow2);
+      }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
@@ -298,7 +314,9 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
             qh[nt][ks][half] = PK && lane >= 16 ? 0u : *reinterpret_cast<const uint32_t *>(qr + d * 2);
             if constexpr (TWO) ql[nt][ks][half] = 0;
           } else {
-            const float2 v = *reinterpret_cast<const float2 *>(qr + d * 4);
+            float2 v = *reinterpret_cast<const float2 *>(qr + d * 4);
+            v.x *= inv;
+            v.y *= inv;
             const uint32_t h = pack_f16(v.x, v.y);
             qh[nt][ks][half] = h;
             if constexpr (LO) {
@@ -313,6 +331,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint32_t col = nt * 8 + 2 * (lane & 3) + j, rc = min(PK ? col & 3 : col, ui.rows - 1);
+        sl[nt][j] = LO ? sl2 * __shfl_sync(0xffffffffu, pow2, 8 * (lane & 3) + 4 * j) : sl2;
         lim[nt][j] = min(ui.lim_base + (int32_t)((ui.R0 + rc) / a.G), (int32_t)ui.len - 1);
       }
     }
@@ -364,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            sc[nt][i] = (acc[nt][i] + acl[nt][i]) * sl2;
+            sc[nt][i] = (acc[nt][i] + acl[nt][i]) * sl[nt][i & 1];
             if constexpr (PK) sc[nt][i] += __shfl_xor_sync(0xffffffffu, sc[nt][i], 2);
           }
       } else {
@@ -387,8 +406,8 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           for (int i = 0; i < 4; ++i) r[i] ^= 0x80808080u;
           const uint32_t a0[4] = {code(r[0], kSelLo), code(r[1], kSelLo), code(r[0], kSelHi), code(r[1], kSelHi)};
           const uint32_t a1[4] = {code(r[2], kSelLo), code(r[3], kSelLo), code(r[2], kSelHi), code(r[3], kSelHi)};
-          const float sa = ksc[(row0 + (lane >> 2)) * NB + bk] * (sl2 * (1.0f / 127.0f));
-          const float sb = ksc[(row0 + (lane >> 2) + 8) * NB + bk] * (sl2 * (1.0f / 127.0f));
+          const float sa = ksc[(row0 + (lane >> 2)) * NB + bk] * (LO ? 1.0f / 127.0f : sl2 * (1.0f / 127.0f));
+          const float sb = ksc[(row0 + (lane >> 2) + 8) * NB + bk] * (LO ? 1.0f / 127.0f : sl2 * (1.0f / 127.0f));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -403,6 +422,12 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
             sc[nt][2] = fmaf(acc[2], sb, sc[nt][2]);
             sc[nt][3] = fmaf(acc[3], sb, sc[nt][3]);
           }
+        }
+        if constexpr (LO) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[nt][i] *= sl[nt][i & 1];
         }
         if constexpr (PK) {
 #pragma unroll

@@ -17,7 +17,8 @@
 //
 // Precision, by the types of the call:
 //   f16 rows, f16 pool: operands are exact, P is rounded once to f16 (kept 2^6 up, away from subnormals);
-//   f32 rows (LO): q and p are split into two f16 halves (22 bits) -- two products for S, two for O; weights
+//   f32 rows (LO): q, without the power of two of its row's largest value, and p are split into two f16 halves (22
+//           bits) -- two products for S, two for O; the softmax scale gives each row its power back; weights
 //           below 2^-31 of a row's largest fall under f16's smallest step and are lost;
 //   q8 pool: code * scale has more than 11 bits, so K and V are split too when they are dequantised into
 //           the operand tiles: one more product each.  (A single f16 rounding of K and V would double the
@@ -72,7 +73,7 @@ struct TcCfg {
   static constexpr int LEAD = Q8 ? 2 : 1;                    // a unit's own cost, in tiles
   static constexpr int NST = D == 256 && Q8 && LO ? 1 : 2;   // ring stages of K and of V
   static constexpr int oQ = 0, oK = NQT * NQ * QT, oV = oK + NST * NK * KVT, oB = oV + NST * NK * KVT;
-  static constexpr int oInfo = oB + 384, oVP = oInfo + 64, oML = oVP + 64, oScan = oML + kM * 8;
+  static constexpr int oInfo = oB + 384, oVP = oInfo + 64, oQP = oVP + 64, oML = oQP + 2 * kM * 4, oScan = oML + kM * 8;
   static constexpr int SMEM = oScan + 24 * 8;
   // a stream's tiles in one accumulator run: at most 64 MMAs for f32 rows (3e-6), 512 for f16 rows (2.5e-5, a
   // twentieth of the result's rounding)
@@ -120,13 +121,6 @@ __device__ __forceinline__ void split8(const float (&x)[8], uint4 &hi, uint4 &lo
   hi = make_uint4(h[0], h[1], h[2], h[3]);
   lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
-
-// The power of two that values below 2^(x + 1) are freed of to stay below 2^14 (x: the exponent in `bits`; at least
-// 2^-126), and its inverse.
-__device__ __forceinline__ float pow2_of(uint32_t bits) {
-  return __uint_as_float((uint32_t)max((int)(bits & 0x7f800000u) - (13 << 23), 1 << 23));
-}
-__device__ __forceinline__ float pow2_inv(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
 
 // Largest block scales (as bits, which order like the magnitudes) of each page list and kv head: V's blocks, K's at
 // kTopK.
@@ -258,6 +252,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   uint32_t *tmem_at = reinterpret_cast<uint32_t *>(bars + 35);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(bars + 36);
   TcInfo *info = reinterpret_cast<TcInfo *>(smem + C::oInfo);
+  volatile float *q_pow2 = reinterpret_cast<float *>(smem + C::oQP);  // [2][kM], by piece (f32 rows)
   volatile float *v_pow2 = reinterpret_cast<float *>(smem + C::oVP);  // [2][8], by piece (q8 pool)
   float2 *ml_s = reinterpret_cast<float2 *>(smem + C::oML);
   const PagedAttnArgs &a = p.a;
@@ -510,6 +505,14 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         const bool more = walk.next(pc, a.bv, p.u, ps);
         uint32_t top = 0;
         if (Q8 && more && gt <= kTopK) top = top_scale(a, pc, gt);
+        float qp[4];  // warp 2: of the piece's rows
+        if (LO && more && warp == 2) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t R = pc.R0 + min(lane + 32u * i, pc.rows - 1);
+            qp[i] = __ldcg(a.q_pow2 + (uint64_t)(R / a.G) * a.H + pc.kvh * a.G + R % a.G);
+          }
+        }
         if (piece > 0) {
           ok = mbar_wait_warp(q_free, (piece - 1) & 1) && mbar_wait_warp(info_free, (piece - 1) & 1);
           if (!ok || __any_sync(0xffffffffu, *abort_flag != 0)) break;
@@ -544,8 +547,12 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
         if constexpr (Q8) {
           if (gt < kTopK) v_pow2[(piece & 1) * 8 + gt] = pow2_of(top);
           if (gt == kTopK) info->k_pow2 = pow2_of(top);
-          __syncwarp();
         }
+        if (LO && warp == 2) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q_pow2[(piece & 1) * kM + lane + 32 * i] = qp[i];
+        }
+        __syncwarp();
         // rows come by TMA as boxes of whole tokens' heads; tokens behind the unit's are other sequences' (or
         // zeros) and the tile's last rows stay as they were: computed along, never written
         loaded = piece + 1;
@@ -596,7 +603,8 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
           for (int i = 0; i < D / 32; ++i) asm volatile("prefetch.global.L2 [%0];" ::"l"(g + 32 * i));
         }
         // (never so small that a masked score times it is not -infinity)
-        if constexpr (Q8) sl2 = fmaxf(a.sl2 * in.k_pow2, 0x1p-126f);
+        if constexpr (LO || Q8)
+          sl2 = fmaxf(a.sl2 * (LO ? q_pow2[(piece & 1) * kM + row] : 1.f) * (Q8 ? in.k_pow2 : 1.f), 0x1p-126f);
         float m_used = kNegBig, l = 0.f;
         float m_sum = kNegBig;     // what the run sum's weights refer to
         bool summed = false;       // whether there is one (the same for the whole stream)
@@ -971,20 +979,33 @@ __global__ void __cluster_dims__(kParts, 1, 1) __launch_bounds__(512)
   cluster.sync();  // nobody's shared memory goes before it is read
 }
 
-// Rows of f32 (or, beside an f32 result, f16) as two f16 halves, high ones first.  n: values / 8.
+// Rows of f32 (or, beside an f32 result, f16) as two f16 halves, high ones first, of the row without the power of two
+// that its largest value asks for (f32 holds values that f16 does not).  n: values / 8, lpr: a row's (16 or 32 lanes).
 // One pass for all kv heads' units, which then fetch their tiles by TMA: loaded and split by two warps of
 // the attention kernel, a unit's rows took 8 us at head_dim 128.
-__global__ void __launch_bounds__(256) split_rows_kernel(const void *q, int q_f16, uint4 *halves, uint64_t n) {
+__global__ void __launch_bounds__(256) split_rows_kernel(const void *q, int q_f16, uint4 *halves, float *pow2, uint64_t n, uint32_t lpr) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const uint64_t step = (uint64_t)gridDim.x * 256;
-  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += step) {
-    float x[8];
-    if (q_f16) load_f16<8>(static_cast<const __half *>(q) + i * 8, x);
-    else load_f32<8>(static_cast<const float *>(q) + i * 8, x);
+  const uint32_t lane = threadIdx.x & 31;
+  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i - lane < n; i += step) {  // (the same for a whole warp)
+    float x[8] = {};
+    if (i < n) {
+      if (q_f16) load_f16<8>(static_cast<const __half *>(q) + i * 8, x);
+      else load_f32<8>(static_cast<const float *>(q) + i * 8, x);
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+    for (uint32_t m = lpr >> 1; m > 0; m >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, m));
+    const float p = pow2_of(top), inv = pow2_inv(p);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] *= inv;
+    if (i >= n) continue;
     uint4 hi, lo;
     split8(x, hi, lo);
     halves[i] = hi;
     halves[n + i] = lo;
+    if (lane % lpr == 0) pow2[i / lpr] = p;
   }
 }
 
@@ -1074,7 +1095,8 @@ int launch_paged_split_rows(const PagedAttnArgs &a, cudaStream_t st) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, split_rows_kernel, a.q, a.q_f16, static_cast<uint4 *>(a.q_halves), n) == cudaSuccess
+  return cudaLaunchKernelEx(&cfg, split_rows_kernel, a.q, a.q_f16, static_cast<uint4 *>(a.q_halves), a.q_pow2, n, a.D / 8) ==
+                 cudaSuccess
              ? BG_OK
              : BG_ELAUNCH;
 }

@@ -213,6 +213,47 @@ def test_every_code(ops, kernel, D, io):  # noqa: F811
     check(r, attend(ops, kernel, r, q, DT[io]), r.attention(q), DT[io])
 
 
+# ---- f32 queries ---------------------------------------------------------------------------------
+@each_kernel
+@pytest.mark.parametrize("mode", ["f16", "q8"])
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("qs", [1e-20, 1e-8, 1e-4, 1e5, 1e20])
+def test_query_scales(ops, kernel, mode, D, qs):  # noqa: F811
+    """f32 queries of any magnitude, with the softmax scale that such queries need."""
+    r = make(kernel, mode, D)
+    q = r.queries(torch.float32, 1.5 * qs)
+    sc = 1 / (qs * math.sqrt(D))
+    for out in DT.values():
+        check(r, attend(ops, kernel, r, q, out, scale=sc), r.attention(q, None, sc), torch.float32)
+
+
+@each_kernel
+@pytest.mark.parametrize("mode", ["f16", "q8"])
+def test_mixed_query_scales(ops, kernel, mode):  # noqa: F811
+    """Rows of one unit that differ by twelve decimal orders, zero rows among them; a row's error is its own."""
+    r = make(kernel, mode)
+    q = r.queries(torch.float32)
+    g = torch.Generator().manual_seed(7)
+    q *= 10.0 ** (12 * torch.rand((r.T, r.H, 1), generator=g) - 6)
+    q[0, 1] = 0
+    got = attend(ops, kernel, r, q, torch.float32, scale=1e-5)
+    for t in range(r.T):
+        for h in range(r.H):
+            one = torch.zeros_like(q)
+            one[t, h] = q[t, h]
+            b = max(i for i in range(3) if r.cu[i] <= t)
+            if t not in (0, r.T - 1) and h % 3:
+                continue
+            K, V = r.kv(b)
+            m = r.lens[b] - r.news[b] + t - r.cu[b] + 1
+            k, v, qq = K[:m, h // r.G], V[:m, h // r.G], q[t, h].double()
+            s = k @ qq * 1e-5
+            p = torch.softmax(s, 0)
+            S = float((k.abs() @ qq.abs()).max()) * 1e-5
+            tol = tolerance(p @ v, p @ v.abs(), S, False, False) + 2.0 ** -31 * v.abs().sum(0)
+            assert ((got[t, h].double() - p @ v).abs() <= tol).all(), (t, h)
+
+
 # ---- long runs of one accumulator ----------------------------------------------------------------
 @pytest.mark.parametrize("mode", ["f16", "q8"])
 @pytest.mark.parametrize("D", [128, 256])
