@@ -21,10 +21,18 @@ struct BatchView {
 };
 
 // Tokens [begin, end) of sequence b.  Device-side values are never trusted to be in range: offsets
-// are clamped to [0, T], lengths to what the sequence's page-table row can hold.
+// are clamped to [0, T], lengths to what the sequence's page-table row can hold -- but a token's position follows
+// from the length as it was given, as in the append.
 struct SeqRange {
   uint32_t begin, n;  // first token, number of tokens
   int32_t len;        // own positions, the new tokens among them
+  int32_t held;       // those that the page table has room for
+  // Own positions that token i of the sequence attends.
+  __device__ __forceinline__ int32_t attended(uint32_t i) const {
+    return min(held, max(0, len - (int32_t)n + (int32_t)i + 1));
+  }
+  // The page table has no room for the length: reported as BG_EINVAL.
+  __device__ __forceinline__ bool too_long() const { return n > 0 && held < len; }
 };
 
 __device__ __forceinline__ SeqRange seq_range(const BatchView &bv, uint32_t b, uint32_t page_size) {
@@ -38,7 +46,8 @@ __device__ __forceinline__ SeqRange seq_range(const BatchView &bv, uint32_t b, u
     r.begin = b;
     r.n = 1;
   }
-  r.len = min(max(__ldg(bv.kv_len + b), 0), (int32_t)(bv.table_stride * page_size));
+  r.len = max(__ldg(bv.kv_len + b), 0);
+  r.held = min(r.len, (int32_t)(bv.table_stride * page_size));
   return r;
 }
 
@@ -108,8 +117,7 @@ inline uint64_t most_tiles(const UnitShape &u, uint64_t tokens, uint64_t batch, 
 // Positions that the last row of chunk ch attends (own part of a sequence), and the chunk's tiles.
 __device__ __forceinline__ uint32_t chunk_tiles(const SeqRange &s, const UnitShape &u, uint32_t ch) {
   const uint32_t end = u.tokens ? min((ch + 1) * u.tokens, s.n) : (min((ch + 1) * u.RU, s.n * u.G) - 1) / u.G + 1;
-  const int32_t m = min(s.len, max(0, s.len - (int32_t)s.n + (int32_t)end));
-  return max(1u, ((uint32_t)m + u.KT - 1) >> u.shift);
+  return max(1u, ((uint32_t)s.attended(end - 1) + u.KT - 1) >> u.shift);
 }
 
 // Tiles of one kv head of a sequence's own units, their leads among them (0: none of this kernel's).
@@ -127,11 +135,11 @@ __device__ __forceinline__ uint32_t batch_rows(const BatchView &bv, uint32_t G) 
   return (uint32_t)min(max(t, 0), (int32_t)bv.T) * G;
 }
 
-// All NTHR threads of the block: the block's span.  `sh`: NTHR / 32 + 2 words of shared memory.  Tile
+// All NTHR threads of the block: the block's span; `bad` is set where a length exceeds its table.  `sh`: NTHR / 32 + 2 words of shared memory.  Tile
 // numbers have 32 bits: most_tiles() of the call's bounds says whether that is enough.
 template <int NTHR>
 __device__ __forceinline__ TileSpan block_span(const BatchView &bv, const UnitShape &u, uint32_t page_size,
-                                               uint32_t min_tiles, uint32_t *sh) {
+                                               uint32_t min_tiles, uint32_t *sh, int *bad) {
   constexpr int NW = NTHR / 32;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t per_thread = (bv.B + NTHR - 1) / NTHR;
@@ -139,7 +147,9 @@ __device__ __forceinline__ TileSpan block_span(const BatchView &bv, const UnitSh
   uint32_t mine = 0;
   uint32_t first = 0;
   for (uint32_t b = lo; b < hi; ++b) {
-    const uint32_t n = u.KV * seq_tiles(seq_range(bv, b, page_size), u);
+    const SeqRange sr = seq_range(bv, b, page_size);
+    if (sr.too_long() && blockIdx.x == 0) atomicExch(bad, BG_EINVAL);
+    const uint32_t n = u.KV * seq_tiles(sr, u);
     if (b == lo) first = n;
     mine += n;
   }
@@ -227,7 +237,7 @@ struct PieceWalk {
     pre = s.pre;
     b = s.b0;
     kvh = ch = in = 0;
-    sr = SeqRange{0, 0, 0};
+    sr = SeqRange{0, 0, 0, 0};
     if (cur < t1 && t1 > pre) seek(bv, u, page_size, s.off0);
   }
 
@@ -266,7 +276,7 @@ struct PieceWalk {
         p.kvh = kvh;
         p.R0 = sr.begin * u.G + ch * u.RU;
         p.rows = min(u.RU, rows - ch * u.RU);
-        p.len = (uint32_t)sr.len;
+        p.len = (uint32_t)sr.held;
         p.lim_base = sr.len - (int32_t)sr.n - (int32_t)sr.begin;
         p.pages = bv.table + (uint64_t)b * bv.table_stride;
         p.list = b;

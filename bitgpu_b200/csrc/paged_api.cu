@@ -139,11 +139,12 @@ size_t workspace_bytes_for(const bg_paged_cache *kv, const bg_paged_batch *b, ui
 
 namespace bg {
 int poll_device_error_paged() {
-  int e = poll_device_error_paged_append();
-  if (!e) e = poll_device_error_paged_generic();
-  if (!e) e = poll_device_error_paged_decode();
-  if (!e) e = poll_device_error_paged_tc();
-  return e;
+  // each one is read and cleared: several kernels of one call may have seen the same fault
+  const int e[] = {poll_device_error_paged_append(), poll_device_error_paged_generic(), poll_device_error_paged_decode(),
+                   poll_device_error_paged_tc()};
+  for (int i = 0; i < 4; ++i)
+    if (e[i]) return e[i];
+  return 0;
 }
 }  // namespace bg
 

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
     prefetch_tmap(&tmV);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const TileSpan span = block_span<kThreads>(a.bv, p.u, a.kv.page_size, a.min_tiles, scan);
+  const TileSpan span = block_span<kThreads>(a.bv, p.u, a.kv.page_size, a.min_tiles, scan, &g_device_error);
 
   if (warp == kConsumers) {  // ---------------- producer ----------------
     PieceWalk walk;

@@ -54,7 +54,8 @@ __global__ void __launch_bounds__(128) paged_generic_kernel(PagedAttnArgs a, uin
   if (b < 0) return;
   const SeqRange sr = seq_range(a.bv, b, a.kv.page_size);
   const uint32_t P = a.bv.prefix_len;
-  const int32_t own = min(sr.len, max(0, sr.len - (int32_t)sr.n + (int32_t)(t - sr.begin) + 1));
+  if (threadIdx.x == 0 && sr.too_long()) atomicExch(&g_generic_error, BG_EINVAL);
+  const int32_t own = sr.attended(t - sr.begin);
   const uint32_t total = P + (uint32_t)own;
   const uint32_t chunk = ((total + nsplit - 1) / nsplit + 31) / 32 * 32;
   const uint32_t lo = min(total, split * chunk), hi = min(total, lo + chunk);

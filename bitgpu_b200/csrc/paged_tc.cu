@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
   if (!Q8) asm volatile("griddepcontrol.wait;" ::: "memory");
   tc_fence_before();
   const TileSpan span = block_span<C::THREADS>(a.bv, p.u, a.kv.page_size, a.min_tiles,
-                                               reinterpret_cast<uint32_t *>(smem + C::oScan));
+                                               reinterpret_cast<uint32_t *>(smem + C::oScan), &g_device_error);
   if (Q8) asm volatile("griddepcontrol.wait;" ::: "memory");
   tc_fence_after();
   const uint32_t tmem = *tmem_at;
@@ -938,7 +938,7 @@ __global__ void __cluster_dims__(kParts, 1, 1) __launch_bounds__(512)
   if (list < a.bv.B) {
     const SeqRange sr = seq_range(a.bv, list, ps);
     pages = a.bv.table + (uint64_t)list * a.bv.table_stride;
-    len = sr.n * a.G > rows_lo ? (uint32_t)sr.len : 0;
+    len = sr.n * a.G > rows_lo ? (uint32_t)sr.held : 0;
   }
   constexpr uint32_t abs = 0x7fffffffu;
   uint32_t k = 0, v[NB];

@@ -221,7 +221,9 @@ int bg_qk_norm_rope(const float *x, uint32_t batch, uint32_t S, uint32_t heads, 
  *     Values below kv_len[b] are the caller's: a NaN or infinity there may also reach rows of the same
  *     sequence whose own position lies in front of it.
  *   - A page id outside the pool is never followed: attention reads zeros for it and the append drops
- *     the row, as it does where the page table is too narrow; bg_device_status then reports BG_EINVAL.
+ *     the row; bg_device_status then reports BG_EINVAL.
+ *   - A kv_len[b] beyond table_stride*page_size is reported in the same way.  Positions still follow from it: the
+ *     append drops the rows behind the table's end, attention attends the positions in front of it.
  * prefix_len + table_stride*page_size has to fit 31 bits. */
 typedef struct {
   void *K, *V;

@@ -254,6 +254,99 @@ def test_mixed_query_scales(ops, kernel, mode):  # noqa: F811
             assert ((got[t, h].double() - p @ v).abs() <= tol).all(), (t, h)
 
 
+# ---- lengths beyond the page table ---------------------------------------------------------------
+@each_kernel
+@pytest.mark.parametrize("mode", ["f16", "q8"])
+@pytest.mark.parametrize("prefix", [0, 40])
+def test_length_beyond_the_table(ops, kernel, mode, prefix):  # noqa: F811
+    """kv_len says more than the table holds: positions are what kv_len says, the append drops those that have no
+    page, attention reads those that have one, both report it, and the other sequences are served."""
+    from bitgpu_b200._lib import BG_EINVAL, lib
+    G, news = KERNELS[kernel]
+    KV, D, page, over = 2, 128, 16, 6
+    r = Ragged([128, 64, 130], news, KV=KV, G=G, D=D, mode=mode, prefix=prefix, seed=3)
+    width = 1 << 14 if kernel == "tc" else 9
+    cap = width * page
+    n = news[2]
+    table = torch.zeros(3, width, dtype=torch.int32)
+    table[:, :9] = r.table[:, :9].clamp(min=0)
+    # the last sequence fills its whole row of the table with one page, over and over
+    table[2] = r.table[2, 0]
+    kv_len = torch.tensor([128, 64, cap + over], dtype=torch.int32)
+    q = r.queries(torch.float32)
+    cache = r.cache(ops)
+    b = ops.PagedBatch(table.cuda(), kv_len.cuda(), torch.tensor(r.cu, dtype=torch.int32).cuda(), r.T, max(news),
+                       r.prefix_pages.cuda() if prefix else None, prefix)
+    lib().bg_force_generic(int(kernel == "cuda"))
+    try:
+        got = ops.paged_attention(q.cuda(), cache, b).cpu().double()
+    finally:
+        lib().bg_force_generic(0)
+    assert lib().bg_device_status(None) == BG_EINVAL
+    assert lib().bg_device_status(None) == 0
+    # the repeated page: attended floor(m / page) times whole, and its first m % page slots once more
+    first = r.table[2, 0].long() * page + torch.arange(page)
+    K, V = r.values[0][first], r.values[1][first]
+    if prefix:
+        pr = r.prefix_rows()
+        PK, PV = r.values[0][pr], r.values[1][pr]
+    r.lens[2] = page  # the oracle's own rows of the other sequences
+    r.news[2] = 0
+    out, A, S = r.attention(q)
+    r.news[2] = n
+    for i in range(n):
+        m = min(cap, cap + over - n + i + 1)
+        w = (torch.tensor(m // page) + (torch.arange(page) < m % page)).double()
+        qq = q[r.cu[2] + i].double().view(KV, G, D)
+        s = torch.einsum("kgd,jkd->kgj", qq, K) * D ** -0.5
+        S = max(S, float(torch.einsum("kgd,jkd->kgj", qq.abs(), K.abs()).max()) * D ** -0.5)
+        v, e = V, s + w.log()
+        if prefix:
+            e = torch.cat([torch.einsum("kgd,jkd->kgj", qq, PK) * D ** -0.5, e], -1)
+            v = torch.cat([PV, V])
+        p = torch.softmax(e, -1)
+        out[r.cu[2] + i] = torch.einsum("kgj,jkd->kgd", p, v).reshape(r.H, D)
+        A[r.cu[2] + i] = torch.einsum("kgj,jkd->kgd", p, v.abs()).reshape(r.H, D)
+    # (the tcgen05 kernel's accumulators run over the whole table here: its own test below bounds their error)
+    tol = tolerance(out, A, S, False, False) + 64 * 2.0 ** -24 * A
+    assert ((got - out).abs() <= tol).all(), float(((got - out).abs() / tol).max())
+
+
+@pytest.mark.parametrize("n", [1, 10, 40])
+def test_append_and_attend_beyond_the_table(ops, n):  # noqa: F811
+    """Four pages of 16, kv_len 70: the tokens at 60 to 63 are appended and attend up to themselves, the ones
+    behind attend what there is."""
+    from bitgpu_b200._lib import BG_EINVAL, lib
+    KV, G, D = 2, 4, 128
+    H = KV * G
+    torch.manual_seed(0)
+    for kind in ("cuda", "fast"):
+        cache = ops.PagedKVCache(6, 16, KV, D, "f16")
+        cache.K.normal_()
+        cache.V.normal_()
+        table = torch.tensor([[3, 0, 5, 1]], dtype=torch.int32).cuda()
+        b = ops.PagedBatch(table, torch.tensor([70], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(),
+                           n, n)
+        x = torch.randn(n, H + 2 * KV, D, device="cuda")
+        ops.paged_append(cache, b, x[:, H:H + KV], x[:, H + KV:])
+        assert lib().bg_device_status(None) == BG_EINVAL
+        lib().bg_force_generic(int(kind == "cuda"))
+        try:
+            got = ops.paged_attention(x[:, :H].contiguous(), cache, b).double()
+        finally:
+            lib().bg_force_generic(0)
+        assert lib().bg_device_status(None) == BG_EINVAL
+        K, V = (t[table[0].long()].view(64, KV, D).double() for t in (cache.K, cache.V))
+        for i in range(n):
+            m = min(64, 70 - n + i + 1)
+            if 70 - n + i < 64:
+                assert torch.equal(V[m - 1].half(), x[i, H + KV:].half())
+            qq = x[i, :H].double().view(KV, G, D)
+            p = torch.softmax(torch.einsum("kgd,jkd->kgj", qq, K[:m]) * D ** -0.5, -1)
+            w = torch.einsum("kgj,jkd->kgd", p, V[:m]).reshape(H, D)
+            assert (got[i] - w).abs().max() <= 1e-5, (kind, i)
+
+
 # ---- long runs of one accumulator ----------------------------------------------------------------
 @pytest.mark.parametrize("mode", ["f16", "q8"])
 @pytest.mark.parametrize("D", [128, 256])
