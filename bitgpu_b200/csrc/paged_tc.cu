@@ -159,14 +159,6 @@ struct CodeScale {
   }
 };
 
-// 1 / (1 + exp(-g)) to about 4 * 2^-24 of its value (a row's thread has head_dim of them in the epilogue, where
-// expf and a division each made a gated prompt three times as long).
-__device__ __forceinline__ float sigmoid(float g) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + ex2_approx(-kLog2e * g)));
-  return r;
-}
-
 // N consecutive words of one row.  A row belongs to one thread, so a store instruction touches 32 rows:
 // 32-byte stores fill whole sectors (16-byte ones write every sector twice: 5.5 -> 2.5 us per 256 rows).
 template <int N>

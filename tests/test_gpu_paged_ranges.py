@@ -254,6 +254,28 @@ def test_mixed_query_scales(ops, kernel, mode):  # noqa: F811
             assert ((got[t, h].double() - p @ v).abs() <= tol).all(), (t, h)
 
 
+# ---- gates ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kernel", [*KERNELS, "tc whole"])
+@pytest.mark.parametrize("mode", ["f16", "q8"])
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("low,high", [(-80, 80), (-80, -20), (-8, 8)])
+def test_gate_range(ops, kernel, mode, D, low, high):  # noqa: F811
+    """A shut gate leaves little of a value, and that little as exact as the value: beside the ungated result's
+    error 8 * 2^-24 (exp to two units in the last place, a sum, a quotient, a product)."""
+    if kernel == "tc whole":  # units that no block's border cuts: gated by the tcgen05 kernel itself
+        r = wide(Ragged([30] * 40, [30] * 40, KV=2, G=4, D=D, mode=mode, seed=1))
+    else:
+        r = make(kernel, mode, D)
+    for io in DT.values():
+        q = r.queries(io)
+        gate = low + (high - low) * torch.rand(q.shape, generator=r.g)
+        plain = attend(ops, kernel, r, q, torch.float32).double()
+        got = attend(ops, kernel, r, q, torch.float32, gate=gate.cuda()).double()
+        want = plain * torch.sigmoid(gate.double())
+        err = (got - want).abs()
+        assert (err <= 8 * 2.0 ** -24 * want.abs() + 2.0 ** -140).all(), float((err / want.abs()).max() * 2 ** 24)
+
+
 # ---- lengths beyond the page table ---------------------------------------------------------------
 @each_kernel
 @pytest.mark.parametrize("mode", ["f16", "q8"])
