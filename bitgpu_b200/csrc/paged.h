@@ -242,69 +242,67 @@ struct PieceWalk {
   }
 
   __device__ __forceinline__ bool next(Piece &p, const BatchView &bv, const UnitShape &u, uint32_t page_size) {
-    {
-      if (cur >= t1) return false;
-      uint32_t at, n, done;  // where the unit's first tile lies, its tiles, those before this block's
-      if (cur < pre) {
-        const uint32_t rows = batch_rows(bv, u.G), nch = (rows + u.RU - 1) / u.RU;
-        n = (bv.prefix_len + u.KT - 1) >> u.shift;
-        const uint32_t unit = cur / (n + u.lead);
-        at = unit * (n + u.lead) + u.lead;
-        p.kvh = unit / nch;
-        p.R0 = unit % nch * u.RU;
-        p.rows = min(u.RU, rows - p.R0);
-        p.len = bv.prefix_len;
-        p.lim_base = 0x40000000;
-        p.pages = bv.prefix_pages;
-        p.list = bv.B;
-        p.own = false;
-        if (cur < at) cur = min(at, t1);
-        if (cur >= t1) return false;  // only (some of) the lead is this block's
-        done = cur - at;
-        p.ntiles = min(n - done, t1 - cur);
-      } else {
-        const uint32_t rows = sr.n * u.G;
-        n = chunk_tiles(sr, u, ch);
-        if (in < u.lead) {
-          const uint32_t skip = min(u.lead - in, t1 - cur);
-          cur += skip;
-          in += skip;
-          if (cur >= t1) return false;
-        }
-        done = in - u.lead;
-        at = cur - done;
-        p.kvh = kvh;
-        p.R0 = sr.begin * u.G + ch * u.RU;
-        p.rows = min(u.RU, rows - ch * u.RU);
-        p.len = (uint32_t)sr.held;
-        p.lim_base = sr.len - (int32_t)sr.n - (int32_t)sr.begin;
-        p.pages = bv.table + (uint64_t)b * bv.table_stride;
-        p.list = b;
-        p.own = true;
-        p.ntiles = min(n - done, t1 - cur);
-        in += p.ntiles;
-        if (done + p.ntiles == n) {  // on to the next unit: chunk, kv head, sequence
-          in = 0;
-          if (++ch * u.RU >= rows) {
-            ch = 0;
-            if (++kvh == u.KV) {
-              kvh = 0;
-              if (cur + p.ntiles < t1) {
-                do {
-                  ++b;
-                  sr = seq_range(bv, b, page_size);
-                } while (seq_tiles(sr, u) == 0);
-              }
+    if (cur >= t1) return false;
+    uint32_t at, n, done;  // where the unit's first tile lies, its tiles, those before this block's
+    if (cur < pre) {
+      const uint32_t rows = batch_rows(bv, u.G), nch = (rows + u.RU - 1) / u.RU;
+      n = (bv.prefix_len + u.KT - 1) >> u.shift;
+      const uint32_t unit = cur / (n + u.lead);
+      at = unit * (n + u.lead) + u.lead;
+      p.kvh = unit / nch;
+      p.R0 = unit % nch * u.RU;
+      p.rows = min(u.RU, rows - p.R0);
+      p.len = bv.prefix_len;
+      p.lim_base = 0x40000000;
+      p.pages = bv.prefix_pages;
+      p.list = bv.B;
+      p.own = false;
+      if (cur < at) cur = min(at, t1);
+      if (cur >= t1) return false;  // only (some of) the lead is this block's
+      done = cur - at;
+      p.ntiles = min(n - done, t1 - cur);
+    } else {
+      const uint32_t rows = sr.n * u.G;
+      n = chunk_tiles(sr, u, ch);
+      if (in < u.lead) {
+        const uint32_t skip = min(u.lead - in, t1 - cur);
+        cur += skip;
+        in += skip;
+        if (cur >= t1) return false;
+      }
+      done = in - u.lead;
+      at = cur - done;
+      p.kvh = kvh;
+      p.R0 = sr.begin * u.G + ch * u.RU;
+      p.rows = min(u.RU, rows - ch * u.RU);
+      p.len = (uint32_t)sr.held;
+      p.lim_base = sr.len - (int32_t)sr.n - (int32_t)sr.begin;
+      p.pages = bv.table + (uint64_t)b * bv.table_stride;
+      p.list = b;
+      p.own = true;
+      p.ntiles = min(n - done, t1 - cur);
+      in += p.ntiles;
+      if (done + p.ntiles == n) {  // on to the next unit: chunk, kv head, sequence
+        in = 0;
+        if (++ch * u.RU >= rows) {
+          ch = 0;
+          if (++kvh == u.KV) {
+            kvh = 0;
+            if (cur + p.ntiles < t1) {
+              do {
+                ++b;
+                sr = seq_range(bv, b, page_size);
+              } while (seq_tiles(sr, u) == 0);
             }
           }
         }
       }
-      p.tile0 = done;
-      p.npieces = (at + n - 1) / per - at / per + 1;
-      p.starts = done == 0;
-      cur += p.ntiles;
-      return true;
     }
+    p.tile0 = done;
+    p.npieces = (at + n - 1) / per - at / per + 1;
+    p.starts = done == 0;
+    cur += p.ntiles;
+    return true;
   }
 };
 
@@ -371,7 +369,7 @@ struct PagedAttnArgs {
   PagedView kv;
   BatchView bv;
   int mode, q_f16, out_f16;
-  uint32_t H, G, D, max_q;
+  uint32_t H, G, D;
   float sl2;  // softmax scale * log2(e)
   const void *q;
   // tcgen05 kernels, rows that are not f16 in and out: q as two f16 halves [2][T][H][D] and each row's power of two

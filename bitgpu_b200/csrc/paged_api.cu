@@ -215,7 +215,6 @@ int bg_paged_attention(const bg_paged_cache *kv, const bg_paged_batch *batch, ui
   a.H = H;
   a.G = H / KV;
   a.D = D;
-  a.max_q = batch->max_q;
   a.sl2 = (scale > 0.f ? scale : 1.0f / sqrtf((float)D)) * kLog2e;
   a.q = q;
   a.gate = gate;

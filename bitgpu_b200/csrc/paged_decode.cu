@@ -188,58 +188,58 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
         ++it;
         if (t > 0) continue;
         // the first tile travels while the unit is made ready: its description and query rows
-      const int us = un % kUnits;
-      if (un >= kUnits) ok = mbar_wait_warp(&uempty[us], ((un / kUnits) - 1) & 1);
-      if (!ok) break;
-      const bool whole = pc.npieces == 1;
-      const uint32_t slot = a.slot0 + (2 * blockIdx.x + (pc.starts ? 1 : 0)) * p.u.RU;
-      if (lane == 0) {
-        UnitInfo *ui = reinterpret_cast<UnitInfo *>(smem + C::oU + us * 64);
-        ui->R0 = pc.R0;
-        ui->rows = pc.rows;
-        ui->kvh = pc.kvh;
-        ui->tile0 = pc.tile0;
-        ui->ntiles = pc.ntiles;
-        ui->len = pc.len;
-        ui->lim_base = pc.lim_base;
-        ui->dest = !whole ? slot : p.join_rows ? kRowBuf : kDirect;
-        ui->row0 = pc.own ? a.own_row0 : a.pre_row0;
-      }
-      if (p.join_rows) {
-        if (pc.starts && (uint32_t)lane < pc.rows) {  // where the row's pieces will be
-          const uint32_t R = pc.R0 + lane;
-          RowPieces rp;
-          rp.idx0 = whole ? (pc.own ? a.own_row0 : a.pre_row0) + R / a.G * a.H + pc.kvh * a.G + R % a.G : slot + lane;
-          rp.npieces = pc.npieces;
-          rp.step = p.u.RU;
-          rp.pad = 0;
-          (pc.own ? a.own_pieces : a.pre_pieces)[(uint64_t)pc.kvh * a.bv.T * a.G + R] = rp;
+        const int us = un % kUnits;
+        if (un >= kUnits) ok = mbar_wait_warp(&uempty[us], ((un / kUnits) - 1) & 1);
+        if (!ok) break;
+        const bool whole = pc.npieces == 1;
+        const uint32_t slot = a.slot0 + (2 * blockIdx.x + (pc.starts ? 1 : 0)) * p.u.RU;
+        if (lane == 0) {
+          UnitInfo *ui = reinterpret_cast<UnitInfo *>(smem + C::oU + us * 64);
+          ui->R0 = pc.R0;
+          ui->rows = pc.rows;
+          ui->kvh = pc.kvh;
+          ui->tile0 = pc.tile0;
+          ui->ntiles = pc.ntiles;
+          ui->len = pc.len;
+          ui->lim_base = pc.lim_base;
+          ui->dest = !whole ? slot : p.join_rows ? kRowBuf : kDirect;
+          ui->row0 = pc.own ? a.own_row0 : a.pre_row0;
         }
-      } else if (!whole && pc.starts && lane == 0) {
-        a.cuts[blockIdx.x] = CutUnit{pc.R0, pc.rows, pc.kvh, pc.npieces};
-      }
-      {
-        const uint32_t cpr = a.q_f16 ? D / 8 : D / 4;  // 16-byte chunks per query row
-        const uint32_t qb = smem_u32(smem + C::oQ + us * C::QSLOT);
-        const uint32_t stride = a.q_f16 ? D * 2 + 16 : C::QROW;
-        const uint32_t tok0 = pc.R0 / a.G, g0 = pc.R0 % a.G;
-        for (uint32_t idx = lane; idx < NN * cpr; idx += 32) {
-          const uint32_t r = idx / cpr, c = idx % cpr;
-          uint32_t tok = tok0, g = g0 + r;
-          while (g >= a.G) {
-            g -= a.G;
-            ++tok;
+        if (p.join_rows) {
+          if (pc.starts && (uint32_t)lane < pc.rows) {  // where the row's pieces will be
+            const uint32_t R = pc.R0 + lane;
+            RowPieces rp;
+            rp.idx0 = whole ? (pc.own ? a.own_row0 : a.pre_row0) + R / a.G * a.H + pc.kvh * a.G + R % a.G : slot + lane;
+            rp.npieces = pc.npieces;
+            rp.step = p.u.RU;
+            rp.pad = 0;
+            (pc.own ? a.own_pieces : a.pre_pieces)[(uint64_t)pc.kvh * a.bv.T * a.G + R] = rp;
           }
-          const bool there = r < pc.rows;
-          const uint64_t off = there ? ((uint64_t)tok * a.H + pc.kvh * a.G + g) * cpr + c : 0;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(qb + r * stride + c * 16),
-                       "l"(static_cast<const uint4 *>(a.q) + off), "r"(there ? 16u : 0u)
-                       : "memory");
+        } else if (!whole && pc.starts && lane == 0) {
+          a.cuts[blockIdx.x] = CutUnit{pc.R0, pc.rows, pc.kvh, pc.npieces};
         }
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ufull[us])) : "memory");
-        if (lane == 0) mbar_arrive(&ufull[us]);
-      }
-      ++un;
+        {
+          const uint32_t cpr = a.q_f16 ? D / 8 : D / 4;  // 16-byte chunks per query row
+          const uint32_t qb = smem_u32(smem + C::oQ + us * C::QSLOT);
+          const uint32_t stride = a.q_f16 ? D * 2 + 16 : C::QROW;
+          const uint32_t tok0 = pc.R0 / a.G, g0 = pc.R0 % a.G;
+          for (uint32_t idx = lane; idx < NN * cpr; idx += 32) {
+            const uint32_t r = idx / cpr, c = idx % cpr;
+            uint32_t tok = tok0, g = g0 + r;
+            while (g >= a.G) {
+              g -= a.G;
+              ++tok;
+            }
+            const bool there = r < pc.rows;
+            const uint64_t off = there ? ((uint64_t)tok * a.H + pc.kvh * a.G + g) * cpr + c : 0;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(qb + r * stride + c * 16),
+                         "l"(static_cast<const uint4 *>(a.q) + off), "r"(there ? 16u : 0u)
+                         : "memory");
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ufull[us])) : "memory");
+          if (lane == 0) mbar_arrive(&ufull[us]);
+        }
+        ++un;
       }
     }
     // the end: a unit without tiles
