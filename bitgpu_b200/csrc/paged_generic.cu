@@ -9,8 +9,9 @@
 // eight positions at a time: each lane multiplies its head_dim / 32 dims for the 8 x 4 (position, head)
 // pairs, and the 32 partial dots are reduced together -- five exchange steps that halve the number of
 // values, 31 shuffles for 32 sums -- which leaves pair (head = lane / 8, position = lane % 8) in its
-// own lane, where the running maximum and sum of the softmax are kept.  Bound: HBM for f32 caches
-// (1 KB per position and kv head at head_dim 128 against about 450 issue slots for 8 positions).
+// own lane, where the running maximum and sum of the softmax are kept.  Bound: issue (about 450 slots for 8
+// positions of head_dim 128): 32 streams of up to 8192 positions over an f32 pool 478 us, 2.2 TB/s, a third of the copy's
+// rate; head_dim 64 366 us (f16 371, q8 851).  Nothing is shared between tokens: one prompt of 2048 takes 3510 us.
 #include "paged.h"
 #include "paged_merge.cuh"
 

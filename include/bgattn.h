@@ -213,7 +213,8 @@ int bg_qk_norm_rope(const float *x, uint32_t batch, uint32_t S, uint32_t heads, 
  * positions 0 .. prefix_len-1 in front of its own, held in prefix_pages[j / page_size].
  * cu_q (not decreasing), kv_len, page_table and prefix_pages are read on the device, so a captured
  * graph follows them; batch, tokens, max_q (the largest number of tokens of a sequence: it selects
- * kernels, results do not depend on it), the table's width and prefix_len are fixed by the call.
+ * kernels, on which results depend by their rounding alone), the table's width and prefix_len are fixed by
+ * the call.
  *   - Token rows at or behind cu_q[batch] are padding: their outputs are left as they were.
  *   - A token whose o is negative has no position: the append skips it, attention gives it the prefix
  *     alone (zeros without one).
