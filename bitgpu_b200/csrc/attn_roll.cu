@@ -517,6 +517,7 @@ __global__ void __launch_bounds__(RCfg<MODE, HPC>::THREADS, 1)
       for (int u = 0; u < NSUB; ++u)
         tile_pv(smem_u32(smem + st[u] * C::STAGE),
                 reinterpret_cast<const float *>(smem + st[u] * C::STAGE + 2 * C::KVT), tl[u].n, pr[u]);
+      __threadfence_block();  // as release_read, for both stages
       __syncwarp();
       if (lane == 0)
 #pragma unroll

@@ -695,8 +695,7 @@ __global__ void __launch_bounds__(160, (MODE == BG_KV_Q8 && NT == 1 && D == 128 
         }
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[s]);
+    release_read(&empty[s]);
   }
 
 #ifdef BG_TRACE

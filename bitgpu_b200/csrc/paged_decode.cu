@@ -574,8 +574,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
+      release_read(&empty[s]);
     }
 
     // ---- the four warps' states meet ----
@@ -658,8 +657,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<MODE, D, NT>::CTAS)
         if (d == 0) a.part_ml[idx_p] = make_float2(mrow[n], lrow_s[n]);
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&uempty[us]);
+    release_read(&uempty[us]);
     if (!meet_all()) return;  // mw .. and e0 are free again
   }
 }

@@ -582,9 +582,8 @@ __global__ void __launch_bounds__(TcCfg<D, Q8, LO, NQT>::THREADS, 1)
       for (uint32_t piece = 0;; ++piece) {
         if (!mbar_wait_warp(q_full, piece & 1)) { ok = false; break; }
         const TcInfo in = *info;
-        __syncwarp();
         if (in.ntiles == 0) break;
-        if (lane == 0) mbar_arrive(info_free);
+        release_read(info_free);
         const uint32_t r = (NQT == 2 ? t * p.rpt : 0) + row;
         const uint32_t R = in.R0 + min(r, in.rows - 1);
         const int lim = min(in.lim_base + (int)(R / a.G), (int)in.len - 1);

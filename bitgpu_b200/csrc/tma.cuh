@@ -33,6 +33,16 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// Whole warp: a buffer that it has read goes back to its producer.  Every lane's reads have to be performed before the
+// arrive that lets the buffer be overwritten, which __syncwarp() alone does not see to: a decode kernel whose code had
+// changed elsewhere gave wrong values in a tile's last blocks in one call of six, and none of 600 with the fence.  It
+// costs nothing measurable beside a tile.
+__device__ __forceinline__ void release_read(uint64_t *bar) {
+  __threadfence_block();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
