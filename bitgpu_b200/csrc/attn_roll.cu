@@ -305,6 +305,8 @@ __global__ void __launch_bounds__(RCfg<MODE, HPC>::THREADS, 1)
 
     float m[2] = {kNegBig, kNegBig}, l[2] = {0.f, 0.f};
     float oacc[KS][4];
+    BlockPow<NB> vpow;  // q8
+    vpow.reset();
 #pragma unroll
     for (int mt = 0; mt < KS; ++mt)
 #pragma unroll
@@ -446,8 +448,9 @@ __global__ void __launch_bounds__(RCfg<MODE, HPC>::THREADS, 1)
         const int sa_i = (warp * TP + ra) * NB, sb_i = (warp * TP + ra + 8) * NB;
 #pragma unroll
         for (int bk = 0; bk < NB; ++bk) {
-          const float va = vsc[sa_i + bk] * (1.0f / 127.0f);  // zero-filled past the tile
-          const float vbb = vsc[sb_i + bk] * (1.0f / 127.0f);
+          const float up = vpow.inv[bk];
+          const float va = vsc[sa_i + bk] * up;  // zero-filled past the tile
+          const float vbb = vsc[sb_i + bk] * up;
           const uint32_t pb0 = movm_t(pack_f16(pr[0] * va, pr[1] * va));
           const uint32_t pb1 = movm_t(pack_f16(pr[2] * vbb, pr[3] * vbb));
           uint32_t r[4];
@@ -472,6 +475,26 @@ __global__ void __launch_bounds__(RCfg<MODE, HPC>::THREADS, 1)
     // column for up to 32 slots, and two independent score chains in flight.
     auto step = [&](auto nsub_c, const uint32_t (&cu)[2], const Tile (&tl)[2], const int (&st)[2]) {
       constexpr int NSUB = decltype(nsub_c)::value;
+      if constexpr (MODE == BG_KV_Q8) {
+        // (here, where the wait ends a block of code anyway: between softmax and output it costs 3 % more)
+        const float *ya[NSUB];
+        bool above = false;
+#pragma unroll
+        for (int u = 0; u < NSUB; ++u) {
+          ya[u] = reinterpret_cast<const float *>(smem + st[u] * C::STAGE + 2 * C::KVT) + TP * HPC * NB + (warp * TP + ra) * NB;
+          above |= vpow.above(ya[u], ya[u] + 8 * NB, lane);
+        }
+        if (__any_sync(0xffffffffu, above))
+#pragma unroll
+          for (int u = 0; u < NSUB; ++u)
+            vpow.admit(ya[u], ya[u] + 8 * NB, lane, [&](int bk, float f) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                oacc[2 * bk][i] *= f;
+                oacc[2 * bk + 1][i] *= f;
+              }
+            });
+      }
       float acc[NSUB][4];
 #pragma unroll
       for (int u = 0; u < NSUB; ++u)
@@ -567,7 +590,7 @@ __global__ void __launch_bounds__(RCfg<MODE, HPC>::THREADS, 1)
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
             const int d = MODE == BG_KV_F16 ? mt * 16 + (lane >> 2) + 8 * hh : mt * 16 + 2 * (lane >> 2) + hh;
-            float v = ok ? oacc[mt][2 * hh + j] * inv : 0.f;
+            float v = ok ? oacc[mt][2 * hh + j] * (MODE == BG_KV_Q8 ? inv * vpow.back(mt / 2) : inv) : 0.f;
             if (p.gate) v = v / (1.0f + expf(-p.gate[grow * kD + d]));
             if (p.out_f16) static_cast<__half *>(p.out)[grow * kD + d] = __float2half_rn(v);
             else static_cast<float *>(p.out)[grow * kD + d] = v;
@@ -581,7 +604,7 @@ __global__ void __launch_bounds__(RCfg<MODE, HPC>::THREADS, 1)
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const int d = MODE == BG_KV_F16 ? mt * 16 + (lane >> 2) + 8 * hh : mt * 16 + 2 * (lane >> 2) + hh;
-          dst[d] = ok ? oacc[mt][2 * hh + j] : 0.f;
+          dst[d] = ok ? oacc[mt][2 * hh + j] * (MODE == BG_KV_Q8 ? vpow.back(mt / 2) : 1.f) : 0.f;
         }
       }
       if (lane < 4) {

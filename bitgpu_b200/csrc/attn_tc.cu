@@ -15,7 +15,8 @@
 //     score accumulator of a warp is converted to the P^T operand in registers with movmatrix;
 //   * q8: codes enter the MMA as exact f16 integers.  The K block scale (one per 32 values) is
 //     applied per block accumulator after the MMA, and the V block scale is folded into P before
-//     its f16 conversion, so the q8 math stays exact up to f32/f16 operand rounding of q and p.
+//     its f16 conversion, a power of two per block taken out (scales are f32, f16 ends at 2^-24), so the
+//     q8 math stays exact up to f32/f16 operand rounding of q and p.
 // Online softmax in log2 units; the four warps' states are merged in shared memory and written as
 // split partials [split][row][D+2] for the LSE merge kernel (shared with the generic path).
 #include <cuda.h>
@@ -384,6 +385,8 @@ __global__ void __launch_bounds__(160, (MODE == BG_KV_Q8 && NT == 1 && D == 128 
 
   float m[NT][2], l[NT][2];
   float oacc[NT][KS][4];
+  BlockPow<NB> vpow;  // q8
+  vpow.reset();
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     m[nt][0] = m[nt][1] = kNegBig;
@@ -419,7 +422,6 @@ __global__ void __launch_bounds__(160, (MODE == BG_KV_Q8 && NT == 1 && D == 128 
     const uint32_t kb = sb, vb = sb + C::KVT;
     const int row0 = warp * 16;
     const uint32_t pa = lo + t * TP + row0 + (lane >> 2), pb = pa + 8;
-
 
     // ---- scores S^T[pos][n] ----
     float sc[NT][4];
@@ -666,10 +668,21 @@ __global__ void __launch_bounds__(160, (MODE == BG_KV_Q8 && NT == 1 && D == 128 
       }
     } else {
       const float *vsc = reinterpret_cast<const float *>(smem + s * C::STAGE + 2 * C::KVT + C::SCT);
+      const float *ya = vsc + (row0 + (lane >> 2)) * NB, *yb = ya + 8 * NB;
+      if (__any_sync(0xffffffffu, vpow.above(ya, yb, lane)))
+        vpow.admit(ya, yb, lane, [&](int bk, float f) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              oacc[nt][2 * bk][i] *= f;
+              oacc[nt][2 * bk + 1][i] *= f;
+            }
+        });
 #pragma unroll
       for (int bk = 0; bk < NB; ++bk) {
-        const float va = vsc[(row0 + (lane >> 2)) * NB + bk] * (1.0f / 127.0f);
-        const float vbb = vsc[(row0 + (lane >> 2) + 8) * NB + bk] * (1.0f / 127.0f);
+        const float up = vpow.inv[bk];
+        const float va = ya[bk] * up, vbb = yb[bk] * up;
         uint32_t pb0[NT], pb1[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -754,7 +767,7 @@ __global__ void __launch_bounds__(160, (MODE == BG_KV_Q8 && NT == 1 && D == 128 
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
           const int d = MODE == BG_KV_F16 ? mt * 16 + (lane >> 2) + 8 * hh : mt * 16 + 2 * (lane >> 2) + hh;
-          mine[d] = oacc[nt][mt][2 * hh + j] * f;
+          mine[d] = oacc[nt][mt][2 * hh + j] * (MODE == BG_KV_Q8 ? f * vpow.back(mt / 2) : f);
         }
       }
     }

@@ -109,6 +109,13 @@ __device__ __forceinline__ int8_t snorm8_encode(float v, float s) {
   return (int8_t)(int)floorf(0.5f + 127.0f * e);
 }
 
+// The power of two that values below 2^(x + 1) are freed of to stay below 2^14 (x: the exponent in `bits`; at least
+// 2^-126), and its inverse.
+__device__ __forceinline__ float pow2_of(uint32_t bits) {
+  return __uint_as_float((uint32_t)max((int)(bits & 0x7f800000u) - (13 << 23), 1 << 23));
+}
+__device__ __forceinline__ float pow2_inv(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

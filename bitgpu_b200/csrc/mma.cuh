@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "common.cuh"
+
 namespace bg {
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -50,6 +52,50 @@ __device__ __forceinline__ uint32_t kNeg1152x2() {
   __half2 h = __half2(__float2half_rn(-1152.f), __float2half_rn(-1152.f));
   return *reinterpret_cast<uint32_t *>(&h);
 }
+
+// Weights p * block scale as one f16, whatever the scales' magnitude: a warp keeps each 32-channel block's output
+// divided by a power of two, so that scales (p is at most 1) times inv[block] stay below 2^15 / 127.  above() says
+// whether a tile's would not (one vote for all blocks, each lane looks at its two rows' blocks of its place in the
+// quad); admit() then lets `down` scale the block's output so far to the next power.  ya, yb: a lane's rows of scales.
+template <int NB>
+struct BlockPow {
+  float inv[NB];       // the inverse power over 127
+  float lim[NB / 4];   // scales that are too large, of blocks lane % 4, + 4
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) inv[b] = 0x1p126f * (1.0f / 127.0f);
+#pragma unroll
+    for (int q = 0; q < NB / 4; ++q) lim[q] = 0x1p-111f;
+  }
+  // The power's inverse itself (inv is 2^(k - 7) times 1.00..).
+  __device__ __forceinline__ float exact(int b) const {
+    return __uint_as_float((__float_as_uint(inv[b]) & 0x7f800000u) + (7u << 23));
+  }
+  __device__ __forceinline__ bool above(const float *ya, const float *yb, uint32_t lane) const {
+    bool is = false;
+#pragma unroll
+    for (int q = 0; q < NB / 4; ++q) {
+      const int b = 4 * q + (lane & 3);
+      is |= fmaxf(fabsf(ya[b]), fabsf(yb[b])) >= lim[q];
+    }
+    return is;
+  }
+  template <typename F>
+  __device__ __forceinline__ void admit(const float *ya, const float *yb, uint32_t lane, F down) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(ya[b]), fabsf(yb[b]))));
+      const float was = exact(b);
+      if (__uint_as_float(bits) * was < 32768.f) continue;
+      const float now = pow2_inv(pow2_of(bits));
+      down(b, now * pow2_inv(was));
+      inv[b] = now * (1.0f / 127.0f);
+      lim[b / 4] = (lane & 3) == (b & 3) ? 32768.f * pow2_inv(now) : lim[b / 4];
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ float back(int b) const { return pow2_inv(exact(b)); }
+};
 
 // Shared-memory byte address of 16-byte chunk `gc` of tile row `row` (128B-swizzled column blocks
 // of TP rows each, the layout TMA writes with CU_TENSOR_MAP_SWIZZLE_128B).

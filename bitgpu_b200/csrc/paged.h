@@ -306,13 +306,6 @@ struct PieceWalk {
   }
 };
 
-// The power of two that values below 2^(x + 1) are freed of to stay below 2^14 (x: the exponent in `bits`; at least
-// 2^-126), and its inverse.
-__device__ __forceinline__ float pow2_of(uint32_t bits) {
-  return __uint_as_float((uint32_t)max((int)(bits & 0x7f800000u) - (13 << 23), 1 << 23));
-}
-__device__ __forceinline__ float pow2_inv(float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
-
 // Where a unit's rows wait to be joined.  Without a prefix only cut units leave any: one CutUnit per
 // block (npieces 0: none).  With a prefix every row joins two lists of pieces: one RowPieces per (kv
 // head, R) and part; piece 0 is partial row idx0, piece k row idx0 + (2k - 1) * step.
